@@ -14,7 +14,16 @@ SRC = [os.path.join(_HERE, 'hip', 'mgproto_kernels.hip'),
        os.path.join(_HERE, 'hip', 'fused_bn.hip'),
        os.path.join(_HERE, 'hip', 'em_kernels.hip'),
        os.path.join(_HERE, 'hip', 'enqueue_kernels.hip'),
-       os.path.join(_HERE, 'hip', 'gemm1x1_kernels.hip')]
+       os.path.join(_HERE, 'hip', 'gemm1x1_kernels.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_quant.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_linear.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_grad.hip'),
+       os.path.join(_HERE, 'hip', 'grad_clip.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_bindings.hip')]
+# no packed fp32 instructions: some of their forms give wrong results on this
+# hardware now and then (hipcc's host pass warns that it has no such feature)
+HIP_FLAGS = ['-O3', '-Xclang', '-target-feature', '-Xclang',
+             '-packed-fp32-ops']
 OUT = os.path.join(_HERE, '_mgproto_hip.so')
 CPU_SRC = [os.path.join(_HERE, 'cpu', 'fastaug.cpp')]
 CPU_OUT = os.path.join(_HERE, '_mgproto_cpu.so')
@@ -45,7 +54,7 @@ def build(verbose: bool = False) -> str:
                sources=SRC,
                build_directory=build_dir,
                extra_cflags=['-O3'],
-               extra_cuda_cflags=['-O3'],
+               extra_cuda_cflags=HIP_FLAGS,
                verbose=verbose,
                is_python_module=True)
     built = os.path.join(build_dir, '_mgproto_hip.so')
