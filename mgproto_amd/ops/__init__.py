@@ -317,3 +317,8 @@ def argmax_hw(probs: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
             return vals, idx.to(torch.long)
     vals, idx = probs.max(dim=1)
     return vals, idx
+
+
+from .gradclip import clip_grads_, grad_norm  # noqa: E402,F401
+from .mx4 import (MX4Tensor, mx4_dequantize, mx4_linear,  # noqa: E402,F401
+                  mx4_quantize)

@@ -1,0 +1,193 @@
+// Shared by the MX4 kernels: types, the block rounding, the launchers.
+//
+// MX4 (OCP Microscaling Formats v1.0, MXFP4): 32 consecutive elements of a
+// row share a power-of-two scale, each element is one of
+// {0, .5, 1, 1.5, 2, 3, 4, 6} with a sign:
+//   E = clamp(floor(log2 max|x|) - 2, -127, 127), byte = E + 127
+//   q = x * 2^-E to the nearest value, ties to the even code, 6 at most.
+// A block with a NaN or an infinity has byte 255 and reads as NaN.
+//
+// Storage: rows padded to Kp = multiple of 128 elements (one matrix-core
+// step), codes [rows, Kp/2] with the low nibble first, scales [rows, Kp/32].
+// Codes and scales of the padding are 0, so it adds nothing to a product.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <cstdint>
+
+namespace mx4 {
+
+enum DType : int { F32 = 0, BF16 = 1, F16 = 2 };
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <int DT> struct Elem;
+template <> struct Elem<F32> { using T = float; };
+template <> struct Elem<BF16> { using T = __bf16; };
+template <> struct Elem<F16> { using T = _Float16; };
+
+// one rounding, to nearest even
+template <int DT>
+static __device__ __forceinline__ typename Elem<DT>::T from_f32(float v) {
+    return (typename Elem<DT>::T)v;
+}
+
+// 2^(byte-127) as a float; 2^-127 lies below the normal numbers. Byte 255
+// gives an infinity here, callers deal with it before.
+static __device__ __forceinline__ float scale_f32(unsigned byte) {
+    return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+
+// The 32 elements of one block as they are loaded: 16 words of two 16-bit
+// elements, or 32 words.
+template <int DT> struct Raw32 { u32x4 u[DT == F32 ? 8 : 4]; };
+
+// max|x| of packed 16-bit floats by their bits (the order of the absolute
+// bits is the order of the values, infinities and NaN on top)
+static __device__ __forceinline__ u16x2 absmax16(u16x2 m, unsigned w) {
+    w &= 0x7fff7fffu;
+    return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w));
+}
+
+template <int DT>
+static __device__ __forceinline__ unsigned absmax_bits(const u32x4* u, int n4) {
+    if constexpr (DT == F32) {
+        unsigned m = 0;
+        #pragma unroll
+        for (int i = 0; i < n4; ++i)
+            #pragma unroll
+            for (int j = 0; j < 4; ++j)
+                m = max(m, u[i][j] & 0x7fffffffu);
+        return m;
+    } else {
+        u16x2 m = {0, 0};
+        #pragma unroll
+        for (int i = 0; i < n4; ++i)
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) m = absmax16(m, u[i][j]);
+        return max((unsigned)m.x, (unsigned)m.y);
+    }
+}
+
+// scale byte of a block from the bits of its absolute maximum
+template <int DT>
+static __device__ __forceinline__ unsigned scale_byte(unsigned bits) {
+    unsigned e;
+    if constexpr (DT == F32) {
+        if (bits >= 0x7f800000u) return 255u;
+        e = bits >> 23;
+    } else if constexpr (DT == BF16) {
+        if (bits >= 0x7f80u) return 255u;
+        e = bits >> 7;
+    } else {
+        if (bits >= 0x7c00u) return 255u;
+        // exact in fp32, where fp16's subnormal numbers are normal
+        e = __float_as_uint((float)__builtin_bit_cast(
+                _Float16, (unsigned short)bits)) >> 23;
+    }
+    return e > 2u ? e - 2u : 0u;   // (e - 127) - 2 + 127, at least 0
+}
+
+// (by value: a bit cast of a vector's element in place takes the first one)
+static __device__ __forceinline__ bf16x2 as_bf16x2(unsigned w) {
+    return __builtin_bit_cast(bf16x2, w);
+}
+static __device__ __forceinline__ f16x2 as_f16x2(unsigned w) {
+    return __builtin_bit_cast(f16x2, w);
+}
+
+// 8 elements (one 16-byte word of 16-bit floats, two of fp32) to 8 codes.
+// The conversion instructions divide by the scale, round to nearest even and
+// saturate at 6; checked value by value, subnormal scale included.
+template <int DT>
+static __device__ __forceinline__ unsigned codes8(const u32x4* u, float s) {
+    unsigned r = 0;
+    if constexpr (DT == F32) {
+        const u32x4 a = u[0], b = u[1];
+        #define MX4_F(i) __uint_as_float(i)
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, MX4_F(a.x), MX4_F(a.y), s, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, MX4_F(a.z), MX4_F(a.w), s, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, MX4_F(b.x), MX4_F(b.y), s, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, MX4_F(b.z), MX4_F(b.w), s, 3);
+        #undef MX4_F
+    } else if constexpr (DT == BF16) {
+        const u32x4 a = u[0];
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_bf16x2(a.x), s, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_bf16x2(a.y), s, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_bf16x2(a.z), s, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, as_bf16x2(a.w), s, 3);
+    } else {
+        const u32x4 a = u[0];
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_f16x2(a.x), s, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_f16x2(a.y), s, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_f16x2(a.z), s, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, as_f16x2(a.w), s, 3);
+    }
+    return r;
+}
+
+// n <= 8 elements at p, the rest zero, as codes8 takes them
+template <int DT>
+static __device__ __forceinline__ void load8_tail(
+        const typename Elem<DT>::T* p, int n, u32x4* u) {
+    if constexpr (DT == F32) {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
+            u[i >> 2][i & 3] = i < n ? __float_as_uint(p[i]) : 0u;
+    } else {
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned lo = 2 * i < n ? q[2 * i] : 0;
+            const unsigned hi = 2 * i + 1 < n ? q[2 * i + 1] : 0;
+            u[0][i] = lo | (hi << 16);
+        }
+    }
+}
+
+// Everything below takes element strides in elements, code and scale rows as
+// Kp/2 and Kp/32 bytes, and runs on `stream`. Sizes are checked by callers.
+
+void quantize(const void* x, int dt, long rows, long K, long ldx,
+              uint8_t* codes, uint8_t* scales, hipStream_t stream);
+
+void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
+                long K, void* out, int dt, hipStream_t stream);
+
+// y[M,N] = Q(x) W^T + bias, x rounded on the way
+void linear(const void* x, int dt, long M, long K, long ldx,
+            const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
+            int bias_dt, void* y, hipStream_t stream);
+
+// the same from rows that are held in 4 bits already
+void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
+              const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
+              int bias_dt, void* y, int dt, hipStream_t stream);
+
+// dx[M,K] = g[M,N] W[N,K] and dw[N,K] = g[M,N]^T X[M,K]; each states the
+// bytes of workspace that it wants
+size_t grad_input_bytes(long M, long N, long K, int g_dt, bool g_aligned);
+void grad_input(const void* g, int g_dt, bool g_aligned, long M, long N,
+                long K, const uint8_t* wc, const uint8_t* ws, void* dx,
+                int dx_dt, void* work, hipStream_t stream);
+size_t grad_weight_bytes(long M, long N, long K, int g_dt);
+void grad_weight(const void* g, int g_dt, long M, long N, long K,
+                 const uint8_t* xc, const uint8_t* xs, void* dw, int dw_dt,
+                 void* work, hipStream_t stream);
+
+// out[n] = sum_m g[m,n]
+size_t col_sum_bytes(long M, long N);
+void col_sum(const void* g, int g_dt, long M, long N, void* out, int out_dt,
+             void* work, hipStream_t stream);
+
+}  // namespace mx4

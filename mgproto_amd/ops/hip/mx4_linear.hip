@@ -1,0 +1,221 @@
+// Products of 4-bit rows: y[M,N] = Q(x)[M,K] W[N,K]^T + bias.
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 takes, in each lane, 32 consecutive codes
+// of one row and their scale byte: lane l holds row l&15, block l>>4 of a
+// 128-step. That is one MX block a lane, so x can be rounded where it is
+// loaded, with no word exchanged between lanes. Sums are fp32; y is rounded
+// once.
+//
+// The weights are the first operand, so that a lane ends up with consecutive
+// columns of y: output row (lane>>4)*4 + r of a tile is mapped to column
+// (lane>>4)*4*FN + j*4 + r of the wave's 16*FN, 4*FN in one piece.
+
+#include <hip/hip_runtime.h>
+
+#include "mx4_common.h"
+
+namespace mx4 {
+namespace {
+
+constexpr int CODES = -1;     // x is held in 4 bits already
+
+static __device__ __forceinline__ float load_any(const void* p, int dt, long i) {
+    if (dt == F32) return reinterpret_cast<const float*>(p)[i];
+    if (dt == BF16) return (float)reinterpret_cast<const __bf16*>(p)[i];
+    return (float)reinterpret_cast<const _Float16*>(p)[i];
+}
+
+static __device__ __forceinline__ i32x8 wide(i32x4 v) {
+    return (i32x8){v.x, v.y, v.z, v.w, 0, 0, 0, 0};
+}
+
+// One block of x: loaded, rounded; codes and scale byte stay in this lane.
+template <int DT, bool VEC>
+static __device__ __forceinline__ i32x4 round_block(
+        const typename Elem<DT>::T* row, int kb, int K, int& byte) {
+    constexpr int W = DT == F32 ? 2 : 1;
+    u32x4 u[4 * W];
+    if (VEC && kb + 32 <= K) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(row + kb);
+        #pragma unroll
+        for (int i = 0; i < 4 * W; ++i) u[i] = p[i];
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i)
+            load8_tail<DT>(row + kb + i * 8, K - kb - i * 8, u + i * W);
+    }
+    byte = (int)scale_byte<DT>(absmax_bits<DT>(u, 4 * W));
+    const float s = scale_f32((unsigned)byte);
+    i32x4 c;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = (int)codes8<DT>(u + i * W, s);
+    return c;
+}
+
+// FM x FN tiles of 16x16 a wave. WK = 1: the four waves lie 2 x 2; WK = 4:
+// they share one tile and take every fourth step each, joined in LDS.
+template <int AT, bool VEC, int OT, int FM, int FN, int WK>
+__global__ __launch_bounds__(256)
+void linear_direct_kernel(const void* __restrict__ xv,
+                          const uint8_t* __restrict__ xs, long M, int K,
+                          int Kp, long ldx, const uint8_t* __restrict__ wc,
+                          const uint8_t* __restrict__ ws, long N,
+                          const void* __restrict__ bias, int bias_dt,
+                          typename Elem<OT>::T* __restrict__ y) {
+    using T = typename Elem<OT>::T;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r16 = lane & 15, g = lane >> 4;
+    constexpr int TM = 16 * FM, TN = 16 * FN;
+    const long m0 = WK == 1 ? (long)blockIdx.x * (2 * TM) + (wave >> 1) * TM
+                            : (long)blockIdx.x * TM;
+    const long n0 = WK == 1 ? (long)blockIdx.y * (2 * TN) + (wave & 1) * TN
+                            : (long)blockIdx.y * TN;
+    const int cb = Kp >> 1, sb = Kp >> 5;        // bytes of a row
+
+    const uint8_t* wrow[FN];
+    const uint8_t* wsrow[FN];
+    #pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const long n = min(n0 + (r16 >> 2) * (4 * FN) + j * 4 + (r16 & 3), N - 1);
+        wrow[j] = wc + n * cb + g * 16;
+        wsrow[j] = ws + n * sb + g;
+    }
+    long xrow[FM];
+    #pragma unroll
+    for (int i = 0; i < FM; ++i) xrow[i] = min(m0 + i * 16 + r16, M - 1);
+
+    f32x4 acc[FM][FN];
+    #pragma unroll
+    for (int i = 0; i < FM; ++i)
+        #pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
+
+    const int steps = Kp >> 7;
+    for (int s = WK == 1 ? 0 : wave; s < steps; s += WK) {
+        i32x4 w[FN], x[FM];
+        int wb[FN], xb[FM];
+        #pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            w[j] = *reinterpret_cast<const i32x4*>(wrow[j] + s * 64);
+            wb[j] = wsrow[j][s * 4];
+        }
+        #pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            if constexpr (AT == CODES) {
+                const uint8_t* xc = reinterpret_cast<const uint8_t*>(xv);
+                x[i] = *reinterpret_cast<const i32x4*>(
+                    xc + xrow[i] * cb + s * 64 + g * 16);
+                xb[i] = xs[xrow[i] * sb + s * 4 + g];
+            } else {
+                using E = typename Elem<AT == CODES ? F32 : AT>::T;
+                x[i] = round_block<AT == CODES ? F32 : AT, VEC>(
+                    reinterpret_cast<const E*>(xv) + xrow[i] * ldx,
+                    s * 128 + g * 32, K, xb[i]);
+            }
+        }
+        #pragma unroll
+        for (int i = 0; i < FM; ++i)
+            #pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    wide(w[j]), wide(x[i]), acc[i][j], 4, 4, 0, wb[j], 0, xb[i]);
+    }
+
+    if constexpr (WK > 1) {      // joined in the order of the waves
+        __shared__ f32x4 part[WK - 1][FM * FN][64];
+        if (wave) {
+            #pragma unroll
+            for (int i = 0; i < FM; ++i)
+                #pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    part[wave - 1][i * FN + j][lane] = acc[i][j];
+        }
+        __syncthreads();
+        if (wave) return;
+        #pragma unroll
+        for (int p = 0; p < WK - 1; ++p)
+            #pragma unroll
+            for (int i = 0; i < FM; ++i)
+                #pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] += part[p][i * FN + j][lane];
+    }
+
+    const bool vec = N % 4 == 0;                 // y starts on 16 bytes
+    #pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const long n = n0 + g * (4 * FN) + j * 4;
+        float b[4];
+        #pragma unroll
+        for (int r = 0; r < 4; ++r)
+            b[r] = bias && n + r < N ? load_any(bias, bias_dt, n + r) : 0.f;
+        #pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const long m = m0 + i * 16 + r16;
+            if (m >= M || n >= N) continue;
+            T* q = y + m * N + n;
+            union { T v[4]; u32x2 u[sizeof(T) / 2]; } o;
+            #pragma unroll
+            for (int r = 0; r < 4; ++r)
+                o.v[r] = from_f32<OT>(acc[i][j][r] + b[r]);
+            if (vec) {
+                #pragma unroll
+                for (int r = 0; r < (int)sizeof(T) / 2; ++r)
+                    reinterpret_cast<u32x2*>(q)[r] = o.u[r];
+            } else {
+                #pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (n + r < N) q[r] = o.v[r];
+            }
+        }
+    }
+}
+
+template <int AT, bool VEC, int OT>
+void launch_direct(const void* x, const uint8_t* xs, long M, long K, long ldx,
+                   const uint8_t* wc, const uint8_t* ws, long N,
+                   const void* bias, int bias_dt, void* y, hipStream_t stream) {
+    const int Kp = (int)((K + 127) / 128 * 128);
+    #define MX4_L(FM, FN, WK) do { \
+        const int tm = (WK == 1 ? 32 : 16) * FM, tn = (WK == 1 ? 32 : 16) * FN; \
+        hipLaunchKernelGGL((linear_direct_kernel<AT, VEC, OT, FM, FN, WK>), \
+            dim3((unsigned)((M + tm - 1) / tm), (unsigned)((N + tn - 1) / tn)), \
+            dim3(256), 0, stream, x, xs, M, (int)K, Kp, ldx, wc, ws, N, bias, \
+            bias_dt, (typename Elem<OT>::T*)y); } while (0)
+    if (M <= 16) MX4_L(1, 1, 4);
+    else if (M * N <= 1024L * 1024) MX4_L(2, 2, 4);
+    else MX4_L(2, 4, 1);
+    #undef MX4_L
+}
+
+}  // namespace
+
+void linear(const void* x, int dt, long M, long K, long ldx,
+            const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
+            int bias_dt, void* y, hipStream_t stream) {
+    const int es = dt == F32 ? 4 : 2;
+    const bool vec = (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0;
+    #define MX4_ARGS x, nullptr, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream
+    if (vec) {
+        if (dt == F32) launch_direct<F32, true, F32>(MX4_ARGS);
+        else if (dt == BF16) launch_direct<BF16, true, BF16>(MX4_ARGS);
+        else launch_direct<F16, true, F16>(MX4_ARGS);
+    } else {
+        if (dt == F32) launch_direct<F32, false, F32>(MX4_ARGS);
+        else if (dt == BF16) launch_direct<BF16, false, BF16>(MX4_ARGS);
+        else launch_direct<F16, false, F16>(MX4_ARGS);
+    }
+    #undef MX4_ARGS
+}
+
+void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
+              const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
+              int bias_dt, void* y, int dt, hipStream_t stream) {
+    #define MX4_ARGS xc, xs, M, K, 0, wc, ws, N, bias, bias_dt, y, stream
+    if (dt == F32) launch_direct<CODES, true, F32>(MX4_ARGS);
+    else if (dt == BF16) launch_direct<CODES, true, BF16>(MX4_ARGS);
+    else launch_direct<CODES, true, F16>(MX4_ARGS);
+    #undef MX4_ARGS
+}
+
+}  // namespace mx4

@@ -1,0 +1,246 @@
+"""4-bit rows (MX e2m1 with a power-of-two scale for 32 elements) and their
+product, on the matrix cores that take them directly.
+
+* ``mx4_quantize(x)`` rounds the last axis to blocks -> ``MX4Tensor``;
+* ``MX4Tensor.dequantize()`` reads it back (exact in bf16 and fp32);
+* ``mx4_linear(x, weight, bias)`` is ``Q(x) Q(weight)^T + bias`` with fp32
+  sums. A held ``MX4Tensor`` weight serves; a float weight is rounded in the
+  call and trains: the gradients are straight-through,
+  ``dx = g Q(w)``, ``dw = g^T Q(x)``, ``db = sum g``.
+
+Format (OCP Microscaling Formats v1.0, MXFP4): a block of 32 has the scale
+``2^E``, ``E = clamp(floor(log2 max|x|) - 2, -127, 127)``, and each element is
+the nearest of ``{0, .5, 1, 1.5, 2, 3, 4, 6} * 2^E`` with its sign, ties to the
+even code, 6 at most. A block that holds a NaN or an infinity reads as NaN.
+
+CPU tensors take the PyTorch form (ops/reference.py), GPU tensors the HIP
+kernels (ops/hip/mx4_*.hip).
+"""
+
+import math
+from typing import Optional, Union
+
+import torch
+
+from . import reference
+
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_float(t: torch.Tensor, what: str):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f'{what}: a tensor, not {type(t).__name__}')
+    if t.dtype not in _CODE:
+        raise TypeError(f'{what}: float32, bfloat16 or float16, not {t.dtype}')
+
+
+def _ext(t: torch.Tensor):
+    """The extension for GPU tensors, None for the PyTorch form."""
+    if not t.is_cuda:
+        return None
+    from . import _native_or_die
+    return _native_or_die()
+
+
+def padded(K: int) -> int:
+    """Elements that a row of K takes up: a multiple of 128."""
+    return -(-K // 128) * 128
+
+
+class MX4Tensor:
+    """Rows held in 4 bits: ``codes`` uint8 [..., Kp/2] (low nibble first) and
+    ``scales`` uint8 [..., Kp/32] (2^(byte-127), 255 = NaN), where Kp is the
+    row length K rounded up to 128; codes and scales behind K are 0.
+    ``dtype`` is the type that ``dequantize`` gives where none is asked."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, K: int,
+                 dtype: torch.dtype = torch.bfloat16):
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError('MX4Tensor: codes and scales are uint8')
+        Kp = padded(K)
+        if (K < 0 or codes.dim() < 1 or codes.shape[-1] * 2 != Kp
+                or scales.shape != (*codes.shape[:-1], Kp // 32)):
+            raise ValueError(
+                f'MX4Tensor: codes {tuple(codes.shape)} and scales '
+                f'{tuple(scales.shape)} do not hold rows of {K}')
+        if codes.device != scales.device:
+            raise ValueError('MX4Tensor: codes and scales on one device')
+        if dtype not in _CODE:
+            raise TypeError(f'MX4Tensor: no values of type {dtype}')
+        self.codes, self.scales = codes.contiguous(), scales.contiguous()
+        self.K, self.dtype = K, dtype
+
+    @classmethod
+    def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor,
+                   dtype: torch.dtype = torch.bfloat16) -> 'MX4Tensor':
+        """From unpadded parts, codes [..., K/2] and scales [..., K/32] with K
+        a multiple of 32, as other programs store them."""
+        K = codes.shape[-1] * 2
+        if K % 32 or scales.shape != (*codes.shape[:-1], K // 32):
+            raise ValueError(
+                f'MX4Tensor: codes {tuple(codes.shape)} and scales '
+                f'{tuple(scales.shape)} are not blocks of 32')
+        pad = padded(K) - K
+        return cls(torch.nn.functional.pad(codes, (0, pad // 2)),
+                   torch.nn.functional.pad(scales, (0, pad // 32)), K, dtype)
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.codes.shape[:-1], self.K))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def to(self, device) -> 'MX4Tensor':
+        return MX4Tensor(self.codes.to(device), self.scales.to(device),
+                         self.K, self.dtype)
+
+    def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return mx4_dequantize(self, dtype)
+
+    def _rows(self):
+        M = math.prod(self.codes.shape[:-1])
+        return (self.codes.view(M, self.codes.shape[-1]),
+                self.scales.view(M, self.scales.shape[-1]))
+
+    def __repr__(self):
+        return (f'MX4Tensor(shape={tuple(self.shape)}, '
+                f'device={self.device}, dtype={self.dtype})')
+
+
+def _matrix(x: torch.Tensor) -> torch.Tensor:
+    """[..., K] -> [M, K] with contiguous rows; a view where it can be."""
+    K = x.shape[-1]
+    M = math.prod(x.shape[:-1])
+    x2 = x.reshape(M, K)
+    if K > 1 and x2.stride(1) != 1 or M > 1 and x2.stride(0) < K:
+        x2 = x2.contiguous()
+    return x2
+
+
+def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
+    """[..., K] float32, bfloat16 or float16 -> 4-bit rows. No gradient."""
+    _check_float(x, 'mx4_quantize')
+    if x.dim() < 1:
+        raise ValueError('mx4_quantize: a tensor of rows, not a number')
+    x2 = _matrix(x.detach())
+    ext = _ext(x2)
+    if ext is not None:
+        codes, scales = ext.mx4_quantize(x2)
+    else:
+        codes, scales = reference.mx4_quantize(x2)
+    lead = x.shape[:-1]
+    return MX4Tensor(codes.view(*lead, codes.shape[-1]),
+                     scales.view(*lead, scales.shape[-1]), x.shape[-1],
+                     x.dtype)
+
+
+def mx4_dequantize(q: MX4Tensor,
+                   dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values that 4-bit rows stand for. bf16 and fp32 hold them all;
+    fp16 rounds, and overflows, where a scale leaves its range."""
+    dtype = dtype or q.dtype
+    if dtype not in _CODE:
+        raise TypeError(f'mx4_dequantize: no values of type {dtype}')
+    codes, scales = q._rows()
+    ext = _ext(codes)
+    if ext is not None:
+        out = ext.mx4_dequantize(codes, scales, q.K, _CODE[dtype])
+    else:
+        out = reference.mx4_dequantize(codes, scales, q.K, dtype)
+    return out.view(q.shape)
+
+
+class _MX4Linear(torch.autograd.Function):
+    """weight: a float [N, K] matrix, or None with (wc, ws) held in 4 bits."""
+
+    @staticmethod
+    def forward(ctx, x2, weight, wc, ws, bias, train):
+        ext = _ext(x2)
+        K = x2.shape[1]
+        if weight is not None:
+            w2 = weight if weight.stride(1) == 1 or K <= 1 \
+                else weight.contiguous()
+            wc, ws = (ext.mx4_quantize(w2) if ext is not None
+                      else reference.mx4_quantize(w2))
+        need_w = train and weight is not None and ctx.needs_input_grad[1]
+        xc = xs = None
+        if need_w:      # the rounded rows are kept, a quarter of x
+            xc, xs = (ext.mx4_quantize(x2) if ext is not None
+                      else reference.mx4_quantize(x2))
+        if ext is None:
+            if xc is None:
+                xc, xs = reference.mx4_quantize(x2)
+            y = reference.mx4_product(xc, xs, wc, ws, K, bias, x2.dtype)
+        elif need_w:
+            y = ext.mx4_linear_q(xc, xs, K, wc, ws, bias, _CODE[x2.dtype])
+        else:
+            y = ext.mx4_linear(x2, wc, ws, bias)
+        ctx.save_for_backward(*((xc, xs) if need_w else (None, None)),
+                              *((wc, ws) if train and ctx.needs_input_grad[0]
+                                else (None, None)))
+        ctx.K, ctx.x_dtype = K, x2.dtype
+        ctx.w_dtype = weight.dtype if weight is not None else None
+        ctx.b_dtype = bias.dtype if bias is not None else None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        xc, xs, wc, ws = ctx.saved_tensors
+        g = g.contiguous()
+        ext = _ext(g)
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            dx = (ext.mx4_grad_input(g, wc, ws, ctx.K, _CODE[ctx.x_dtype])
+                  if ext is not None else
+                  reference.mx4_grad_input(g, wc, ws, ctx.K, ctx.x_dtype))
+        if ctx.needs_input_grad[1]:
+            dw = (ext.mx4_grad_weight(g, xc, xs, ctx.K, _CODE[ctx.w_dtype])
+                  if ext is not None else
+                  reference.mx4_grad_weight(g, xc, xs, ctx.K, ctx.w_dtype))
+        if ctx.needs_input_grad[4]:
+            db = (ext.col_sum(g, _CODE[ctx.b_dtype]) if ext is not None
+                  else g.float().sum(0).to(ctx.b_dtype))
+        return dx, dw, None, None, db, None
+
+
+def mx4_linear(x: torch.Tensor, weight: Union[MX4Tensor, torch.Tensor],
+               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``Q(x) Q(weight)^T + bias``: x [..., K], weight [N, K], bias [N]; the
+    result [..., N] has x's type. Sums are fp32, rounded once.
+
+    A NaN or an infinity in a block of x makes its row NaN, one in a block of
+    the weight its column. Differentiable once, in x, a float weight and bias.
+    """
+    _check_float(x, 'mx4_linear: input')
+    held = isinstance(weight, MX4Tensor)
+    if not held:
+        _check_float(weight, 'mx4_linear: weight')
+    if x.dim() < 1:
+        raise ValueError('mx4_linear: input: rows, not a number')
+    if len(weight.shape) != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f'mx4_linear: input {tuple(x.shape)} and weight '
+                         f'{tuple(weight.shape)} do not match')
+    if weight.device != x.device:
+        raise ValueError(f'mx4_linear: input on {x.device}, weight on '
+                         f'{weight.device}')
+    if bias is not None:
+        _check_float(bias, 'mx4_linear: bias')
+        if bias.shape != (weight.shape[0],):
+            raise ValueError(f'mx4_linear: bias {tuple(bias.shape)} for '
+                             f'{weight.shape[0]} columns')
+        if bias.device != x.device:
+            raise ValueError(f'mx4_linear: input on {x.device}, bias on '
+                             f'{bias.device}')
+        bias = bias.contiguous()
+    x2 = _matrix(x)
+    wc, ws = weight._rows() if held else (None, None)
+    y = _MX4Linear.apply(x2, None if held else weight, wc, ws, bias,
+                         torch.is_grad_enabled())
+    return y.view(*x.shape[:-1], weight.shape[0])

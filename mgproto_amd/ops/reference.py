@@ -21,6 +21,7 @@ import math
 from typing import Tuple
 
 import torch
+import torch.nn.functional as F
 
 LOG_2PI = math.log(2.0 * math.pi)
 
@@ -315,3 +316,131 @@ def argmin_hw(probs: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 # Aux — Proxy-Anchor loss pieces (reference utils/losses.py:41-61) live in
 # mgproto_amd.losses; they are small GEMMs and stay on the PyTorch path.
 # ---------------------------------------------------------------------------
+
+
+# ---------------------------------------------------------------------------
+# 4-bit rows (OCP Microscaling Formats v1.0, MXFP4) and their product
+# ---------------------------------------------------------------------------
+
+def _power_of_two(e: torch.Tensor) -> torch.Tensor:
+    """2^e as float32 for whole e in [-127, 127], by its bits."""
+    e = e.to(torch.int32)
+    return torch.where(e > -127, (e + 127) << 23, 1 << 22).to(
+        torch.int32).view(torch.float32)
+
+
+def mx4_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """[M, K] -> codes uint8 [M, Kp/2], scales uint8 [M, Kp/32], Kp = K
+    rounded up to 128."""
+    M, K = x.shape
+    Kp = -(-K // 128) * 128
+    v = F.pad(x.float(), (0, Kp - K)).reshape(M, Kp // 32, 32)
+    amax = v.abs().amax(dim=2)
+    bad = ~torch.isfinite(amax)
+    # the exponent field is floor(log2 amax) + 127; 0 for subnormal numbers
+    field = (amax.view(torch.int32) >> 23) & 0xff
+    byte = (field - 2).clamp(min=0)
+    unit = _power_of_two(byte - 127).unsqueeze(2)
+    r = v.abs() / unit
+    step = torch.where(r < 2, 0.5, torch.where(r < 4, 1.0, 2.0))
+    r = (torch.round(r / step) * step).clamp(max=6.0)     # ties to even
+    grid = torch.tensor([0., .5, 1., 1.5, 2., 3., 4., 6.], device=x.device)
+    r = torch.where(bad.unsqueeze(2), 0.0, r)
+    code = torch.searchsorted(grid, r.contiguous())
+    code = code + 8 * (torch.signbit(v) & ~bad.unsqueeze(2))
+    code = code.view(M, Kp // 2, 2)
+    codes = (code[..., 0] | code[..., 1] << 4).to(torch.uint8)
+    scales = torch.where(bad, 255, byte).to(torch.uint8)
+    return codes, scales
+
+
+def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int,
+                   dtype: torch.dtype) -> torch.Tensor:
+    M, nb = scales.shape
+    c = torch.stack([codes & 15, codes >> 4], dim=2).view(M, nb, 32).long()
+    grid = torch.tensor([0., .5, 1., 1.5, 2., 3., 4., 6.],
+                        device=codes.device)
+    v = grid[c & 7]
+    v = torch.where(c >= 8, -v, v)
+    unit = _power_of_two(scales.to(torch.int32).clamp(max=254) - 127)
+    unit = torch.where(scales == 255, math.nan, unit)
+    return (v * unit.unsqueeze(2)).view(M, nb * 32)[:, :K].to(dtype)
+
+
+def mx4_product(xc, xs, wc, ws, K: int, bias, dtype) -> torch.Tensor:
+    y = (mx4_dequantize(xc, xs, K, torch.float32)
+         @ mx4_dequantize(wc, ws, K, torch.float32).t())
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(dtype)
+
+
+def mx4_grad_input(g, wc, ws, K: int, dtype) -> torch.Tensor:
+    return (g.float() @ mx4_dequantize(wc, ws, K, torch.float32)).to(dtype)
+
+
+def mx4_grad_weight(g, xc, xs, K: int, dtype) -> torch.Tensor:
+    return (g.float().t()
+            @ mx4_dequantize(xc, xs, K, torch.float32)).to(dtype)
+
+
+# ---------------------------------------------------------------------------
+# global gradient norm and clipping
+# ---------------------------------------------------------------------------
+
+def grad_norm(grads, p: float) -> torch.Tensor:
+    """float64 number."""
+    total = torch.zeros((), dtype=torch.float64, device=grads[0].device)
+    for g in grads:
+        if not g.numel():
+            continue
+        a = g.double().abs()
+        if p == math.inf:
+            total = torch.maximum(total, a.amax())        # a NaN stays
+        else:
+            total = total + (a if p == 1.0 else a * a).sum()
+    return total.sqrt() if p == 2.0 else total
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """No gaps and no element twice, in whatever order of the axes."""
+    at = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride())
+                                if n != 1), key=lambda e: e[1]):
+        if stride != at:
+            return t.numel() == 0
+        at *= size
+    return True
+
+
+def _check_written(grads, outs):
+    """A written tensor may share memory with no other one, but for its own
+    source in the same place and of the same type."""
+    spans = []
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        if not _dense(o):
+            raise RuntimeError(f'clip_grads_: tensor {i} is written and has '
+                               'gaps or shares elements with itself')
+        if o.numel():
+            spans.append((o.data_ptr(), i, True, o))
+            if g.data_ptr() != o.data_ptr() or g.dtype != o.dtype:
+                spans.append((g.data_ptr(), i, False, g))
+    any_end = out_end = 0
+    for lo, i, written, t in sorted(spans, key=lambda e: e[0]):
+        if lo < out_end or written and lo < any_end:
+            raise RuntimeError('clip_grads_: a tensor that is written shares '
+                               f'memory with another one (number {i})')
+        end = lo + t.element_size() * (1 + sum(
+            (n - 1) * st for n, st in zip(t.shape, t.stride())))
+        any_end = max(any_end, end)
+        if written:
+            out_end = max(out_end, end)
+
+
+def clip_grads(grads, outs, max_norm: float, p: float) -> torch.Tensor:
+    norm = grad_norm(grads, p)
+    factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
+    _check_written(grads, outs)
+    for g, o in zip(grads, outs):
+        o.copy_((g.double() * factor).to(o.dtype))
+    return norm.float()

@@ -1,0 +1,261 @@
+"""4-bit rows and their product on the GPU against the definition in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from mgproto_amd import ops
+from mx4_oracle import GRID, assert_close, values
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _same(q, ref):
+    assert torch.equal(q.codes.cpu(), ref.codes)
+    assert torch.equal(q.scales.cpu(), ref.scales)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('M,K', [(1, 1), (3, 32), (5, 33), (64, 127),
+                                 (4, 128), (7, 300), (1000, 1024),
+                                 (333, 1003)])
+def test_quantize(M, K, dtype):
+    x = (torch.randn(M, K) * torch.exp(3 * torch.randn(M, K))).clamp(
+        -6e4, 6e4).to(dtype)
+    x[M // 2, K // 2] = math.inf
+    x[M - 1, 0] = math.nan
+    q = ops.mx4_quantize(x.cuda())
+    _same(q, ops.mx4_quantize(x))
+    for t in DTYPES:
+        want = ops.mx4_quantize(x).dequantize(t)
+        got = q.dequantize(t).cpu()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+    ok = ~want.isnan()
+    assert torch.equal(q.dequantize(torch.float32).cpu().double()[ok],
+                       values(x)[ok])
+
+
+def test_quantize_every_value_at_every_scale():
+    mid = (GRID[1:] + GRID[:-1]) / 2
+    row = torch.cat([GRID, mid, mid * (1 + 2 ** -20), mid * (1 - 2 ** -20)])
+    row = torch.cat([row, -row])
+    row = torch.nn.functional.pad(row, (0, -len(row) % 31)).view(-1, 31)
+    x = torch.cat([row, torch.full((len(row), 1), 6.0)], dim=1).double()
+    for e in (-149, -140, -130, -127, -126, -125, -60, 0, 60, 124, 125):
+        xe = (x * 2.0 ** e).float()
+        _same(ops.mx4_quantize(xe.cuda()), ops.mx4_quantize(xe))
+        xe = xe.bfloat16()
+        _same(ops.mx4_quantize(xe.cuda()), ops.mx4_quantize(xe))
+    for e in (-24, -14, 0, 13):
+        xe = (x * 2.0 ** e).half()
+        _same(ops.mx4_quantize(xe.cuda()), ops.mx4_quantize(xe))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_quantize_strides_and_alignments(dtype):
+    base = torch.randn(40, 300).to(dtype)
+    for view in (lambda t: t[:, :256], lambda t: t[:, 1:257],
+                 lambda t: t[:, 8:200], lambda t: t[::3, 3:100],
+                 lambda t: t.t(), lambda t: t[:1].expand(5, 300)):
+        _same(ops.mx4_quantize(view(base.cuda())),
+              ops.mx4_quantize(view(base)))
+
+
+SIZES = [(1, 1, 1), (1, 32, 16), (2, 33, 5), (16, 128, 64), (17, 129, 65),
+         (33, 96, 40), (64, 2048, 256), (130, 257, 131), (300, 200, 1000),
+         (1100, 64, 1001), (8, 4096, 512), (513, 640, 384)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('M,K,N', SIZES)
+def test_linear_and_its_gradients(M, K, N, dtype):
+    x = torch.randn(M, K).to(dtype)
+    w = torch.randn(N, K) / K ** 0.5
+    b = torch.randn(N)
+    g = torch.randn(M, N).to(dtype)
+    xd, wd, bd = (t.cuda().requires_grad_() for t in (x, w, b))
+    y = ops.mx4_linear(xd, wd, bd)
+    dx, dw, db = torch.autograd.grad(y, (xd, wd, bd), g.cuda())
+    assert y.dtype == dtype and dx.dtype == dtype
+    assert dw.dtype == db.dtype == torch.float32
+    xv, wv, g64 = values(x), values(w), g.double()
+    want = xv @ wv.t() + b.double()
+    mass = xv.abs() @ wv.abs().t() + b.double().abs()
+    assert_close(y, want, mass, K + 1)
+    assert_close(dx, g64 @ wv, g64.abs() @ wv.abs(), 3 * N)
+    assert_close(dw, g64.t() @ xv, g64.abs().t() @ xv.abs(), 3 * M)
+    assert_close(db, g64.sum(0), g64.abs().sum(0), M)
+    # a held weight takes the form that rounds x on the way
+    held = ops.mx4_quantize(wd)
+    assert_close(ops.mx4_linear(xd, held, bd), want, mass, K + 1)
+    with torch.no_grad():
+        assert_close(ops.mx4_linear(xd, wd, bd), want, mass, K + 1)
+
+
+@pytest.mark.parametrize('M,K,N', SIZES + [(2000, 512, 300)])
+def test_whole_numbers_are_exact(M, K, N):
+    # every sum is a whole number of quarters below 2^22: fp32 holds it
+    x = GRID[torch.randint(0, 8, (M, K))] * (torch.randint(0, 2, (M, K)) * 2 - 1)
+    w = GRID[torch.randint(0, 8, (N, K))] * (torch.randint(0, 2, (N, K)) * 2 - 1)
+    g = torch.randint(-4, 5, (M, N)).double()
+    xv, wv = values(x.float()), values(w.float())
+    x, w = (t.float().cuda().requires_grad_() for t in (x, w))
+    y = ops.mx4_linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), g.float().cuda())
+    assert torch.equal(y.double().cpu(), xv @ wv.t())
+    assert torch.equal(dx.double().cpu(), g @ wv)
+    assert torch.equal(dw.double().cpu(), g.t() @ xv)
+    held = ops.mx4_quantize(w)
+    for dtype in DTYPES:
+        y = ops.mx4_linear(x.detach().to(dtype), held)
+        assert torch.equal(y.cpu(), (xv @ wv.t()).to(dtype))
+    # a gradient in bf16 and fp16 holds these numbers too
+    for dtype in (torch.bfloat16, torch.float16):
+        xt = x.detach().to(dtype).requires_grad_()
+        y = ops.mx4_linear(xt, w)
+        dx, dw = torch.autograd.grad(y, (xt, w), g.to(dtype).cuda())
+        assert torch.equal(dx.cpu(), (g @ wv).to(dtype))
+        assert torch.equal(dw.double().cpu(), g.t() @ xv)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('M', [1, 40, 3000])
+def test_strides_and_alignments(dtype, M):
+    base = torch.randn(M, 300).to(dtype).cuda()
+    w = ops.mx4_quantize(torch.randn(96, 256).cuda())
+    for lo in (0, 1, 8, 44):
+        x = base[:, lo:lo + 256]
+        assert torch.equal(ops.mx4_linear(x, w),
+                           ops.mx4_linear(x.contiguous(), w))
+    x = torch.randn(256, M).to(dtype).cuda().t()
+    assert torch.equal(ops.mx4_linear(x, w),
+                       ops.mx4_linear(x.contiguous(), w))
+    # an expanded output gradient
+    x = base[:, :256].detach().requires_grad_()
+    y = ops.mx4_linear(x, w)
+    (d1,) = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    (d2,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(d1, d2)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('M', [4, 100, 2000])
+def test_nan_and_infinity_stay_in_their_rows(dtype, M):
+    K, N = 160, 200
+    x, w = torch.randn(M, K).to(dtype), torch.randn(N, K)
+    x[1, 40], x[3, 159], w[7, 0] = math.nan, -math.inf, math.inf
+    g = torch.randn(M, N).to(dtype)
+    xd, wd = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = ops.mx4_linear(xd, wd)
+    dx, dw = torch.autograd.grad(y, (xd, wd), g.cuda())
+    bad = torch.zeros(M, N, dtype=torch.bool)
+    bad[1], bad[3], bad[:, 7] = True, True, True
+    assert torch.equal(y.cpu().isnan(), bad)
+    assert torch.equal(ops.mx4_linear(xd, ops.mx4_quantize(wd)).cpu().isnan(),
+                       bad)
+    # a block reads as NaN in the gradients, too
+    badx = torch.zeros(M, K, dtype=torch.bool)
+    badx[:, :32] = True
+    assert torch.equal(dx.cpu().isnan(), badx)
+    badw = torch.zeros(N, K, dtype=torch.bool)
+    badw[:, 32:64], badw[:, 128:160] = True, True
+    assert torch.equal(dw.cpu().isnan(), badw)
+
+
+def test_scales_far_apart():
+    x = torch.randn(50, 256) * torch.exp2(
+        torch.randint(-60, 60, (50, 8)).float()).repeat_interleave(32, 1)
+    w = torch.randn(70, 256) * torch.exp2(
+        torch.randint(-60, 60, (70, 8)).float()).repeat_interleave(32, 1)
+    y = ops.mx4_linear(x.cuda(), w.cuda())
+    xv, wv = values(x), values(w)
+    assert_close(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), 256)
+
+
+def test_empty_sizes():
+    for M, K, N in [(0, 32, 4), (3, 0, 4), (3, 32, 0)]:
+        x = torch.randn(M, K, device='cuda', requires_grad=True)
+        w = torch.randn(N, K, device='cuda', requires_grad=True)
+        b = torch.randn(N, device='cuda', requires_grad=True)
+        y = ops.mx4_linear(x, w, b)
+        assert y.shape == (M, N)
+        if K == 0:
+            assert torch.equal(y, b.expand(M, N))
+        for t, d in zip((x, w, b), torch.autograd.grad(y.sum(), (x, w, b))):
+            assert d.shape == t.shape
+            if M * K * N == 0 and t is not b:
+                assert not d.any()
+
+
+@pytest.mark.parametrize('M', [1, 300])
+def test_other_stream_and_graph(M):
+    K, N = 320, 130
+    w = torch.randn(N, K, device='cuda', requires_grad=True)
+    held = ops.mx4_quantize(w)
+    x = torch.zeros(M, K, device='cuda', dtype=torch.bfloat16,
+                    requires_grad=True)
+    g = torch.randn(M, N, device='cuda').bfloat16()
+    ins = [torch.randn(M, K, device='cuda').bfloat16() for _ in range(3)]
+
+    def step():
+        y = ops.mx4_linear(x, w)
+        return (y.detach(), ops.mx4_linear(x.detach(), held),
+                *torch.autograd.grad(y, (x, w), g))
+
+    want = []
+    for t in ins:
+        with torch.no_grad():
+            x.copy_(t)
+        want.append([r.clone() for r in step()])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(again, want[-1]):
+        assert torch.equal(a, b)
+    del again
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for t, ws in zip(ins * 2, want * 2):
+        with torch.no_grad():
+            x.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, ws):
+            assert torch.equal(a, b)
+        torch.randn(1000, device='cuda').sum().item()
+
+
+def test_results_do_not_change_from_run_to_run():
+    x = torch.randn(3000, 512, device='cuda').bfloat16().requires_grad_()
+    w = torch.randn(256, 512, device='cuda', requires_grad=True)
+    g = torch.randn(3000, 256, device='cuda').bfloat16()
+    runs = []
+    for _ in range(3):
+        y = ops.mx4_linear(x, w)
+        runs.append((y, *torch.autograd.grad(y, (x, w), g)))
+    for r in runs[1:]:
+        for a, b in zip(runs[0], r):
+            assert torch.equal(a, b)
+
+
+def test_refusals():
+    q = ops.mx4_quantize(torch.randn(8, 64))
+    with pytest.raises(ValueError, match='weight on cpu'):
+        ops.mx4_linear(torch.randn(4, 64, device='cuda'), q)
+    ext = ops._native_or_die()
+    qd = q.to('cuda')
+    x = torch.randn(4, 64, device='cuda')
+    with pytest.raises(RuntimeError, match='do not hold rows'):
+        ext.mx4_linear(x, qd.codes[:, :32].contiguous(), qd.scales, None)
+    with pytest.raises(RuntimeError, match='contiguous'):
+        ext.mx4_linear(x.t(), qd.codes, qd.scales, None)
+    with pytest.raises(RuntimeError, match='does not match'):
+        ext.mx4_grad_input(torch.randn(4, 7, device='cuda'), qd.codes,
+                           qd.scales, 64, 0)
