@@ -53,7 +53,7 @@ void check_packed(const Tensor& codes, const Tensor& scales, int64_t K,
                     codes.is_contiguous() && scales.is_contiguous(), what,
                 ": contiguous matrices");
     const int64_t Kp = (K + 127) / 128 * 128;
-    TORCH_CHECK(K >= 0 && K < (1L << 30) && codes.size(1) == Kp / 2 &&
+    TORCH_CHECK(K >= 0 && K < (1L << 22) && codes.size(1) == Kp / 2 &&
                     scales.size(1) == Kp / 32 &&
                     codes.size(0) == scales.size(0), what,
                 ": codes ", codes.sizes(), " and scales ", scales.sizes(),
@@ -101,8 +101,19 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
     return out;
 }
 
+// what one tile of 16 x 16 a block can number
+void check_tiles(int64_t M, int64_t N) {
+    TORCH_CHECK((M + 15) / 16 * ((N + 15) / 16) < (1L << 31),
+                "mx4_linear: ", M, " x ", N, " results are too many");
+}
+
+int pick(int64_t form, int chosen) {
+    TORCH_CHECK(form >= -1 && form < mx4::FORMS, "mx4_linear: no form ", form);
+    return form < 0 ? chosen : (int)form;
+}
+
 Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws,
-              const c10::optional<Tensor>& bias) {
+              const c10::optional<Tensor>& bias, int64_t form) {
     check_rows(x, "mx4_linear: input");
     const int64_t M = x.size(0), K = x.size(1), N = wc.size(0);
     check_packed(wc, ws, K, "mx4_linear: weight");
@@ -110,32 +121,43 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws,
     check_bias(bias, N, x);
     const int dt = dtype_code(x, "mx4_linear: input");
     c10::DeviceGuard guard(x.device());
+    check_tiles(M, N);
     auto y = at::empty({M, N}, x.options());
-    if (M && N)
-        mx4::linear(x.data_ptr(), dt, M, K, M > 1 ? x.stride(0) : K,
-                    wc.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), N,
-                    bias ? bias->data_ptr() : nullptr,
-                    bias ? dtype_code(*bias, "mx4_linear: bias") : 0,
-                    y.data_ptr(), current_stream());
+    if (!M || !N) return y;
+    const int64_t ldx = M > 1 ? x.stride(0) : K;
+    const bool aligned = (uintptr_t)x.data_ptr() % 16 == 0 &&
+                         ldx * x.element_size() % 16 == 0;
+    const int f = pick(form, mx4::linear_form(M, K, N, dt, aligned));
+    Tensor work;
+    if (const size_t bytes = mx4::linear_bytes(f, M, K))
+        work = workspace(bytes, x);
+    mx4::linear(x.data_ptr(), dt, M, K, ldx, wc.data_ptr<uint8_t>(),
+                ws.data_ptr<uint8_t>(), N, bias ? bias->data_ptr() : nullptr,
+                bias ? dtype_code(*bias, "mx4_linear: bias") : 0, y.data_ptr(),
+                f, work.defined() ? work.data_ptr() : nullptr,
+                current_stream());
     return y;
 }
 
 Tensor linear_q(const Tensor& xc, const Tensor& xs, int64_t K,
                 const Tensor& wc, const Tensor& ws,
-                const c10::optional<Tensor>& bias, int64_t dt) {
+                const c10::optional<Tensor>& bias, int64_t dt, int64_t form) {
     check_packed(xc, xs, K, "mx4_linear: input");
     check_packed(wc, ws, K, "mx4_linear: weight");
     TORCH_CHECK(xc.device() == wc.device(), "mx4_linear: one GPU for all");
     const int64_t M = xc.size(0), N = wc.size(0);
     check_bias(bias, N, xc);
     c10::DeviceGuard guard(xc.device());
+    check_tiles(M, N);
     auto y = at::empty({M, N}, xc.options().dtype(scalar_type(dt)));
     if (M && N)
         mx4::linear_q(xc.data_ptr<uint8_t>(), xs.data_ptr<uint8_t>(), M, K,
                       wc.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), N,
                       bias ? bias->data_ptr() : nullptr,
                       bias ? dtype_code(*bias, "mx4_linear: bias") : 0,
-                      y.data_ptr(), (int)dt, current_stream());
+                      y.data_ptr(), (int)dt,
+                      pick(form, mx4::linear_q_form(M, K, N)),
+                      current_stream());
     return y;
 }
 
@@ -320,8 +342,14 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
 void register_mx4(pybind11::module& m) {
     m.def("mx4_quantize", &quantize, "rows to MX4 codes and scales");
     m.def("mx4_dequantize", &dequantize, "MX4 codes and scales to values");
-    m.def("mx4_linear", &linear, "Q(x) W^T + bias, x rounded on the way");
-    m.def("mx4_linear_q", &linear_q, "X W^T + bias from 4-bit rows");
+    namespace py = pybind11;
+    m.def("mx4_linear", &linear, "Q(x) W^T + bias", py::arg("x"),
+          py::arg("codes"), py::arg("scales"), py::arg("bias"),
+          py::arg("form") = -1);
+    m.def("mx4_linear_q", &linear_q, "X W^T + bias from 4-bit rows",
+          py::arg("xcodes"), py::arg("xscales"), py::arg("K"),
+          py::arg("codes"), py::arg("scales"), py::arg("bias"),
+          py::arg("dtype"), py::arg("form") = -1);
     m.def("mx4_grad_input", &grad_input, "g W");
     m.def("mx4_grad_weight", &grad_weight, "g^T X");
     m.def("col_sum", &col_sum, "column sums of a matrix");

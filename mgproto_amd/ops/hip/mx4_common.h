@@ -164,15 +164,29 @@ void quantize(const void* x, int dt, long rows, long K, long ldx,
 void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
                 long K, void* out, int dt, hipStream_t stream);
 
-// y[M,N] = Q(x) W^T + bias, x rounded on the way
+// Forms of the product. linear_form() and linear_q_form() choose; each form
+// is right for every size.
+enum Form : int {
+    ROWS16 = 0,       // 16 x 16 of y a block, its waves share the sum
+    ROWS32 = 1,       // 32 x 32 of y a block, the same
+    ROUNDING = 2,     // tiles; x rounded on its way into LDS
+    TILES128 = 3,     // tiles of 4-bit rows; x rounded before
+    TILES256 = 4,
+    FORMS = 5
+};
+
+// y[M,N] = Q(x) W^T + bias
+int linear_form(long M, long K, long N, int dt, bool aligned);
+size_t linear_bytes(int form, long M, long K);        // of workspace
 void linear(const void* x, int dt, long M, long K, long ldx,
             const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
-            int bias_dt, void* y, hipStream_t stream);
+            int bias_dt, void* y, int form, void* work, hipStream_t stream);
 
 // the same from rows that are held in 4 bits already
+int linear_q_form(long M, long K, long N);
 void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
-              int bias_dt, void* y, int dt, hipStream_t stream);
+              int bias_dt, void* y, int dt, int form, hipStream_t stream);
 
 // dx[M,K] = g[M,N] W[N,K] and dw[N,K] = g[M,N]^T X[M,K]; each states the
 // bytes of workspace that it wants

@@ -13,21 +13,12 @@
 #include <hip/hip_runtime.h>
 
 #include "mx4_common.h"
+#include "mx4_linear.h"
 
 namespace mx4 {
 namespace {
 
 constexpr int CODES = -1;     // x is held in 4 bits already
-
-static __device__ __forceinline__ float load_any(const void* p, int dt, long i) {
-    if (dt == F32) return reinterpret_cast<const float*>(p)[i];
-    if (dt == BF16) return (float)reinterpret_cast<const __bf16*>(p)[i];
-    return (float)reinterpret_cast<const _Float16*>(p)[i];
-}
-
-static __device__ __forceinline__ i32x8 wide(i32x4 v) {
-    return (i32x8){v.x, v.y, v.z, v.w, 0, 0, 0, 0};
-}
 
 // One block of x: loaded, rounded; codes and scale byte stay in this lane.
 template <int DT, bool VEC>
@@ -52,24 +43,20 @@ static __device__ __forceinline__ i32x4 round_block(
     return c;
 }
 
-// FM x FN tiles of 16x16 a wave. WK = 1: the four waves lie 2 x 2; WK = 4:
-// they share one tile and take every fourth step each, joined in LDS.
-template <int AT, bool VEC, int OT, int FM, int FN, int WK>
+// FM x FN tiles of 16 x 16 a block. Its four waves take every fourth step of
+// 128 each and are joined in LDS, in their order.
+template <int AT, bool VEC, int OT, int FM, int FN>
 __global__ __launch_bounds__(256)
-void linear_direct_kernel(const void* __restrict__ xv,
-                          const uint8_t* __restrict__ xs, long M, int K,
-                          int Kp, long ldx, const uint8_t* __restrict__ wc,
-                          const uint8_t* __restrict__ ws, long N,
-                          const void* __restrict__ bias, int bias_dt,
-                          typename Elem<OT>::T* __restrict__ y) {
-    using T = typename Elem<OT>::T;
+void linear_rows_kernel(const void* __restrict__ xv,
+                        const uint8_t* __restrict__ xs, long M, int K, int Kp,
+                        long ldx, const uint8_t* __restrict__ wc,
+                        const uint8_t* __restrict__ ws, long N,
+                        const void* __restrict__ bias, int bias_dt,
+                        typename Elem<OT>::T* __restrict__ y, int nt) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r16 = lane & 15, g = lane >> 4;
-    constexpr int TM = 16 * FM, TN = 16 * FN;
-    const long m0 = WK == 1 ? (long)blockIdx.x * (2 * TM) + (wave >> 1) * TM
-                            : (long)blockIdx.x * TM;
-    const long n0 = WK == 1 ? (long)blockIdx.y * (2 * TN) + (wave & 1) * TN
-                            : (long)blockIdx.y * TN;
+    const long m0 = (long)(blockIdx.x / nt) * (16 * FM);
+    const long n0 = (long)(blockIdx.x % nt) * (16 * FN);
     const int cb = Kp >> 1, sb = Kp >> 5;        // bytes of a row
 
     const uint8_t* wrow[FN];
@@ -91,7 +78,7 @@ void linear_direct_kernel(const void* __restrict__ xv,
         for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
 
     const int steps = Kp >> 7;
-    for (int s = WK == 1 ? 0 : wave; s < steps; s += WK) {
+    for (int s = wave; s < steps; s += 4) {
         i32x4 w[FN], x[FM];
         int wb[FN], xb[FM];
         #pragma unroll
@@ -121,100 +108,109 @@ void linear_direct_kernel(const void* __restrict__ xv,
                     wide(w[j]), wide(x[i]), acc[i][j], 4, 4, 0, wb[j], 0, xb[i]);
     }
 
-    if constexpr (WK > 1) {      // joined in the order of the waves
-        __shared__ f32x4 part[WK - 1][FM * FN][64];
-        if (wave) {
-            #pragma unroll
-            for (int i = 0; i < FM; ++i)
-                #pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    part[wave - 1][i * FN + j][lane] = acc[i][j];
-        }
-        __syncthreads();
-        if (wave) return;
+    __shared__ f32x4 part[3][FM * FN][64];
+    if (wave) {
         #pragma unroll
-        for (int p = 0; p < WK - 1; ++p)
+        for (int i = 0; i < FM; ++i)
             #pragma unroll
-            for (int i = 0; i < FM; ++i)
-                #pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] += part[p][i * FN + j][lane];
+            for (int j = 0; j < FN; ++j)
+                part[wave - 1][i * FN + j][lane] = acc[i][j];
     }
-
-    const bool vec = N % 4 == 0;                 // y starts on 16 bytes
+    __syncthreads();
+    if (wave) return;
     #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const long n = n0 + g * (4 * FN) + j * 4;
-        float b[4];
+    for (int p = 0; p < 3; ++p)
         #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            b[r] = bias && n + r < N ? load_any(bias, bias_dt, n + r) : 0.f;
-        #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const long m = m0 + i * 16 + r16;
-            if (m >= M || n >= N) continue;
-            T* q = y + m * N + n;
-            union { T v[4]; u32x2 u[sizeof(T) / 2]; } o;
+        for (int i = 0; i < FM; ++i)
             #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                o.v[r] = from_f32<OT>(acc[i][j][r] + b[r]);
-            if (vec) {
-                #pragma unroll
-                for (int r = 0; r < (int)sizeof(T) / 2; ++r)
-                    reinterpret_cast<u32x2*>(q)[r] = o.u[r];
-            } else {
-                #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < N) q[r] = o.v[r];
-            }
-        }
-    }
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] += part[p][i * FN + j][lane];
+    store_rows<OT, FM, FN>(acc, y, M, N, m0 + r16, n0 + g * (4 * FN), bias,
+                           bias_dt);
 }
 
 template <int AT, bool VEC, int OT>
-void launch_direct(const void* x, const uint8_t* xs, long M, long K, long ldx,
-                   const uint8_t* wc, const uint8_t* ws, long N,
-                   const void* bias, int bias_dt, void* y, hipStream_t stream) {
+void launch_rows(const void* x, const uint8_t* xs, long M, long K, long ldx,
+                 const uint8_t* wc, const uint8_t* ws, long N,
+                 const void* bias, int bias_dt, void* y, int form,
+                 hipStream_t stream) {
     const int Kp = (int)((K + 127) / 128 * 128);
-    #define MX4_L(FM, FN, WK) do { \
-        const int tm = (WK == 1 ? 32 : 16) * FM, tn = (WK == 1 ? 32 : 16) * FN; \
-        hipLaunchKernelGGL((linear_direct_kernel<AT, VEC, OT, FM, FN, WK>), \
-            dim3((unsigned)((M + tm - 1) / tm), (unsigned)((N + tn - 1) / tn)), \
-            dim3(256), 0, stream, x, xs, M, (int)K, Kp, ldx, wc, ws, N, bias, \
-            bias_dt, (typename Elem<OT>::T*)y); } while (0)
-    if (M <= 16) MX4_L(1, 1, 4);
-    else if (M * N <= 1024L * 1024) MX4_L(2, 2, 4);
-    else MX4_L(2, 4, 1);
+    #define MX4_L(F) do { \
+        const long mt = (M + 16 * F - 1) / (16 * F), nt = (N + 16 * F - 1) / (16 * F); \
+        hipLaunchKernelGGL((linear_rows_kernel<AT, VEC, OT, F, F>), \
+            dim3((unsigned)(mt * nt)), dim3(256), 0, stream, x, xs, M, (int)K, \
+            Kp, ldx, wc, ws, N, bias, bias_dt, (typename Elem<OT>::T*)y, \
+            (int)nt); } while (0)
+    if (form == ROWS16) MX4_L(1);
+    else MX4_L(2);
     #undef MX4_L
 }
 
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
 }  // namespace
+
+int linear_form(long M, long K, long N, int dt, bool aligned) {
+    if (M <= 16) return ROWS16;
+    if (M * N <= 1024L * 1024) return ROWS32;
+    if (N <= 512) return ROUNDING;
+    return linear_q_form(M, K, N);
+}
+
+int linear_q_form(long M, long K, long N) {
+    if (M <= 16) return ROWS16;
+    if (M * N <= 1024L * 1024) return ROWS32;
+    return (M + 255) / 256 * ((N + 255) / 256) >= 256 ? TILES256 : TILES128;
+}
+
+size_t linear_bytes(int form, long M, long K) {
+    if (form < TILES128) return 0;
+    const long Kp = (K + 127) / 128 * 128;
+    return up256(M * (Kp / 2)) + M * (Kp / 32);
+}
 
 void linear(const void* x, int dt, long M, long K, long ldx,
             const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
-            int bias_dt, void* y, hipStream_t stream) {
+            int bias_dt, void* y, int form, void* work, hipStream_t stream) {
     const int es = dt == F32 ? 4 : 2;
     const bool vec = (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0;
-    #define MX4_ARGS x, nullptr, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream
+    if (form == ROUNDING) {
+        tiled(x, dt, vec, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream);
+        return;
+    }
+    if (form > ROUNDING) {
+        const long Kp = (K + 127) / 128 * 128;
+        uint8_t* xc = (uint8_t*)work;
+        uint8_t* xs = xc + up256(M * (Kp / 2));
+        quantize(x, dt, M, K, ldx, xc, xs, stream);
+        linear_q(xc, xs, M, K, wc, ws, N, bias, bias_dt, y, dt, form, stream);
+        return;
+    }
+    #define MX4_ARGS x, nullptr, M, K, ldx, wc, ws, N, bias, bias_dt, y, form, stream
     if (vec) {
-        if (dt == F32) launch_direct<F32, true, F32>(MX4_ARGS);
-        else if (dt == BF16) launch_direct<BF16, true, BF16>(MX4_ARGS);
-        else launch_direct<F16, true, F16>(MX4_ARGS);
+        if (dt == F32) launch_rows<F32, true, F32>(MX4_ARGS);
+        else if (dt == BF16) launch_rows<BF16, true, BF16>(MX4_ARGS);
+        else launch_rows<F16, true, F16>(MX4_ARGS);
     } else {
-        if (dt == F32) launch_direct<F32, false, F32>(MX4_ARGS);
-        else if (dt == BF16) launch_direct<BF16, false, BF16>(MX4_ARGS);
-        else launch_direct<F16, false, F16>(MX4_ARGS);
+        if (dt == F32) launch_rows<F32, false, F32>(MX4_ARGS);
+        else if (dt == BF16) launch_rows<BF16, false, BF16>(MX4_ARGS);
+        else launch_rows<F16, false, F16>(MX4_ARGS);
     }
     #undef MX4_ARGS
 }
 
 void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
-              int bias_dt, void* y, int dt, hipStream_t stream) {
-    #define MX4_ARGS xc, xs, M, K, 0, wc, ws, N, bias, bias_dt, y, stream
-    if (dt == F32) launch_direct<CODES, true, F32>(MX4_ARGS);
-    else if (dt == BF16) launch_direct<CODES, true, BF16>(MX4_ARGS);
-    else launch_direct<CODES, true, F16>(MX4_ARGS);
+              int bias_dt, void* y, int dt, int form, hipStream_t stream) {
+    if (form >= ROUNDING) {
+        tiled_q(xc, xs, M, K, wc, ws, N, bias, bias_dt, y, dt,
+                form == TILES256, stream);
+        return;
+    }
+    #define MX4_ARGS xc, xs, M, K, 0, wc, ws, N, bias, bias_dt, y, form, stream
+    if (dt == F32) launch_rows<CODES, true, F32>(MX4_ARGS);
+    else if (dt == BF16) launch_rows<CODES, true, BF16>(MX4_ARGS);
+    else launch_rows<CODES, true, F16>(MX4_ARGS);
     #undef MX4_ARGS
 }
 

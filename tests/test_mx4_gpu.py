@@ -122,9 +122,34 @@ def test_whole_numbers_are_exact(M, K, N):
         assert torch.equal(dw.double().cpu(), g.t() @ xv)
 
 
+@pytest.mark.parametrize('form', range(5))
+@pytest.mark.parametrize('M,K,N', SIZES + [(260, 1, 260), (129, 384, 70),
+                                           (700, 1000, 520)])
+def test_every_form_at_every_size(M, K, N, form):
+    ext = ops._native_or_die()
+    x = GRID[torch.randint(0, 8, (M, K))] * (torch.randint(0, 2, (M, K)) * 2 - 1)
+    w = GRID[torch.randint(0, 8, (N, K))] * (torch.randint(0, 2, (N, K)) * 2 - 1)
+    b = torch.randint(-8, 9, (N,)).float()
+    want = values(x.float()) @ values(w.float()).t() + b
+    wq = ops.mx4_quantize(w.float().cuda())
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1),
+                        (torch.float16, 2)):
+        base = torch.full((M, K + 9), math.nan, dtype=dtype, device='cuda')
+        for lo in (0, 1, 8):
+            xd = base[:, lo:lo + K]
+            xd.copy_(x)
+            y = ext.mx4_linear(xd, wq.codes, wq.scales, b.cuda(), form)
+            assert torch.equal(y.cpu(), want.to(dtype))
+            base.fill_(math.nan)
+        q = ops.mx4_quantize(x.to(dtype).cuda())
+        y = ext.mx4_linear_q(q.codes, q.scales, K, wq.codes, wq.scales,
+                             b.to(dtype).cuda(), code, form)
+        assert torch.equal(y.cpu(), want.to(dtype))
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('M', [1, 40, 3000])
-def test_strides_and_alignments(dtype, M):
+def test_strides_and_alignments_of_rows(dtype, M):
     base = torch.randn(M, 300).to(dtype).cuda()
     w = ops.mx4_quantize(torch.randn(96, 256).cuda())
     for lo in (0, 1, 8, 44):
