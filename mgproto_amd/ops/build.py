@@ -17,7 +17,8 @@ SRC = [os.path.join(_HERE, 'hip', 'mgproto_kernels.hip'),
        os.path.join(_HERE, 'hip', 'gemm1x1_kernels.hip'),
        os.path.join(_HERE, 'hip', 'mx4_quant.hip'),
        os.path.join(_HERE, 'hip', 'mx4_linear.hip'),
-       os.path.join(_HERE, 'hip', 'mx4_tiled.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_tiles.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_rounding.hip'),
        os.path.join(_HERE, 'hip', 'mx4_grad.hip'),
        os.path.join(_HERE, 'hip', 'grad_clip.hip'),
        os.path.join(_HERE, 'hip', 'mx4_bindings.hip')]

@@ -42,24 +42,25 @@ void check_rows(const Tensor& x, const char* what) {
     TORCH_CHECK(x.size(1) < (1L << 30), what, ": rows too long");
 }
 
-// codes [rows, Kp/2] and scales [rows, Kp/32] for rows of K elements
+// 4-bit rows of K elements, as mx4_common.h lays them out
 void check_packed(const Tensor& codes, const Tensor& scales, int64_t K,
                   const char* what) {
     TORCH_CHECK(codes.is_cuda() && codes.device() == scales.device(), what,
                 ": codes and scales on one GPU");
     TORCH_CHECK(codes.scalar_type() == at::kByte &&
                     scales.scalar_type() == at::kByte, what, ": uint8");
-    TORCH_CHECK(codes.dim() == 2 && scales.dim() == 2 &&
+    TORCH_CHECK(codes.dim() == 3 && scales.dim() == 3 &&
                     codes.is_contiguous() && scales.is_contiguous(), what,
-                ": contiguous matrices");
-    const int64_t Kp = (K + 127) / 128 * 128;
-    TORCH_CHECK(K >= 0 && K < (1L << 22) && codes.size(1) == Kp / 2 &&
-                    scales.size(1) == Kp / 32 &&
-                    codes.size(0) == scales.size(0), what,
-                ": codes ", codes.sizes(), " and scales ", scales.sizes(),
-                " do not hold rows of ", K);
-    TORCH_CHECK((uintptr_t)codes.data_ptr() % 16 == 0, what,
-                ": codes start on 16 bytes");
+                ": contiguous codes and scales");
+    TORCH_CHECK(K >= 0 && K < (1L << 22) &&
+                    codes.size(0) == mx4::steps_of(K) && codes.size(2) == 64 &&
+                    scales.size(0) == mx4::chunks_of(K) &&
+                    scales.size(2) == 16 && codes.size(1) == scales.size(1),
+                what, ": codes ", codes.sizes(), " and scales ",
+                scales.sizes(), " do not hold rows of ", K);
+    TORCH_CHECK(((uintptr_t)codes.data_ptr() |
+                 (uintptr_t)scales.data_ptr()) % 16 == 0, what,
+                ": codes and scales start on 16 bytes");
 }
 
 void check_bias(const c10::optional<Tensor>& bias, int64_t N,
@@ -79,10 +80,10 @@ std::tuple<Tensor, Tensor> quantize(const Tensor& x) {
     check_rows(x, "mx4_quantize");
     const int dt = dtype_code(x, "mx4_quantize");
     c10::DeviceGuard guard(x.device());
-    const int64_t R = x.size(0), K = x.size(1), Kp = (K + 127) / 128 * 128;
+    const int64_t R = x.size(0), K = x.size(1);
     auto opt = x.options().dtype(at::kByte);
-    auto codes = at::empty({R, Kp / 2}, opt);
-    auto scales = at::empty({R, Kp / 32}, opt);
+    auto codes = at::empty({mx4::steps_of(K), R, 64}, opt);
+    auto scales = at::empty({mx4::chunks_of(K), R, 16}, opt);
     mx4::quantize(x.data_ptr(), dt, R, K, R > 1 ? x.stride(0) : K,
                   codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
                   current_stream());
@@ -93,10 +94,10 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
                   int64_t dt) {
     check_packed(codes, scales, K, "mx4_dequantize");
     c10::DeviceGuard guard(codes.device());
-    auto out = at::empty({codes.size(0), K},
+    auto out = at::empty({codes.size(1), K},
                          codes.options().dtype(scalar_type(dt)));
     mx4::dequantize(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
-                    codes.size(0), K, out.data_ptr(), (int)dt,
+                    codes.size(1), K, out.data_ptr(), (int)dt,
                     current_stream());
     return out;
 }
@@ -115,7 +116,7 @@ int pick(int64_t form, int chosen) {
 Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws,
               const c10::optional<Tensor>& bias, int64_t form) {
     check_rows(x, "mx4_linear: input");
-    const int64_t M = x.size(0), K = x.size(1), N = wc.size(0);
+    const int64_t M = x.size(0), K = x.size(1), N = wc.size(1);
     check_packed(wc, ws, K, "mx4_linear: weight");
     TORCH_CHECK(x.device() == wc.device(), "mx4_linear: one GPU for all");
     check_bias(bias, N, x);
@@ -145,7 +146,7 @@ Tensor linear_q(const Tensor& xc, const Tensor& xs, int64_t K,
     check_packed(xc, xs, K, "mx4_linear: input");
     check_packed(wc, ws, K, "mx4_linear: weight");
     TORCH_CHECK(xc.device() == wc.device(), "mx4_linear: one GPU for all");
-    const int64_t M = xc.size(0), N = wc.size(0);
+    const int64_t M = xc.size(1), N = wc.size(1);
     check_bias(bias, N, xc);
     c10::DeviceGuard guard(xc.device());
     check_tiles(M, N);
@@ -173,7 +174,7 @@ Tensor grad_input(const Tensor& g, const Tensor& wc, const Tensor& ws,
     check_grad(g);
     check_packed(wc, ws, K, "mx4_linear: weight");
     const int64_t M = g.size(0), N = g.size(1);
-    TORCH_CHECK(wc.size(0) == N && g.device() == wc.device(),
+    TORCH_CHECK(wc.size(1) == N && g.device() == wc.device(),
                 "mx4_linear: output gradient does not match the weight");
     const int gd = dtype_code(g, "mx4_linear: output gradient");
     c10::DeviceGuard guard(g.device());
@@ -193,7 +194,7 @@ Tensor grad_weight(const Tensor& g, const Tensor& xc, const Tensor& xs,
     check_grad(g);
     check_packed(xc, xs, K, "mx4_linear: input");
     const int64_t M = g.size(0), N = g.size(1);
-    TORCH_CHECK(xc.size(0) == M && g.device() == xc.device(),
+    TORCH_CHECK(xc.size(1) == M && g.device() == xc.device(),
                 "mx4_linear: output gradient does not match the input");
     const int gd = dtype_code(g, "mx4_linear: output gradient");
     c10::DeviceGuard guard(g.device());

@@ -7,9 +7,14 @@
 //   q = x * 2^-E to the nearest value, ties to the even code, 6 at most.
 // A block with a NaN or an infinity has byte 255 and reads as NaN.
 //
-// Storage: rows padded to Kp = multiple of 128 elements (one matrix-core
-// step), codes [rows, Kp/2] with the low nibble first, scales [rows, Kp/32].
-// Codes and scales of the padding are 0, so it adds nothing to a product.
+// Storage of [R, K], for the matrix cores' reads: rows are padded with zeros to
+// Kp, a multiple of 128 elements (one step of v_mfma_scale_f32_16x16x128), and
+//   codes  [Kp/128][R][64]: a step's 64 bytes of all rows in one piece, so that
+//          any run of rows is one run of memory for a step;
+//   scales [up(Kp/512)][R][16]: of four steps, byte 4*g + s is the scale of
+//          block g of step s, so that lane group g has its four in one word and
+//          the instruction picks the byte of the step.
+// Codes: low nibble first. Scales of the padding are 0 as well.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -155,8 +160,20 @@ static __device__ __forceinline__ void load8_tail(
     }
 }
 
-// Everything below takes element strides in elements, code and scale rows as
-// Kp/2 and Kp/32 bytes, and runs on `stream`. Sizes are checked by callers.
+constexpr int STEP = 128;              // elements of a step
+
+static inline __host__ __device__ long steps_of(long K) { return (K + 127) / 128; }
+static inline __host__ __device__ long chunks_of(long K) { return (K + 511) / 512; }
+static inline size_t code_bytes(long R, long K) { return (size_t)steps_of(K) * R * 64; }
+static inline size_t scale_bytes(long R, long K) { return (size_t)chunks_of(K) * R * 16; }
+
+// where block b (of 32) of a row has its scale
+static __device__ __forceinline__ size_t scale_at(long R, long row, int b) {
+    return ((size_t)(b >> 4) * R + row) * 16 + (b & 3) * 4 + (b >> 2 & 3);
+}
+
+// Everything below takes strides in elements and runs on `stream`. Sizes are
+// checked by callers.
 
 void quantize(const void* x, int dt, long rows, long K, long ldx,
               uint8_t* codes, uint8_t* scales, hipStream_t stream);

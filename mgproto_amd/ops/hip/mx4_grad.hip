@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 #include "mx4_common.h"
+#include "mx4_linear.h"
 
 namespace mx4 {
 namespace {
@@ -73,34 +74,29 @@ void parts_t_kernel(const typename Elem<DT>::T* __restrict__ g, long R, long C,
     }
 }
 
-// codes [R, Kp/2] -> out [K][Rp]
+// 4-bit rows [R, K] -> out [K][Rp]
 __global__ __launch_bounds__(256)
 void values_t_kernel(const uint8_t* __restrict__ codes,
                      const uint8_t* __restrict__ scales, long R, long K,
-                     int Kp, long Rp, __bf16* __restrict__ out) {
+                     long Rp, __bf16* __restrict__ out) {
     __shared__ float tile[64][65];
     const long r0 = (long)blockIdx.x * 64, k0 = (long)blockIdx.y * 64;
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     {   // 8 codes a thread, 32 rows at a time
         const int u = threadIdx.x & 7, rr = threadIdx.x >> 3;
+        const int k = (int)k0 + u * 8;
         for (int i = rr; i < 64; i += 32) {
             const long r = r0 + i;
             unsigned c = 0, byte = 0;
-            if (r < R) {                       // 64 divides Kp
-                c = reinterpret_cast<const unsigned*>(
-                    codes + r * (Kp >> 1))[(k0 >> 3) + u];
-                byte = scales[r * (Kp >> 5) + (k0 >> 5) + (u >> 2)];
+            if (r < R) {                       // 64 divides a step
+                c = reinterpret_cast<const unsigned*>(codes)[
+                    ((size_t)(k >> 7) * R + r) * 16 + (k >> 3 & 15)];
+                byte = scales[scale_at(R, r, k >> 5)];
             }
-            const float s = byte == 255u ? 1.f : scale_f32(byte);
-            f32x2 f[4];
-            f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
-            f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
-            f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
-            f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+            float f[8];
+            values8(c, byte, f);
             #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                tile[i][u * 8 + e] = byte == 255u
-                    ? __uint_as_float(0x7fc00000u) : f[e >> 1][e & 1];
+            for (int e = 0; e < 8; ++e) tile[i][u * 8 + e] = f[e];
         }
     }
     __syncthreads();
@@ -114,12 +110,6 @@ void values_t_kernel(const uint8_t* __restrict__ codes,
 // ---------------------------------------------------------------------------
 // C[M,N] = sum_p A_p[M,Kc] B[N,Kc]^T, rows of multiples of 64 elements
 // ---------------------------------------------------------------------------
-
-static __device__ __forceinline__ void to_lds16(const void* g, void* l) {
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void*)(uintptr_t)g,
-        (__attribute__((address_space(3))) void*)(uint32_t)(uintptr_t)l, 16, 0, 0);
-}
 
 // Grid (row tiles, column tiles, splits). A split sums its share of the
 // steps of all parts; with more than one split C is fp32 [splits][M][N].
@@ -152,8 +142,8 @@ void product_nt_kernel(const unsigned short* __restrict__ A, long lda,
             const int r = call * 8 + (lane >> 3), c = lane & 7;
             const int ca = c ^ ((r >> 1) & 7);
             const int cn = c ^ (((r >> 4) & 3) | ((r >> 1) & 1) << 2);
-            to_lds16(a + min(m0 + r, M - 1) * lda + ca * 8, &lds[buf][0][call * 512]);
-            to_lds16(b + min(n0 + r, N - 1) * ldb + cn * 8, &lds[buf][1][call * 512]);
+            copy16_to_lds(a + min(m0 + r, M - 1) * lda + ca * 8, &lds[buf][0][call * 512]);
+            copy16_to_lds(b + min(n0 + r, N - 1) * ldb + cn * 8, &lds[buf][1][call * 512]);
         }
     };
 
@@ -356,13 +346,13 @@ void grad_input(const void* g, int g_dt, bool g_aligned, long M, long N,
                 long K, const uint8_t* wc, const uint8_t* ws, void* dx,
                 int dx_dt, void* work, hipStream_t stream) {
     const long Np = up64(N);
-    const int Kp = (int)((K + 127) / 128 * 128), P = parts_of(g_dt);
+    const int P = parts_of(g_dt);
     char* at = (char*)work;
     __bf16* wt = (__bf16*)at;
     at += up256((size_t)K * Np * 2);
     hipLaunchKernelGGL(values_t_kernel,
                        dim3((unsigned)(Np / 64), (unsigned)((K + 63) / 64)),
-                       dim3(256), 0, stream, wc, ws, N, K, Kp, Np, wt);
+                       dim3(256), 0, stream, wc, ws, N, K, Np, wt);
     const unsigned short* a = (const unsigned short*)g;
     if (!in_place(N, g_dt, g_aligned)) {
         unsigned short* parts = (unsigned short*)at;
@@ -393,7 +383,7 @@ void grad_weight(const void* g, int g_dt, long M, long N, long K,
                  const uint8_t* xc, const uint8_t* xs, void* dw, int dw_dt,
                  void* work, hipStream_t stream) {
     const long Mp = up64(M);
-    const int Kp = (int)((K + 127) / 128 * 128), P = parts_of(g_dt);
+    const int P = parts_of(g_dt);
     char* at = (char*)work;
     __bf16* xt = (__bf16*)at;
     at += up256((size_t)K * Mp * 2);
@@ -401,7 +391,7 @@ void grad_weight(const void* g, int g_dt, long M, long N, long K,
     at += up256((size_t)P * N * Mp * 2);
     hipLaunchKernelGGL(values_t_kernel,
                        dim3((unsigned)(Mp / 64), (unsigned)((K + 63) / 64)),
-                       dim3(256), 0, stream, xc, xs, M, K, Kp, Mp, xt);
+                       dim3(256), 0, stream, xc, xs, M, K, Mp, xt);
     const dim3 grid((unsigned)(Mp / 64), (unsigned)((N + 63) / 64));
     #define MX4_G(DT) \
         hipLaunchKernelGGL((parts_t_kernel<DT>), grid, dim3(256), 0, stream, \

@@ -13,10 +13,40 @@ static __device__ __forceinline__ i32x8 wide(i32x4 v) {
     return (i32x8){v.x, v.y, v.z, v.w, 0, 0, 0, 0};
 }
 
-static __device__ __forceinline__ float load_any(const void* p, int dt, long i) {
-    if (dt == F32) return reinterpret_cast<const float*>(p)[i];
-    if (dt == BF16) return (float)reinterpret_cast<const __bf16*>(p)[i];
-    return (float)reinterpret_cast<const _Float16*>(p)[i];
+// the values of 8 codes under one scale byte
+static __device__ __forceinline__ void values8(unsigned c, unsigned byte,
+                                               float (&f)[8]) {
+    const float s = byte == 255u ? 1.f : scale_f32(byte);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
+    const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+    const float nan = __uint_as_float(0x7fc00000u);
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+    f[4] = d.x; f[5] = d.y; f[6] = e.x; f[7] = e.y;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = byte == 255u ? nan : f[i];
+}
+
+#define MX4_GLOBAL(p) (const __attribute__((address_space(1))) void*)(uintptr_t)(p)
+#define MX4_LDS(p) (__attribute__((address_space(3))) void*)(uint32_t)(uintptr_t)(p)
+// 16 bytes a lane from memory into LDS, past the registers: lane i's go to
+// l + 16 i, with l the same in the wave
+static __device__ __forceinline__ void copy16_to_lds(const void* g, void* l) {
+    __builtin_amdgcn_global_load_lds(MX4_GLOBAL(g), MX4_LDS(l), 16, 0, 0);
+}
+
+// In LDS a step's codes are rows of 64 bytes, four pieces of 16; piece g of row
+// r lies at g ^ key(r). A read takes 16 bytes a lane, lane group g piece g of 16
+// rows, and is served in four turns: lanes 0-3, 12-15 and 20-27 together, 4-11,
+// 16-19 and 28-31 together, and so on. These keys put a turn's 16 pieces on 16
+// different places of the 256 bytes that the banks give at once (measured: 4
+// cycles a read, 8 without a key).
+// rows of x are read 16 consecutive ones at a time
+static __device__ __forceinline__ int x_key(int r) { return r >> 1 & 3; }
+// rows of W in four runs of four, 4*FN apart
+template <int FN> static __device__ __forceinline__ int w_key(int r) {
+    return r / (4 * FN) & 2;
 }
 
 // maximum over the four lanes of a quad
@@ -25,33 +55,54 @@ static __device__ __forceinline__ unsigned quad_max(unsigned m) {
     return max(m, (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));
 }
 
+// 4*FN values of the bias from column n on, 0 where there is none
+template <int FN>
+static __device__ __forceinline__ void load_bias(float (&b)[4 * FN],
+                                                 const void* bias, int dt,
+                                                 long n, long N) {
+    #pragma unroll
+    for (int i = 0; i < 4 * FN; ++i) b[i] = 0.f;
+    if (!bias) return;
+    if (dt == F32) {
+        const float* p = reinterpret_cast<const float*>(bias);
+        #pragma unroll
+        for (int i = 0; i < 4 * FN; ++i) b[i] = p[min(n + i, N - 1)];
+    } else {
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(bias);
+        unsigned short u[4 * FN];
+        #pragma unroll
+        for (int i = 0; i < 4 * FN; ++i) u[i] = p[min(n + i, N - 1)];
+        #pragma unroll
+        for (int i = 0; i < 4 * FN; ++i)
+            b[i] = dt == BF16 ? __uint_as_float((unsigned)u[i] << 16)
+                              : (float)__builtin_bit_cast(_Float16, u[i]);
+    }
+}
+
 // Rows m, m + 16, ... of y from column n on: 4*FN consecutive columns a lane.
 // Pieces of 16 bytes where rows start on them, single elements elsewhere.
 template <int OT, int FM, int FN>
 static __device__ __forceinline__ void store_rows(
         const f32x4 (&acc)[FM][FN], typename Elem<OT>::T* y, long M, long N,
-        long m, long n, const void* bias, int bias_dt) {
+        long m, long n, const float (&b)[4 * FN]) {
     using T = typename Elem<OT>::T;
     constexpr int PER = OT == F32 ? 1 : (FN % 2 ? 1 : 2);   // tiles a piece
     constexpr int W = 4 * PER;                              // columns a piece
     const bool vec = N % W == 0;
     #pragma unroll
-    for (int j = 0; j < FN; j += PER) {
-        const long c = n + j * 4;
-        float b[W];
+    for (int i = 0; i < FM; ++i) {
+        const long row = m + i * 16;
+        if (row >= M) continue;
         #pragma unroll
-        for (int r = 0; r < W; ++r)
-            b[r] = bias && c + r < N ? load_any(bias, bias_dt, c + r) : 0.f;
-        #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-            const long row = m + i * 16;
-            if (row >= M || c >= N) continue;
+        for (int j = 0; j < FN; j += PER) {
+            const long c = n + j * 4;
             T* q = y + row * N + c;
             union { T v[W]; u32x2 h[W * sizeof(T) / 8]; } o;
             #pragma unroll
             for (int r = 0; r < W; ++r)
-                o.v[r] = from_f32<OT>(acc[i][j + r / 4][r % 4] + b[r]);
+                o.v[r] = from_f32<OT>(acc[i][j + r / 4][r % 4] + b[j * 4 + r]);
             if (vec) {
+                if (c >= N) continue;
                 if constexpr (W * sizeof(T) == 16)
                     *reinterpret_cast<u32x4*>(q) =
                         (u32x4){o.h[0].x, o.h[0].y, o.h[1].x, o.h[1].y};
@@ -66,12 +117,13 @@ static __device__ __forceinline__ void store_rows(
     }
 }
 
-// mx4_tiled.hip
-void tiled_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
-             const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
-             int bias_dt, void* y, int dt, bool large, hipStream_t stream);
-void tiled(const void* x, int dt, bool vec, long M, long K, long ldx,
+// mx4_tiles.hip
+void tiles(const uint8_t* xc, const uint8_t* xs, long M, long K,
            const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
-           int bias_dt, void* y, hipStream_t stream);
+           int bias_dt, void* y, int dt, bool large, hipStream_t stream);
+// mx4_rounding.hip
+void rounding(const void* x, int dt, bool vec, long M, long K, long ldx,
+              const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
+              int bias_dt, void* y, hipStream_t stream);
 
 }  // namespace mx4

@@ -48,7 +48,7 @@ static __device__ __forceinline__ i32x4 round_block(
 template <int AT, bool VEC, int OT, int FM, int FN>
 __global__ __launch_bounds__(256)
 void linear_rows_kernel(const void* __restrict__ xv,
-                        const uint8_t* __restrict__ xs, long M, int K, int Kp,
+                        const uint8_t* __restrict__ xs, long M, int K, int steps,
                         long ldx, const uint8_t* __restrict__ wc,
                         const uint8_t* __restrict__ ws, long N,
                         const void* __restrict__ bias, int bias_dt,
@@ -57,15 +57,13 @@ void linear_rows_kernel(const void* __restrict__ xv,
     const int r16 = lane & 15, g = lane >> 4;
     const long m0 = (long)(blockIdx.x / nt) * (16 * FM);
     const long n0 = (long)(blockIdx.x % nt) * (16 * FN);
-    const int cb = Kp >> 1, sb = Kp >> 5;        // bytes of a row
-
-    const uint8_t* wrow[FN];
-    const uint8_t* wsrow[FN];
+    const uint8_t* wp[FN];
+    const uint8_t* wsp[FN];
     #pragma unroll
     for (int j = 0; j < FN; ++j) {
         const long n = min(n0 + (r16 >> 2) * (4 * FN) + j * 4 + (r16 & 3), N - 1);
-        wrow[j] = wc + n * cb + g * 16;
-        wsrow[j] = ws + n * sb + g;
+        wp[j] = wc + n * 64 + g * 16;
+        wsp[j] = ws + n * 16 + g * 4;
     }
     long xrow[FM];
     #pragma unroll
@@ -77,22 +75,21 @@ void linear_rows_kernel(const void* __restrict__ xv,
         #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
 
-    const int steps = Kp >> 7;
     for (int s = wave; s < steps; s += 4) {
         i32x4 w[FN], x[FM];
         int wb[FN], xb[FM];
         #pragma unroll
         for (int j = 0; j < FN; ++j) {
-            w[j] = *reinterpret_cast<const i32x4*>(wrow[j] + s * 64);
-            wb[j] = wsrow[j][s * 4];
+            w[j] = *reinterpret_cast<const i32x4*>(wp[j] + (size_t)s * N * 64);
+            wb[j] = wsp[j][(size_t)(s >> 2) * N * 16 + (s & 3)];
         }
         #pragma unroll
         for (int i = 0; i < FM; ++i) {
             if constexpr (AT == CODES) {
-                const uint8_t* xc = reinterpret_cast<const uint8_t*>(xv);
                 x[i] = *reinterpret_cast<const i32x4*>(
-                    xc + xrow[i] * cb + s * 64 + g * 16);
-                xb[i] = xs[xrow[i] * sb + s * 4 + g];
+                    reinterpret_cast<const uint8_t*>(xv)
+                    + ((size_t)s * M + xrow[i]) * 64 + g * 16);
+                xb[i] = xs[scale_at(M, xrow[i], s * 4 + g)];
             } else {
                 using E = typename Elem<AT == CODES ? F32 : AT>::T;
                 x[i] = round_block<AT == CODES ? F32 : AT, VEC>(
@@ -125,8 +122,9 @@ void linear_rows_kernel(const void* __restrict__ xv,
             #pragma unroll
             for (int j = 0; j < FN; ++j)
                 acc[i][j] += part[p][i * FN + j][lane];
-    store_rows<OT, FM, FN>(acc, y, M, N, m0 + r16, n0 + g * (4 * FN), bias,
-                           bias_dt);
+    float b[4 * FN];
+    load_bias<FN>(b, bias, bias_dt, n0 + g * (4 * FN), N);
+    store_rows<OT, FM, FN>(acc, y, M, N, m0 + r16, n0 + g * (4 * FN), b);
 }
 
 template <int AT, bool VEC, int OT>
@@ -134,12 +132,11 @@ void launch_rows(const void* x, const uint8_t* xs, long M, long K, long ldx,
                  const uint8_t* wc, const uint8_t* ws, long N,
                  const void* bias, int bias_dt, void* y, int form,
                  hipStream_t stream) {
-    const int Kp = (int)((K + 127) / 128 * 128);
     #define MX4_L(F) do { \
         const long mt = (M + 16 * F - 1) / (16 * F), nt = (N + 16 * F - 1) / (16 * F); \
         hipLaunchKernelGGL((linear_rows_kernel<AT, VEC, OT, F, F>), \
             dim3((unsigned)(mt * nt)), dim3(256), 0, stream, x, xs, M, (int)K, \
-            Kp, ldx, wc, ws, N, bias, bias_dt, (typename Elem<OT>::T*)y, \
+            (int)steps_of(K), ldx, wc, ws, N, bias, bias_dt, (typename Elem<OT>::T*)y, \
             (int)nt); } while (0)
     if (form == ROWS16) MX4_L(1);
     else MX4_L(2);
@@ -165,8 +162,7 @@ int linear_q_form(long M, long K, long N) {
 
 size_t linear_bytes(int form, long M, long K) {
     if (form < TILES128) return 0;
-    const long Kp = (K + 127) / 128 * 128;
-    return up256(M * (Kp / 2)) + M * (Kp / 32);
+    return up256(code_bytes(M, K)) + scale_bytes(M, K);
 }
 
 void linear(const void* x, int dt, long M, long K, long ldx,
@@ -175,13 +171,12 @@ void linear(const void* x, int dt, long M, long K, long ldx,
     const int es = dt == F32 ? 4 : 2;
     const bool vec = (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0;
     if (form == ROUNDING) {
-        tiled(x, dt, vec, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream);
+        rounding(x, dt, vec, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream);
         return;
     }
     if (form > ROUNDING) {
-        const long Kp = (K + 127) / 128 * 128;
         uint8_t* xc = (uint8_t*)work;
-        uint8_t* xs = xc + up256(M * (Kp / 2));
+        uint8_t* xs = xc + up256(code_bytes(M, K));
         quantize(x, dt, M, K, ldx, xc, xs, stream);
         linear_q(xc, xs, M, K, wc, ws, N, bias, bias_dt, y, dt, form, stream);
         return;
@@ -203,8 +198,8 @@ void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
               int bias_dt, void* y, int dt, int form, hipStream_t stream) {
     if (form >= ROUNDING) {
-        tiled_q(xc, xs, M, K, wc, ws, N, bias, bias_dt, y, dt,
-                form == TILES256, stream);
+        tiles(xc, xs, M, K, wc, ws, N, bias, bias_dt, y, dt,
+              form == TILES256, stream);
         return;
     }
     #define MX4_ARGS xc, xs, M, K, 0, wc, ws, N, bias, bias_dt, y, form, stream

@@ -1,136 +1,171 @@
 // Rows to MX4 blocks and back. See mx4_common.h for the format.
 //
 // Bound by memory: 2 (or 4) bytes in and 0.53 out an element, the reverse for
-// reading back. Four lanes share a block, 8 elements each, so that a wave
-// reads 1 KB (16-bit) or 2 KB (fp32) in one piece and writes 256 bytes of
-// codes in one; the block's maximum goes over the four lanes by two shuffles.
+// reading back. Four lanes share a block, 8 elements each, and its maximum goes
+// over them by two lane exchanges. A wave takes 512 elements of a row (or 128
+// of four rows, where rows are that short), so that it reads in pieces of 1 KB
+// or more, and four such pieces at once to have enough loads under way.
 
 #include <hip/hip_runtime.h>
 
 #include "mx4_common.h"
+#include "mx4_linear.h"
 
 namespace mx4 {
 namespace {
 
-template <int DT, bool VEC>
+constexpr int ROWS = 4;       // pieces a wave has under way
+
+// LPR lanes hold a row's piece: 64 of them 512 elements, 16 of them 128
+template <int DT, bool VEC, int LPR>
 __global__ __launch_bounds__(256)
-void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long rows,
-                     int K, int Kp, long ldx, unsigned* __restrict__ codes,
-                     uint8_t* __restrict__ scales) {
+void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long R, int K,
+                     int steps, long ldx, uint8_t* __restrict__ codes,
+                     uint8_t* __restrict__ scales, int chunks) {
     constexpr int W = DT == F32 ? 2 : 1;
-    const int upr = Kp >> 3;                     // units of 8 in a row
-    const long total = rows * upr;
-    const long step = (long)gridDim.x * 256;
-    for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
-        const long row = t / upr;
-        const int k = (int)(t - row * upr) << 3;
-        u32x4 u[W];
-        const typename Elem<DT>::T* p = x + row * ldx + k;
+    constexpr int RPW = 64 / LPR;                // rows side by side
+    const int lane = threadIdx.x & 63, sub = lane % LPR;
+    const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int chunk = (int)(wave % chunks);
+    const long row0 = wave / chunks * (RPW * ROWS) + lane / LPR;
+    const int k = chunk * 512 + sub * 8, s = k >> 7;
+    u32x4 u[ROWS][W];
+    #pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const long row = row0 + i * RPW;
+        const typename Elem<DT>::T* p = x + min(row, R - 1) * ldx + k;
         if (VEC && k + 8 <= K) {
             #pragma unroll
-            for (int i = 0; i < W; ++i)
-                u[i] = reinterpret_cast<const u32x4*>(p)[i];
+            for (int e = 0; e < W; ++e)
+                u[i][e] = reinterpret_cast<const u32x4*>(p)[e];
         } else {
-            load8_tail<DT>(p, K - k, u);
+            load8_tail<DT>(p, K - k, u[i]);
         }
-        // upr is a multiple of 16 and so is the count of live lanes of a
-        // wave: the four lanes of a block are live together
-        unsigned m = absmax_bits<DT>(u, W);
-        m = max(m, (unsigned)__shfl_xor((int)m, 1));
-        m = max(m, (unsigned)__shfl_xor((int)m, 2));
-        const unsigned byte = scale_byte<DT>(m);
-        codes[t] = byte == 255u ? 0u : codes8<DT>(u, scale_f32(byte));
-        if ((t & 3) == 0) scales[t >> 2] = (uint8_t)byte;
+    }
+    #pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const long row = row0 + i * RPW;
+        const unsigned byte = scale_byte<DT>(quad_max(absmax_bits<DT>(u[i], W)));
+        const unsigned c = codes8<DT>(u[i], scale_f32(byte));
+        // block g of four steps lies in lanes 4g, 4g + 16, ...; behind the
+        // row the elements were zeros and so are the bytes
+        unsigned four = byte;
+        if constexpr (LPR == 64) {
+            four |= (unsigned)__shfl((int)byte, (lane & 15) + 16) << 8;
+            four |= (unsigned)__shfl((int)byte, (lane & 15) + 32) << 16;
+            four |= (unsigned)__shfl((int)byte, (lane & 15) + 48) << 24;
+        }
+        if (row >= R) continue;
+        if (s < steps)
+            reinterpret_cast<unsigned*>(codes)[
+                ((size_t)s * R + row) * 16 + (sub & 15)] = byte == 255u ? 0u : c;
+        if (sub < 16 && (sub & 3) == 0)
+            reinterpret_cast<unsigned*>(scales)[
+                ((size_t)chunk * R + row) * 4 + (sub >> 2)] = four;
     }
 }
 
-template <int DT, bool VEC>
+template <int DT, bool VEC, int LPR>
 __global__ __launch_bounds__(256)
-void dequantize_kernel(const unsigned* __restrict__ codes,
-                       const uint8_t* __restrict__ scales, long rows, int K,
-                       int Kp, typename Elem<DT>::T* __restrict__ out) {
+void dequantize_kernel(const uint8_t* __restrict__ codes,
+                       const uint8_t* __restrict__ scales, long R, int K,
+                       typename Elem<DT>::T* __restrict__ out, int chunks) {
     using T = typename Elem<DT>::T;
-    const int upr = (K + 7) >> 3;
-    const long total = rows * upr;
-    const long step = (long)gridDim.x * 256;
-    for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
-        const long row = t / upr;
-        const int k = (int)(t - row * upr) << 3;
-        const unsigned c = codes[row * (Kp >> 3) + (k >> 3)];
-        const unsigned byte = scales[row * (Kp >> 5) + (k >> 5)];
-        const float s = byte == 255u ? 1.f : scale_f32(byte);
-        f32x2 f[4];
-        f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
-        f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
-        f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
-        f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+    constexpr int RPW = 64 / LPR;
+    const int lane = threadIdx.x & 63, sub = lane % LPR;
+    const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int chunk = (int)(wave % chunks);
+    const long row0 = wave / chunks * (RPW * ROWS) + lane / LPR;
+    const int k = chunk * 512 + sub * 8;
+    if (k >= K) return;
+    unsigned c[ROWS], byte[ROWS];
+    #pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const long row = min(row0 + i * RPW, R - 1);
+        c[i] = reinterpret_cast<const unsigned*>(codes)[
+            ((size_t)(k >> 7) * R + row) * 16 + (sub & 15)];
+        byte[i] = scales[scale_at(R, row, k >> 5)];
+    }
+    #pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const long row = row0 + i * RPW;
+        if (row >= R) continue;
         union { T v[8]; u32x4 u[sizeof(T) / 2]; } o;
+        float f[8];
+        values8(c[i], byte[i], f);
         #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            o.v[i] = from_f32<DT>(byte == 255u ? __uint_as_float(0x7fc00000u)
-                                               : f[i >> 1][i & 1]);
+        for (int e = 0; e < 8; ++e) o.v[e] = from_f32<DT>(f[e]);
         T* q = out + row * K + k;
         if (VEC) {
             #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-                reinterpret_cast<u32x4*>(q)[i] = o.u[i];
+            for (int e = 0; e < (int)sizeof(T) / 2; ++e)
+                reinterpret_cast<u32x4*>(q)[e] = o.u[e];
         } else {
-            for (int i = 0; i < 8 && k + i < K; ++i) q[i] = o.v[i];
+            #pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < K) q[e] = o.v[e];
         }
     }
 }
 
-unsigned grid_for(long total) {
-    const long blocks = (total + 255) / 256;
-    return (unsigned)(blocks < 256 * 32 ? blocks : 256 * 32);
+// blocks of four waves; short rows lie four side by side
+unsigned blocks_for(long R, long K, bool shortrow) {
+    const long waves = shortrow ? (R + 4 * ROWS - 1) / (4 * ROWS)
+                                : (R + ROWS - 1) / ROWS * chunks_of(K);
+    return (unsigned)((waves + 3) / 4);
 }
 
 }  // namespace
 
 void quantize(const void* x, int dt, long rows, long K, long ldx,
               uint8_t* codes, uint8_t* scales, hipStream_t stream) {
-    const int Kp = (int)((K + 127) / 128 * 128);
-    const long total = rows * (Kp / 8);
-    if (total == 0) return;
+    if (rows == 0 || K == 0) return;
     const int es = dt == F32 ? 4 : 2;
     const bool vec = (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0;
-    #define MX4_Q(DT, V) \
-        hipLaunchKernelGGL((quantize_kernel<DT, V>), dim3(grid_for(total)), \
-                           dim3(256), 0, stream, \
-                           (const typename Elem<DT>::T*)x, rows, (int)K, Kp, \
-                           ldx, (unsigned*)codes, scales)
+    const bool shortrow = K <= 128;
+    const dim3 grid(blocks_for(rows, K, shortrow));
+    #define MX4_Q(DT, V, L) \
+        hipLaunchKernelGGL((quantize_kernel<DT, V, L>), grid, dim3(256), 0, \
+                           stream, (const typename Elem<DT>::T*)x, rows, \
+                           (int)K, (int)steps_of(K), ldx, codes, scales, \
+                           (int)chunks_of(K))
+    #define MX4_L(DT, V) do { if (shortrow) MX4_Q(DT, V, 16); \
+                              else MX4_Q(DT, V, 64); } while (0)
     if (vec) {
-        if (dt == F32) MX4_Q(F32, true);
-        else if (dt == BF16) MX4_Q(BF16, true);
-        else MX4_Q(F16, true);
+        if (dt == F32) MX4_L(F32, true);
+        else if (dt == BF16) MX4_L(BF16, true);
+        else MX4_L(F16, true);
     } else {
-        if (dt == F32) MX4_Q(F32, false);
-        else if (dt == BF16) MX4_Q(BF16, false);
-        else MX4_Q(F16, false);
+        if (dt == F32) MX4_L(F32, false);
+        else if (dt == BF16) MX4_L(BF16, false);
+        else MX4_L(F16, false);
     }
+    #undef MX4_L
     #undef MX4_Q
 }
 
 void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
                 long K, void* out, int dt, hipStream_t stream) {
-    const int Kp = (int)((K + 127) / 128 * 128);
-    const long total = rows * ((K + 7) / 8);
-    if (total == 0) return;
+    if (rows == 0 || K == 0) return;
     const bool vec = K % 8 == 0;     // fresh outputs start on 16 bytes
-    #define MX4_D(DT, V) \
-        hipLaunchKernelGGL((dequantize_kernel<DT, V>), dim3(grid_for(total)), \
-                           dim3(256), 0, stream, (const unsigned*)codes, \
-                           scales, rows, (int)K, Kp, \
-                           (typename Elem<DT>::T*)out)
+    const bool shortrow = K <= 128;
+    const dim3 grid(blocks_for(rows, K, shortrow));
+    #define MX4_D(DT, V, L) \
+        hipLaunchKernelGGL((dequantize_kernel<DT, V, L>), grid, dim3(256), 0, \
+                           stream, codes, scales, rows, (int)K, \
+                           (typename Elem<DT>::T*)out, (int)chunks_of(K))
+    #define MX4_L(DT, V) do { if (shortrow) MX4_D(DT, V, 16); \
+                              else MX4_D(DT, V, 64); } while (0)
     if (vec) {
-        if (dt == F32) MX4_D(F32, true);
-        else if (dt == BF16) MX4_D(BF16, true);
-        else MX4_D(F16, true);
+        if (dt == F32) MX4_L(F32, true);
+        else if (dt == BF16) MX4_L(BF16, true);
+        else MX4_L(F16, true);
     } else {
-        if (dt == F32) MX4_D(F32, false);
-        else if (dt == BF16) MX4_D(BF16, false);
-        else MX4_D(F16, false);
+        if (dt == F32) MX4_L(F32, false);
+        else if (dt == BF16) MX4_L(BF16, false);
+        else MX4_L(F16, false);
     }
+    #undef MX4_L
     #undef MX4_D
 }
 

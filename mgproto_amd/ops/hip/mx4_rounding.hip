@@ -1,0 +1,203 @@
+// Products whose rows are rounded on the way: y = Q(x) W^T + bias for many rows
+// and few columns, where the time is x's way from memory.
+//
+// A block of 128 rows takes all columns it can (up to 256), so that x is read
+// and rounded once for each 256 of them. Two buffers of 256 elements: while the
+// matrix cores work on one, the weights' codes go into the other past the
+// registers, and the next rows of x come into registers, are rounded there
+// (four lanes share a block, two lane exchanges for its maximum) and written as
+// codes. One barrier a buffer.
+
+#include <hip/hip_runtime.h>
+
+#include "mx4_common.h"
+#include "mx4_linear.h"
+
+namespace mx4 {
+namespace {
+
+template <int DT, bool VEC, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN)
+void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
+                     int steps, long ldx, const uint8_t* __restrict__ wc,
+                     const uint8_t* __restrict__ ws, long N,
+                     const void* __restrict__ bias, int bias_dt,
+                     typename Elem<DT>::T* __restrict__ y, int nt, int total) {
+    constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int W = DT == F32 ? 2 : 1;
+    constexpr int UNITS = BM * 32 / THREADS;     // of 8 elements, 32 a row
+    constexpr int CALLS = BN / 16;               // copies of a step's codes
+    // codes of two steps; x's scale bytes: 2*g + s of a row; W's as stored
+    __shared__ __attribute__((aligned(16))) uint8_t xl[2][2][BM * 64];
+    __shared__ __attribute__((aligned(16))) uint8_t wl[2][2][BN * 64];
+    __shared__ __attribute__((aligned(16))) uint8_t xsl[2][BM * 8];
+    __shared__ __attribute__((aligned(16))) uint8_t wsl[2][BN * 16];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int wm = (wave / WN) * (FM * 16), wn = (wave % WN) * (FN * 16);
+
+    // Blocks go round the 8 dies; a die has a run of tiles, the columns of the
+    // same rows one after the other, so that x comes from its L2 again.
+    const int xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+    const int t = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
+    const long m0 = (long)(t / nt) * BM, n0 = (long)(t % nt) * BN;
+    const int lastw = (int)min((long)BN, N - n0) - 1;
+    const int lastx = (int)min((long)BM, M - m0) - 1;
+    const int turns = (steps + 1) >> 1;
+
+    auto send_w = [&](int k, int buf) {
+        #pragma unroll
+        for (int q = 0; q < 2 * CALLS / WAVES; ++q) {
+            const int call = q * WAVES + wave;
+            const int s = call / CALLS, c = call % CALLS;
+            if (2 * k + s >= steps) break;
+            const int r = c * 16 + (lane >> 2);
+            copy16_to_lds(wc + ((size_t)(2 * k + s) * N + n0 + min(r, lastw)) * 64
+                              + ((lane & 3) ^ w_key<FN>(r)) * 16,
+                          wl[buf][s] + c * 1024);
+        }
+        if ((k & 1) == 0 && wave < BN / 64) {    // four steps' scales
+            const int r = wave * 64 + lane;
+            copy16_to_lds(ws + ((size_t)(k >> 1) * N + n0 + min(r, lastw)) * 16,
+                          wsl[k >> 1 & 1] + wave * 1024);
+        }
+    };
+    u32x4 raw[UNITS][W];
+    const typename Elem<DT>::T* x0 = x + m0 * ldx;
+    auto load_x = [&](int k) {
+        #pragma unroll
+        for (int q = 0; q < UNITS; ++q) {
+            const int u = q * THREADS + tid, r = u >> 5;
+            const int at = k * 256 + (u & 31) * 8;
+            const typename Elem<DT>::T* p = x0 + min(r, lastx) * ldx + at;
+            if (VEC && at + 8 <= K) {
+                #pragma unroll
+                for (int i = 0; i < W; ++i)
+                    raw[q][i] = reinterpret_cast<const u32x4*>(p)[i];
+            } else {
+                load8_tail<DT>(p, K - at, raw[q]);
+            }
+        }
+    };
+    auto store_x = [&](int buf) {
+        #pragma unroll
+        for (int q = 0; q < UNITS; ++q) {
+            const int u = q * THREADS + tid, r = u >> 5, c8 = u & 31;
+            const int s = c8 >> 4, b = c8 >> 2 & 3;
+            const unsigned byte = scale_byte<DT>(quad_max(absmax_bits<DT>(raw[q], W)));
+            const unsigned c = codes8<DT>(raw[q], scale_f32(byte));
+            *reinterpret_cast<unsigned*>(
+                xl[buf][s] + r * 64 + ((b ^ x_key(r)) << 4) + (c8 & 3) * 4) = c;
+            if ((c8 & 3) == 0) xsl[buf][r * 8 + 2 * b + s] = (uint8_t)byte;
+        }
+    };
+
+    f32x4 acc[FM][FN];
+    #pragma unroll
+    for (int i = 0; i < FM; ++i)
+        #pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
+
+    const int xr = wm + r16, wr = wn + (r16 >> 2) * (4 * FN) + (r16 & 3);
+    const int xp = xr * 64 + ((g ^ x_key(xr)) << 4);
+    const int wp = wr * 64 + ((g ^ w_key<FN>(wr)) << 4);
+    auto compute = [&](int k, int buf, auto both) {
+        int wb[FN], xb[FM];
+        #pragma unroll
+        for (int j = 0; j < FN; ++j)
+            wb[j] = *reinterpret_cast<const unsigned short*>(
+                wsl[k >> 1 & 1] + (wr + j * 4) * 16 + g * 4 + (k & 1) * 2);
+        #pragma unroll
+        for (int i = 0; i < FM; ++i)
+            xb[i] = *reinterpret_cast<const unsigned short*>(
+                xsl[buf] + (xr + i * 16) * 8 + 2 * g);
+        #pragma unroll
+        for (int s = 0; s < (decltype(both)::value ? 2 : 1); ++s) {
+            i32x4 w[FN];
+            #pragma unroll
+            for (int j = 0; j < FN; ++j)
+                w[j] = *reinterpret_cast<const i32x4*>(wl[buf][s] + wp + j * 256);
+            #pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const i32x4 a = *reinterpret_cast<const i32x4*>(xl[buf][s] + xp + i * 1024);
+                #pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = s == 0
+                        ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                              wide(w[j]), wide(a), acc[i][j], 4, 4, 0, wb[j], 0, xb[i])
+                        : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                              wide(w[j]), wide(a), acc[i][j], 4, 4, 1, wb[j], 1, xb[i]);
+            }
+        }
+    };
+    // Waits until a buffer's bytes have arrived and no wave reads the other
+    // one any more, and sends for the next.
+    auto turn = [&](int k) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (k + 1 < turns) {
+            send_w(k + 1, (k + 1) & 1);
+            load_x(k + 1);
+        }
+    };
+    if (turns) {
+        send_w(0, 0);
+        load_x(0);
+        store_x(0);
+    }
+    const int whole = steps >> 1;
+    for (int k = 0; k < whole; ++k) {
+        turn(k);
+        compute(k, k & 1, std::true_type());
+        if (k + 1 < turns) store_x((k + 1) & 1);
+    }
+    if (steps & 1) {
+        turn(whole);
+        compute(whole, whole & 1, std::false_type());
+    }
+
+    const long n = n0 + wn + g * (4 * FN);
+    float b[4 * FN];
+    load_bias<FN>(b, bias, bias_dt, n, N);
+    store_rows<DT, FM, FN>(acc, y, M, N, m0 + wm + r16, n, b);
+}
+
+template <int DT, bool VEC, int BM, int BN, int WM, int WN>
+void launch_rounding(const void* x, long M, long K, long ldx,
+                     const uint8_t* wc, const uint8_t* ws, long N,
+                     const void* bias, int bias_dt, void* y,
+                     hipStream_t stream) {
+    using T = typename Elem<DT>::T;
+    const int mt = (int)((M + BM - 1) / BM), nt = (int)((N + BN - 1) / BN);
+    hipLaunchKernelGGL((rounding_kernel<DT, VEC, BM, BN, WM, WN>),
+                       dim3((unsigned)(mt * nt)), dim3(64 * WM * WN), 0, stream,
+                       (const T*)x, M, (int)K, (int)steps_of(K), ldx, wc, ws, N,
+                       bias, bias_dt, (T*)y, nt, mt * nt);
+}
+
+}  // namespace
+
+void rounding(const void* x, int dt, bool vec, long M, long K, long ldx,
+              const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
+              int bias_dt, void* y, hipStream_t stream) {
+    #define MX4_T(DT, V, BN, WM, WN) \
+        launch_rounding<DT, V, 128, BN, WM, WN>(x, M, K, ldx, wc, ws, N, bias, \
+                                                bias_dt, y, stream)
+    #define MX4_V(DT, BN, WM, WN) do { \
+        if (vec) MX4_T(DT, true, BN, WM, WN); \
+        else MX4_T(DT, false, BN, WM, WN); } while (0)
+    #define MX4_D(BN, WM, WN) do { \
+        if (dt == F32) MX4_V(F32, BN, WM, WN); \
+        else if (dt == BF16) MX4_V(BF16, BN, WM, WN); \
+        else MX4_V(F16, BN, WM, WN); } while (0)
+    if (N > 128) MX4_D(256, 2, 4);
+    else if (N > 64) MX4_D(128, 4, 2);
+    else MX4_D(64, 8, 1);
+    #undef MX4_D
+    #undef MX4_V
+    #undef MX4_T
+}
+
+}  // namespace mx4

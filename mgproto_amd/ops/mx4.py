@@ -42,51 +42,63 @@ def _ext(t: torch.Tensor):
     return _native_or_die()
 
 
-def padded(K: int) -> int:
-    """Elements that a row of K takes up: a multiple of 128."""
-    return -(-K // 128) * 128
-
-
 class MX4Tensor:
-    """Rows held in 4 bits: ``codes`` uint8 [..., Kp/2] (low nibble first) and
-    ``scales`` uint8 [..., Kp/32] (2^(byte-127), 255 = NaN), where Kp is the
-    row length K rounded up to 128; codes and scales behind K are 0.
-    ``dtype`` is the type that ``dequantize`` gives where none is asked."""
+    """Rows held in 4 bits, laid out for the matrix cores.
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, K: int,
+    For ``rows`` = R rows of K elements, ``codes`` is uint8 [ceil(K/128), R,
+    64]: the 64 bytes of 128 elements (low nibble first) of all rows, then the
+    next 128; ``scales`` is uint8 [ceil(K/512), R, 16], where the byte
+    ``4*g + s`` belongs to block ``g`` of the ``s``-th 128 (2^(byte-127), 255 =
+    NaN). Codes and scales behind K are 0. ``parts`` and ``from_parts`` give
+    and take the plain order. ``dtype`` is the type that ``dequantize`` gives
+    where none is asked."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape,
                  dtype: torch.dtype = torch.bfloat16):
+        shape = torch.Size(shape)
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError('MX4Tensor: codes and scales are uint8')
-        Kp = padded(K)
-        if (K < 0 or codes.dim() < 1 or codes.shape[-1] * 2 != Kp
-                or scales.shape != (*codes.shape[:-1], Kp // 32)):
+        if len(shape) < 1 or min(shape) < 0:
+            raise ValueError(f'MX4Tensor: no rows of shape {tuple(shape)}')
+        R, K = math.prod(shape[:-1]), shape[-1]
+        if (codes.shape != (-(-K // 128), R, 64)
+                or scales.shape != (-(-K // 512), R, 16)):
             raise ValueError(
                 f'MX4Tensor: codes {tuple(codes.shape)} and scales '
-                f'{tuple(scales.shape)} do not hold rows of {K}')
+                f'{tuple(scales.shape)} do not hold {R} rows of {K}')
         if codes.device != scales.device:
             raise ValueError('MX4Tensor: codes and scales on one device')
         if dtype not in _CODE:
             raise TypeError(f'MX4Tensor: no values of type {dtype}')
         self.codes, self.scales = codes.contiguous(), scales.contiguous()
-        self.K, self.dtype = K, dtype
+        self.shape, self.dtype = shape, dtype
 
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16) -> 'MX4Tensor':
-        """From unpadded parts, codes [..., K/2] and scales [..., K/32] with K
-        a multiple of 32, as other programs store them."""
+        """From codes [..., K/2] and scales [..., K/32] in plain order, K a
+        multiple of 32, as other programs store them."""
         K = codes.shape[-1] * 2
         if K % 32 or scales.shape != (*codes.shape[:-1], K // 32):
             raise ValueError(
                 f'MX4Tensor: codes {tuple(codes.shape)} and scales '
                 f'{tuple(scales.shape)} are not blocks of 32')
-        pad = padded(K) - K
-        return cls(torch.nn.functional.pad(codes, (0, pad // 2)),
-                   torch.nn.functional.pad(scales, (0, pad // 32)), K, dtype)
+        shape = (*codes.shape[:-1], K)
+        R = math.prod(shape[:-1])
+        return cls(*reference.mx4_arrange(codes.reshape(R, K // 2),
+                                          scales.reshape(R, K // 32)),
+                   shape, dtype)
+
+    def parts(self):
+        """(codes [..., K/2], scales [..., K/32]) in plain order, K rounded up
+        to a multiple of 32."""
+        nb, lead = -(-self.K // 32), self.shape[:-1]
+        codes, scales = reference.mx4_plain(self.codes, self.scales, self.K)
+        return codes.view(*lead, nb * 16), scales.view(*lead, nb)
 
     @property
-    def shape(self) -> torch.Size:
-        return torch.Size((*self.codes.shape[:-1], self.K))
+    def K(self) -> int:
+        return self.shape[-1]
 
     @property
     def device(self) -> torch.device:
@@ -98,15 +110,10 @@ class MX4Tensor:
 
     def to(self, device) -> 'MX4Tensor':
         return MX4Tensor(self.codes.to(device), self.scales.to(device),
-                         self.K, self.dtype)
+                         self.shape, self.dtype)
 
     def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return mx4_dequantize(self, dtype)
-
-    def _rows(self):
-        M = math.prod(self.codes.shape[:-1])
-        return (self.codes.view(M, self.codes.shape[-1]),
-                self.scales.view(M, self.scales.shape[-1]))
 
     def __repr__(self):
         return (f'MX4Tensor(shape={tuple(self.shape)}, '
@@ -134,10 +141,7 @@ def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
         codes, scales = ext.mx4_quantize(x2)
     else:
         codes, scales = reference.mx4_quantize(x2)
-    lead = x.shape[:-1]
-    return MX4Tensor(codes.view(*lead, codes.shape[-1]),
-                     scales.view(*lead, scales.shape[-1]), x.shape[-1],
-                     x.dtype)
+    return MX4Tensor(codes, scales, x.shape, x.dtype)
 
 
 def mx4_dequantize(q: MX4Tensor,
@@ -147,12 +151,11 @@ def mx4_dequantize(q: MX4Tensor,
     dtype = dtype or q.dtype
     if dtype not in _CODE:
         raise TypeError(f'mx4_dequantize: no values of type {dtype}')
-    codes, scales = q._rows()
-    ext = _ext(codes)
+    ext = _ext(q.codes)
     if ext is not None:
-        out = ext.mx4_dequantize(codes, scales, q.K, _CODE[dtype])
+        out = ext.mx4_dequantize(q.codes, q.scales, q.K, _CODE[dtype])
     else:
-        out = reference.mx4_dequantize(codes, scales, q.K, dtype)
+        out = reference.mx4_dequantize(q.codes, q.scales, q.K, dtype)
     return out.view(q.shape)
 
 
@@ -240,7 +243,7 @@ def mx4_linear(x: torch.Tensor, weight: Union[MX4Tensor, torch.Tensor],
                              f'{bias.device}')
         bias = bias.contiguous()
     x2 = _matrix(x)
-    wc, ws = weight._rows() if held else (None, None)
+    wc, ws = (weight.codes, weight.scales) if held else (None, None)
     y = _MX4Linear.apply(x2, None if held else weight, wc, ws, bias,
                          torch.is_grad_enabled())
     return y.view(*x.shape[:-1], weight.shape[0])

@@ -329,11 +329,31 @@ def _power_of_two(e: torch.Tensor) -> torch.Tensor:
         torch.int32).view(torch.float32)
 
 
+def mx4_arrange(codes: torch.Tensor, scales: torch.Tensor):
+    """Plain [R, K/2] and [R, K/32] -> codes [ceil(K/128), R, 64] and scales
+    [ceil(K/512), R, 16], where byte 4*g + s is block g of the s-th 128."""
+    R, nb = scales.shape
+    steps, chunks = -(-nb // 4), -(-nb // 16)
+    codes = F.pad(codes, (0, steps * 64 - nb * 16)).view(R, steps, 64)
+    scales = F.pad(scales, (0, chunks * 16 - nb)).view(R, chunks, 4, 4)
+    return (codes.permute(1, 0, 2).contiguous(),
+            scales.permute(1, 0, 3, 2).reshape(chunks, R, 16))
+
+
+def mx4_plain(codes: torch.Tensor, scales: torch.Tensor, K: int):
+    """The reverse of mx4_arrange, without the padding."""
+    steps, R, _ = codes.shape
+    chunks, nb = scales.shape[0], -(-K // 32)
+    codes = codes.permute(1, 0, 2).reshape(R, steps * 64)
+    scales = scales.view(chunks, R, 4, 4).permute(1, 0, 3, 2).reshape(
+        R, chunks * 16)
+    return codes[:, :nb * 16].contiguous(), scales[:, :nb].contiguous()
+
+
 def mx4_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """[M, K] -> codes uint8 [M, Kp/2], scales uint8 [M, Kp/32], Kp = K
-    rounded up to 128."""
+    """[M, K] -> codes and scales as mx4_arrange lays them out."""
     M, K = x.shape
-    Kp = -(-K // 128) * 128
+    Kp = -(-K // 32) * 32
     v = F.pad(x.float(), (0, Kp - K)).reshape(M, Kp // 32, 32)
     amax = v.abs().amax(dim=2)
     bad = ~torch.isfinite(amax)
@@ -351,11 +371,12 @@ def mx4_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     code = code.view(M, Kp // 2, 2)
     codes = (code[..., 0] | code[..., 1] << 4).to(torch.uint8)
     scales = torch.where(bad, 255, byte).to(torch.uint8)
-    return codes, scales
+    return mx4_arrange(codes, scales)
 
 
 def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int,
                    dtype: torch.dtype) -> torch.Tensor:
+    codes, scales = mx4_plain(codes, scales, K)
     M, nb = scales.shape
     c = torch.stack([codes & 15, codes >> 4], dim=2).view(M, nb, 32).long()
     grid = torch.tensor([0., .5, 1., 1.5, 2., 3., 4., 6.],

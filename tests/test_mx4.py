@@ -20,8 +20,16 @@ def test_round_trip_is_the_definition(M, K, dtype):
         -6e4, 6e4).to(dtype)
     q = ops.mx4_quantize(x)
     assert q.shape == (M, K) and q.dtype == dtype
-    assert q.codes.shape == (M, -(-K // 128) * 64)
-    assert q.scales.shape == (M, -(-K // 128) * 4)
+    codes, scales = q.parts()
+    assert codes.shape == (M, -(-K // 32) * 16)
+    assert scales.shape == (M, -(-K // 32))
+    again = ops.MX4Tensor.from_parts(codes, scales, dtype)
+    assert torch.equal(again.codes, q.codes)
+    assert torch.equal(again.scales, q.scales)
+    # element k is the nibble k & 1 of byte k / 2
+    code = codes[M - 1, (K - 1) // 2] >> 4 * ((K - 1) & 1) & 7
+    assert float(GRID[code.item()]) * 2.0 ** (int(scales[M - 1, -1]) - 127) \
+        == float(q.dequantize()[M - 1, K - 1].abs())
     assert torch.equal(q.dequantize().double(), values(x))
     assert torch.equal(q.dequantize(torch.float32).double(), values(x))
 
@@ -48,8 +56,10 @@ def test_scales_at_the_ends():
     x[4, 5] = math.nan
     x[5, 5] = -math.inf
     q = ops.mx4_quantize(x)
-    assert q.scales[:, 0].tolist() == [252, 0, 0, 125, 255, 255]
-    assert q.scales[:, 1:].eq(0).all() and q.codes[4:].eq(0).all()
+    codes, scales = q.parts()
+    assert scales[:, 0].tolist() == [252, 0, 0, 125, 255, 255]
+    assert codes[4:].eq(0).all()
+    assert q.scales[..., 1:].eq(0).all()          # behind the row
     v = q.dequantize()
     assert torch.equal(v[:4].double(), values(x)[:4])
     assert v[4:].isnan().all()
@@ -58,12 +68,14 @@ def test_scales_at_the_ends():
 def test_leading_axes_strides_and_parts():
     x = torch.randn(2, 3, 64)
     q = ops.mx4_quantize(x)
-    assert q.shape == (2, 3, 64) and q.codes.shape == (2, 3, 64)
+    assert q.shape == (2, 3, 64) and q.codes.shape == (1, 6, 64)
     t = torch.randn(64, 5).t()               # rows not contiguous
     assert torch.equal(ops.mx4_quantize(t).dequantize(),
                        ops.mx4_quantize(t.contiguous()).dequantize())
-    p = ops.MX4Tensor.from_parts(q.codes[..., :32], q.scales[..., :2],
-                                 torch.float32)
+    codes, scales = q.parts()
+    assert codes.shape == (2, 3, 32) and scales.shape == (2, 3, 2)
+    p = ops.MX4Tensor.from_parts(codes, scales, torch.float32)
+    assert p.shape == (2, 3, 64)
     assert torch.equal(p.dequantize(), q.dequantize())
     assert ops.mx4_quantize(torch.zeros(0, 32)).dequantize().shape == (0, 32)
     assert ops.mx4_quantize(torch.zeros(4, 0)).dequantize().shape == (4, 0)
@@ -150,12 +162,14 @@ def test_refusals():
         ops.mx4_linear(x, w.double())
     with pytest.raises(ValueError, match='weight on meta'):
         ops.mx4_linear(x, w.to('meta'))
-    with pytest.raises(ValueError, match='rows of 65'):
-        ops.MX4Tensor(q.codes[:, :16], q.scales, 65)
+    with pytest.raises(ValueError, match='8 rows of 129'):
+        ops.MX4Tensor(q.codes, q.scales, (8, 129))
+    with pytest.raises(ValueError, match='7 rows of 64'):
+        ops.MX4Tensor(q.codes, q.scales, (7, 64))
     with pytest.raises(TypeError):
-        ops.MX4Tensor(q.codes.int(), q.scales, 64)
+        ops.MX4Tensor(q.codes.int(), q.scales, (8, 64))
     with pytest.raises(ValueError, match='blocks of 32'):
-        ops.MX4Tensor.from_parts(q.codes[:, :15], q.scales[:, :1])
+        ops.MX4Tensor.from_parts(*(t[:, :1] for t in q.parts()))
     with pytest.raises(TypeError, match='float64'):
         q.dequantize(torch.float64)
     xg = x.clone().requires_grad_()

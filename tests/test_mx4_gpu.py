@@ -278,7 +278,7 @@ def test_refusals():
     qd = q.to('cuda')
     x = torch.randn(4, 64, device='cuda')
     with pytest.raises(RuntimeError, match='do not hold rows'):
-        ext.mx4_linear(x, qd.codes[:, :32].contiguous(), qd.scales, None)
+        ext.mx4_linear(x, qd.codes[:, :, :32].contiguous(), qd.scales, None)
     with pytest.raises(RuntimeError, match='contiguous'):
         ext.mx4_linear(x.t(), qd.codes, qd.scales, None)
     with pytest.raises(RuntimeError, match='does not match'):
