@@ -28,12 +28,25 @@ static __device__ __forceinline__ void values8(unsigned c, unsigned byte,
     for (int i = 0; i < 8; ++i) f[i] = byte == 255u ? nan : f[i];
 }
 
-#define MX4_GLOBAL(p) (const __attribute__((address_space(1))) void*)(uintptr_t)(p)
-#define MX4_LDS(p) (__attribute__((address_space(3))) void*)(uint32_t)(uintptr_t)(p)
-// 16 bytes a lane from memory into LDS, past the registers: lane i's go to
-// l + 16 i, with l the same in the wave
-static __device__ __forceinline__ void copy16_to_lds(const void* g, void* l) {
-    __builtin_amdgcn_global_load_lds(MX4_GLOBAL(g), MX4_LDS(l), 16, 0, 0);
+// 16 bytes a lane from memory into LDS, past the registers: lane i's, from
+// base + off, go to l + 16 i; base and l are the same in the wave. In assembly,
+// because the compiler would wait for every such copy before the next read of
+// LDS, whichever bytes that reads: waiting is the caller's, by wait_copies() and
+// a barrier. No register is written. The pause covers a base that a vector
+// instruction wrote just before.
+static __device__ __forceinline__ unsigned lds_address(const void* l) {
+    return (unsigned)(uintptr_t)l;
+}
+static __device__ __forceinline__ void copy16_to_lds(const void* base,
+                                                     unsigned off, unsigned l) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\t"
+                 "global_load_lds_dwordx4 %0, %1"
+                 :: "v"(off), "s"(base), "s"(l) : "memory");
+}
+// until at most N of this wave's memory instructions are under way (they end
+// in their order), and its reads of LDS are over
+template <int N> static __device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
 }
 
 // In LDS a step's codes are rows of 64 bytes, four pieces of 16; piece g of row
@@ -67,6 +80,9 @@ static __device__ __forceinline__ void load_bias(float (&b)[4 * FN],
         const float* p = reinterpret_cast<const float*>(bias);
         #pragma unroll
         for (int i = 0; i < 4 * FN; ++i) b[i] = p[min(n + i, N - 1)];
+        // (waited for here, not in every step of the loop that comes next)
+        #pragma unroll
+        for (int i = 0; i < 4 * FN; ++i) asm volatile("" : "+v"(b[i]));
     } else {
         const unsigned short* p = reinterpret_cast<const unsigned short*>(bias);
         unsigned short u[4 * FN];

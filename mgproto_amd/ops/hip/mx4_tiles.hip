@@ -24,7 +24,7 @@ namespace mx4 {
 namespace {
 
 template <int OT, int BM, int BN, int WM, int WN, int S>
-__global__ __launch_bounds__(64 * WM * WN)
+__global__ __launch_bounds__(64 * WM * WN, 2)
 void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs,
                   long M, int steps, const uint8_t* __restrict__ wc,
                   const uint8_t* __restrict__ ws, long N,
@@ -36,11 +36,12 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
     constexpr int XQ = BM / 16 / WAVES, WQ = BN / 16 / WAVES;   // copies a step
     constexpr int SQ = R / 64 / WAVES;                          // ... four steps
     static_assert(BM % (16 * WAVES) == 0 && BN % (16 * WAVES) == 0 &&
-                  R % (64 * WAVES) == 0 && BM % 64 == 0, "whole copies");
-    // the ring of codes, and two buffers of scales. (One array: with two the
-    // compiler waits for all copies before it reads.)
+                  R % (64 * WAVES) == 0 && BM % 64 == 0 &&
+                  FM % (XQ + WQ) == 0 && S >= 3, "whole copies");
+    // the ring of codes, and two buffers of scales
     __shared__ __attribute__((aligned(16))) uint8_t lds[S * R * 64 + 2 * R * 16];
     uint8_t* const scales = lds + S * R * 64;
+    const unsigned to = lds_address(lds);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
@@ -85,35 +86,50 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
         }
     };
     int lc = 0;                                   // buffer of the next scales
-    auto send = [&](int buf) {
-        if ((lk & 3) == 0) {
-            #pragma unroll
-            for (int q = 0; q < SQ; ++q) {
-                const int call = q * WAVES + wave;
-                copy16_to_lds((call < BM / 64 ? lxs : lws) + (unsigned)so[q],
-                              scales + lc * (R * 16) + call * 1024);
-            }
-            lxs += M * 16, lws += N * 16, lc ^= 1;
+    bool more = true;                             // anything left to send
+    auto send_scales = [&]() {
+        if (lk & 3 || !more) return;
+        #pragma unroll
+        for (int q = 0; q < SQ; ++q) {
+            const int call = q * WAVES + wave;
+            copy16_to_lds(call < BM / 64 ? lxs : lws, (unsigned)so[q],
+                          to + S * R * 64 + lc * (R * 16) + call * 1024);
         }
-        #pragma unroll
-        for (int q = 0; q < XQ; ++q)
-            copy16_to_lds(lx + (unsigned)xo[q],
-                          lds + buf * (R * 64) + (q * WAVES + wave) * 1024);
-        #pragma unroll
-        for (int q = 0; q < WQ; ++q)
-            copy16_to_lds(lw + (unsigned)wo[q],
-                          lds + buf * (R * 64) + BM * 64 + (q * WAVES + wave) * 1024);
+        lxs += M * 16, lws += N * 16, lc ^= 1;
+    };
+    auto send_codes = [&](int buf, int q) {       // one copy of XQ + WQ
+        if (q < XQ)
+            copy16_to_lds(lx, (unsigned)xo[q],
+                          to + buf * (R * 64) + (q * WAVES + wave) * 1024);
+        else
+            copy16_to_lds(lw, (unsigned)wo[q - XQ],
+                          to + buf * (R * 64) + BM * 64
+                              + ((q - XQ) * WAVES + wave) * 1024);
+    };
+    // Behind the last step the same bytes are sent again and again, so that
+    // the count of copies stays what the waits take it for.
+    auto sent = [&]() {
+        if (!more) return;
         lx += M * 64, lw += N * 64;
         if (++lk == steps) {
-            lk = 0, lt += stride;
-            if (lt < hi) aim();
+            lk = 0;
+            more = lt + stride < hi;
+            if (more) lt += stride;
+            aim();
         }
     };
-    if (lt < hi && steps) {
+    if (lt >= hi || !steps) {
+        if (lt >= hi) return;
+        more = false;
+    } else {
         aim();
         #pragma unroll
-        for (int b = 0; b < S - 1; ++b)
-            if (lt < hi) send(b);
+        for (int b = 0; b < S - 1; ++b) {
+            if (b) sent();
+            send_scales();
+            #pragma unroll
+            for (int q = 0; q < XQ + WQ; ++q) send_codes(b, q);
+        }
     }
 
     // Where this lane reads: rows 16 apart (x) and 4 apart (W) have the same
@@ -123,36 +139,49 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
     const int wp = (BM + wr) * 64 + ((g ^ w_key<FN>(wr)) << 4);
     const int xsp = xr * 16 + g * 4, wsp = (BM + wr) * 16 + g * 4;
     int buf = 0, sbuf = 0;
+    int xb[FM], wb[FN];
+    i32x4 w[FN], x[FM];
+    // the first reads of a step, made while the step before still computes
+    auto begin = [&](int buf) {
+        const uint8_t* c = lds + buf * (R * 64);
+        #pragma unroll
+        for (int j = 0; j < FN; ++j)
+            w[j] = *reinterpret_cast<const i32x4*>(c + wp + j * 256);
+        x[0] = *reinterpret_cast<const i32x4*>(c + xp);
+        x[1] = *reinterpret_cast<const i32x4*>(c + xp + 1024);
+    };
+    wait_copies<0>();
+    __syncthreads();
+    begin(0);
     for (int t = lo + (blockIdx.x >> 3); t < hi; t += stride) {
         f32x4 acc[FM][FN];
         #pragma unroll
         for (int i = 0; i < FM; ++i)
             #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
-        int xb[FM], wb[FN];
 
         for (int k = 0; k < steps; ++k) {
-            // This step's bytes have arrived: what was sent for the S - 2
-            // steps behind it may still be under way (and what left since,
-            // results of the last tile, came after it). Then every wave is done
-            // with the buffer of the step before, which is filled again.
-            const bool more = lt < hi;
-            if (more)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)"
-                             :: "n"((S - 2) * (XQ + WQ)) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            // The bytes of the step behind this one have arrived: only what was
+            // sent for the S - 3 steps after it may still be under way (and
+            // what left since, results of the last tile, came later). Then
+            // every wave is done with the buffer of the step before this one,
+            // which is filled again.
+            wait_copies<(S - 3) * (XQ + WQ)>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (more) send(buf == 0 ? S - 1 : buf - 1);
+            const int free = buf == 0 ? S - 1 : buf - 1;
             const uint8_t* c = lds + buf * (R * 64);
+            buf = buf == S - 1 ? 0 : buf + 1;
+            sent();
+            send_scales();
             if ((k & 3) == 0) {
+                const uint8_t* s = scales + sbuf * (R * 16);
                 #pragma unroll
                 for (int j = 0; j < FN; ++j)
-                    wb[j] = *reinterpret_cast<const int*>(scales + sbuf * (R * 16) + wsp + j * 64);
+                    wb[j] = *reinterpret_cast<const int*>(s + wsp + j * 64);
                 #pragma unroll
                 for (int i = 0; i < FM; ++i)
-                    xb[i] = *reinterpret_cast<const int*>(scales + sbuf * (R * 16) + xsp + i * 256);
+                    xb[i] = *reinterpret_cast<const int*>(s + xsp + i * 256);
                 sbuf ^= 1;
             } else {                              // the next byte of each
                 #pragma unroll
@@ -160,26 +189,27 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
                 #pragma unroll
                 for (int i = 0; i < FM; ++i) xb[i] = (unsigned)xb[i] >> 8;
             }
-            i32x4 w[FN];
-            #pragma unroll
-            for (int j = 0; j < FN; ++j)
-                w[j] = *reinterpret_cast<const i32x4*>(c + wp + j * 256);
+            // reads two rows ahead of the matrix instructions, and the copies
+            // spread among these, so that neither holds them up
+            constexpr int EACH = FM / (XQ + WQ);
             #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const i32x4 x = *reinterpret_cast<const i32x4*>(c + xp + i * 1024);
+                if (i + 2 < FM)
+                    x[i + 2] = *reinterpret_cast<const i32x4*>(
+                        c + xp + (i + 2) * 1024);
+                if (i % EACH == 0) send_codes(free, i / EACH);
                 #pragma unroll
                 for (int j = 0; j < FN; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                        wide(w[j]), wide(x), acc[i][j], 4, 4, 0, wb[j], 0, xb[i]);
+                        wide(w[j]), wide(x[i]), acc[i][j], 4, 4, 0, wb[j], 0, xb[i]);
             }
-            // reads run two rows ahead of the matrix instructions
-            __builtin_amdgcn_sched_group_barrier(0x100, FN + 2, 0);
+            begin(buf);
             #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x8, FN, 0);
                 if (i + 2 < FM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if (i == FM - 1) __builtin_amdgcn_sched_group_barrier(0x100, FN + 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, FN, 0);
             }
-            buf = buf == S - 1 ? 0 : buf + 1;
         }
 
         long m0, n0;
@@ -189,6 +219,7 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
         load_bias<FN>(b, bias, bias_dt, n, N);
         store_rows<OT, FM, FN>(acc, y, M, N, m0 + wm + r16, n, b);
     }
+    wait_copies<0>();      // no copy is under way when LDS is given up
 }
 
 template <int OT, int BM, int BN, int WM, int WN, int S>
