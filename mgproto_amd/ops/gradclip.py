@@ -15,8 +15,7 @@ from . import reference
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _tensors(ts, what: str) -> List[torch.Tensor]:
-    ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
+def _tensors(ts: List[torch.Tensor], what: str):
     for t in ts:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f'{what}: tensors, not {type(t).__name__}')
@@ -28,7 +27,6 @@ def _tensors(ts, what: str) -> List[torch.Tensor]:
         if t.device != ts[0].device:
             raise ValueError(f'{what}: tensors on {ts[0].device} and '
                              f'{t.device}')
-    return ts
 
 
 def _check_p(norm_type: float, what: str) -> float:
@@ -38,29 +36,34 @@ def _check_p(norm_type: float, what: str) -> float:
     return p
 
 
-def _ext(t: torch.Tensor):
-    if not t.is_cuda:
+def _list(ts) -> List[torch.Tensor]:
+    return [ts] if isinstance(ts, torch.Tensor) else list(ts)
+
+
+def _ext(ts):
+    """The extension for GPU tensors, which makes the checks below itself."""
+    if not (ts and isinstance(ts[0], torch.Tensor) and ts[0].is_cuda):
         return None
     from . import _native_or_die
     return _native_or_die()
 
 
-@torch.no_grad()
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]],
               norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of the list together, a float32 number on
     their device. An empty list has the norm 0 (on the CPU)."""
-    ts = _tensors(grads, 'grad_norm')
+    ts = _list(grads)
+    ext = _ext(ts)
+    if ext is not None:
+        return ext.grad_norm(ts, norm_type)
+    _tensors(ts, 'grad_norm')
     p = _check_p(norm_type, 'grad_norm')
     if not ts:
         return torch.zeros(())
-    ext = _ext(ts[0])
-    if ext is None:
+    with torch.no_grad():
         return reference.grad_norm(ts, p).float()
-    return ext.grad_norm(ts, p)
 
 
-@torch.no_grad()
 def clip_grads_(grads: Union[torch.Tensor, Iterable[torch.Tensor]],
                 max_norm: float, norm_type: float = 2.0,
                 out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
@@ -72,11 +75,16 @@ def clip_grads_(grads: Union[torch.Tensor, Iterable[torch.Tensor]],
     What is written has to be dense and apart from everything else in the
     call. A norm that is NaN makes every element NaN; an infinite one makes
     the finite elements 0 and the infinite ones NaN."""
-    ts = _tensors(grads, 'clip_grads_')
+    ts = _list(grads)
+    outs = ts if out is None else _list(out)
+    ext = _ext(ts)
+    if ext is not None:
+        return ext.clip_grads(ts, outs, max_norm, norm_type)
+    _tensors(ts, 'clip_grads_')
+    _tensors(outs, 'clip_grads_: out')
     p = _check_p(norm_type, 'clip_grads_')
     if not max_norm >= 0:
         raise ValueError(f'clip_grads_: max_norm {max_norm}')
-    outs = ts if out is None else _tensors(out, 'clip_grads_: out')
     if len(outs) != len(ts):
         raise ValueError(f'clip_grads_: {len(ts)} gradients, {len(outs)} '
                          'outputs')
@@ -89,10 +97,5 @@ def clip_grads_(grads: Union[torch.Tensor, Iterable[torch.Tensor]],
                          f'{outs[0].device}')
     if not ts:
         return torch.zeros(())
-    ext = _ext(ts[0])
-    if ext is None:
+    with torch.no_grad():
         return reference.clip_grads(ts, outs, float(max_norm), p)
-    norm = ext.clip_grads(ts, outs, float(max_norm), p)
-    for o in outs:       # written behind autograd's back
-        torch.autograd.graph.increment_version(o)
-    return norm

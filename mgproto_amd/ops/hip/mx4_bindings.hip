@@ -13,7 +13,17 @@
 
 namespace {
 
+namespace py = pybind11;
 using at::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+// A call's argument is refused as Python would refuse it.
+template <class E, class... A>
+void refuse_unless(bool ok, A&&... what) {
+    if (!ok) throw E(c10::str(std::forward<A>(what)...));
+}
+#define CHECK_TYPE(ok, ...) refuse_unless<py::type_error>(ok, __VA_ARGS__)
+#define CHECK_VALUE(ok, ...) refuse_unless<py::value_error>(ok, __VA_ARGS__)
 
 int dtype_code(const Tensor& t, const char* what) {
     switch (t.scalar_type()) {
@@ -21,8 +31,9 @@ int dtype_code(const Tensor& t, const char* what) {
         case at::kBFloat16: return mx4::BF16;
         case at::kHalf: return mx4::F16;
         default:
-            TORCH_CHECK(false, what, ": float32, bfloat16 or float16, not ",
-                        t.scalar_type());
+            throw py::type_error(c10::str(
+                what, ": float32, bfloat16 or float16, not ",
+                t.scalar_type()));
     }
 }
 
@@ -34,12 +45,29 @@ at::ScalarType scalar_type(int64_t dt) {
 
 hipStream_t current_stream() { return at::hip::getCurrentHIPStream(); }
 
-// rows of elements next to each other, at any distance
-void check_rows(const Tensor& x, const char* what) {
-    TORCH_CHECK(x.is_cuda() && x.dim() == 2, what, ": a matrix on the GPU");
-    TORCH_CHECK(x.size(1) <= 1 || x.stride(1) == 1, what,
-                ": rows must be contiguous");
-    TORCH_CHECK(x.size(1) < (1L << 30), what, ": rows too long");
+// [..., K] as [M, K] with contiguous rows: a view where it can be
+Tensor matrix(const Tensor& x, const char* what) {
+    CHECK_VALUE(x.dim() >= 1, what, ": rows, not a number");
+    CHECK_VALUE(x.is_cuda(), what, ": on ", x.device(), ", not on a GPU");
+    const int64_t K = x.size(-1);
+    CHECK_VALUE(K < (1L << 22), what, ": rows of at most 2^22 elements");
+    int64_t M = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
+    Tensor x2 = x.dim() == 2 ? x : x.reshape({M, K});
+    if ((K > 1 && x2.stride(1) != 1) || (M > 1 && x2.stride(0) < K))
+        x2 = x2.contiguous();
+    return x2;
+}
+
+int64_t row_stride(const Tensor& x) {
+    return x.size(0) > 1 ? x.stride(0) : x.size(1);
+}
+
+// the result's shape: x's, with N for the last
+std::vector<int64_t> shape_of(const Tensor& x, int64_t N) {
+    auto s = x.sizes().vec();
+    s.back() = N;
+    return s;
 }
 
 // 4-bit rows of K elements, as mx4_common.h lays them out
@@ -63,12 +91,12 @@ void check_packed(const Tensor& codes, const Tensor& scales, int64_t K,
                 ": codes and scales start on 16 bytes");
 }
 
-void check_bias(const c10::optional<Tensor>& bias, int64_t N,
-                const Tensor& like) {
+void check_bias(const OptTensor& bias, int64_t N, const Tensor& like) {
     if (!bias.has_value()) return;
-    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N &&
-                    bias->is_contiguous() && bias->device() == like.device(),
-                "bias: contiguous, ", N, " values, on the same GPU");
+    CHECK_VALUE(bias->dim() == 1 && bias->size(0) == N, "mx4_linear: bias ",
+                bias->sizes(), " for ", N, " columns");
+    CHECK_VALUE(bias->device() == like.device(), "mx4_linear: input on ",
+                like.device(), ", bias on ", bias->device());
 }
 
 Tensor workspace(size_t bytes, const Tensor& like) {
@@ -76,18 +104,25 @@ Tensor workspace(size_t bytes, const Tensor& like) {
                      like.options().dtype(at::kByte));
 }
 
-std::tuple<Tensor, Tensor> quantize(const Tensor& x) {
-    check_rows(x, "mx4_quantize");
-    const int dt = dtype_code(x, "mx4_quantize");
-    c10::DeviceGuard guard(x.device());
-    const int64_t R = x.size(0), K = x.size(1);
-    auto opt = x.options().dtype(at::kByte);
-    auto codes = at::empty({mx4::steps_of(K), R, 64}, opt);
-    auto scales = at::empty({mx4::chunks_of(K), R, 16}, opt);
-    mx4::quantize(x.data_ptr(), dt, R, K, R > 1 ? x.stride(0) : K,
-                  codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
+struct Packed { Tensor codes, scales; };
+
+Packed pack(const Tensor& x2, int dt) {
+    const int64_t R = x2.size(0), K = x2.size(1);
+    auto opt = x2.options().dtype(at::kByte);
+    Packed p{at::empty({mx4::steps_of(K), R, 64}, opt),
+             at::empty({mx4::chunks_of(K), R, 16}, opt)};
+    mx4::quantize(x2.data_ptr(), dt, R, K, row_stride(x2),
+                  p.codes.data_ptr<uint8_t>(), p.scales.data_ptr<uint8_t>(),
                   current_stream());
-    return {codes, scales};
+    return p;
+}
+
+std::tuple<Tensor, Tensor> quantize(const Tensor& x) {
+    const int dt = dtype_code(x, "mx4_quantize");
+    const Tensor x2 = matrix(x, "mx4_quantize");
+    c10::DeviceGuard guard(x2.device());
+    Packed p = pack(x2, dt);
+    return {p.codes, p.scales};
 }
 
 Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
@@ -102,124 +137,168 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
     return out;
 }
 
-// what one tile of 16 x 16 a block can number
+// what blocks of 16 x 16 results can number
 void check_tiles(int64_t M, int64_t N) {
-    TORCH_CHECK((M + 15) / 16 * ((N + 15) / 16) < (1L << 31),
-                "mx4_linear: ", M, " x ", N, " results are too many");
+    CHECK_VALUE((M + 15) / 16 * ((N + 15) / 16) < (1L << 31), "mx4_linear: ",
+                M, " x ", N, " results are too many");
 }
 
 int pick(int64_t form, int chosen) {
-    TORCH_CHECK(form >= -1 && form < mx4::FORMS, "mx4_linear: no form ", form);
+    CHECK_VALUE(form >= -1 && form < mx4::FORMS, "mx4_linear: no form ", form);
     return form < 0 ? chosen : (int)form;
 }
 
-Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws,
-              const c10::optional<Tensor>& bias, int64_t form) {
-    check_rows(x, "mx4_linear: input");
-    const int64_t M = x.size(0), K = x.size(1), N = wc.size(1);
-    check_packed(wc, ws, K, "mx4_linear: weight");
-    TORCH_CHECK(x.device() == wc.device(), "mx4_linear: one GPU for all");
-    check_bias(bias, N, x);
+struct Bias {            // contiguous, and its type
+    Tensor t;
+    int dt = 0;
+    explicit Bias(const OptTensor& b) {
+        if (!b.has_value()) return;
+        dt = dtype_code(*b, "mx4_linear: bias");
+        t = b->contiguous();
+    }
+    const void* ptr() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+
+// Q(x) W^T + bias with held weights, no gradient
+Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws, int64_t K,
+              const OptTensor& bias, int64_t form) {
     const int dt = dtype_code(x, "mx4_linear: input");
-    c10::DeviceGuard guard(x.device());
+    const Tensor x2 = matrix(x, "mx4_linear: input");
+    const int64_t M = x2.size(0), N = wc.size(1);
+    CHECK_VALUE(x2.size(1) == K, "mx4_linear: input ", x.sizes(),
+                " and weight [", N, ", ", K, "] do not match");
+    CHECK_VALUE(x.device() == wc.device(), "mx4_linear: input on ", x.device(),
+                ", weight on ", wc.device());
+    check_packed(wc, ws, K, "mx4_linear: weight");
+    check_bias(bias, N, x);
     check_tiles(M, N);
-    auto y = at::empty({M, N}, x.options());
+    c10::DeviceGuard guard(x.device());
+    auto y = at::empty(shape_of(x, N), x.options());
     if (!M || !N) return y;
-    const int64_t ldx = M > 1 ? x.stride(0) : K;
-    const bool aligned = (uintptr_t)x.data_ptr() % 16 == 0 &&
-                         ldx * x.element_size() % 16 == 0;
-    const int f = pick(form, mx4::linear_form(M, K, N, dt, aligned));
+    const Bias b(bias);
+    const int64_t ldx = row_stride(x2);
+    const bool aligned = (uintptr_t)x2.data_ptr() % 16 == 0 &&
+                         ldx * x2.element_size() % 16 == 0;
+    const int f = pick(form, mx4::linear_form(M, K, N, aligned));
     Tensor work;
     if (const size_t bytes = mx4::linear_bytes(f, M, K))
         work = workspace(bytes, x);
-    mx4::linear(x.data_ptr(), dt, M, K, ldx, wc.data_ptr<uint8_t>(),
-                ws.data_ptr<uint8_t>(), N, bias ? bias->data_ptr() : nullptr,
-                bias ? dtype_code(*bias, "mx4_linear: bias") : 0, y.data_ptr(),
-                f, work.defined() ? work.data_ptr() : nullptr,
-                current_stream());
+    mx4::linear(x2.data_ptr(), dt, M, K, ldx, wc.data_ptr<uint8_t>(),
+                ws.data_ptr<uint8_t>(), N, b.ptr(), b.dt, y.data_ptr(), f,
+                work.defined() ? work.data_ptr() : nullptr, current_stream());
     return y;
 }
 
-Tensor linear_q(const Tensor& xc, const Tensor& xs, int64_t K,
-                const Tensor& wc, const Tensor& ws,
-                const c10::optional<Tensor>& bias, int64_t dt, int64_t form) {
-    check_packed(xc, xs, K, "mx4_linear: input");
-    check_packed(wc, ws, K, "mx4_linear: weight");
-    TORCH_CHECK(xc.device() == wc.device(), "mx4_linear: one GPU for all");
+Tensor product_q(const Tensor& xc, const Tensor& xs, int64_t K,
+                 const Tensor& wc, const Tensor& ws, const OptTensor& bias,
+                 std::vector<int64_t> shape, int dt, int64_t form) {
     const int64_t M = xc.size(1), N = wc.size(1);
     check_bias(bias, N, xc);
-    c10::DeviceGuard guard(xc.device());
     check_tiles(M, N);
-    auto y = at::empty({M, N}, xc.options().dtype(scalar_type(dt)));
-    if (M && N)
-        mx4::linear_q(xc.data_ptr<uint8_t>(), xs.data_ptr<uint8_t>(), M, K,
-                      wc.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), N,
-                      bias ? bias->data_ptr() : nullptr,
-                      bias ? dtype_code(*bias, "mx4_linear: bias") : 0,
-                      y.data_ptr(), (int)dt,
-                      pick(form, mx4::linear_q_form(M, K, N)),
-                      current_stream());
+    auto y = at::empty(shape, xc.options().dtype(scalar_type(dt)));
+    if (!M || !N) return y;
+    const Bias b(bias);
+    const int f = std::max(pick(form, mx4::linear_q_form(M, K, N)),
+                           (int)mx4::HELD16);
+    mx4::linear_q(xc.data_ptr<uint8_t>(), xs.data_ptr<uint8_t>(), M, K,
+                  wc.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), N, b.ptr(),
+                  b.dt, y.data_ptr(), dt, f, current_stream());
     return y;
 }
 
-void check_grad(const Tensor& g) {
-    TORCH_CHECK(g.is_cuda() && g.dim() == 2 && g.is_contiguous(),
-                "mx4_linear: output gradient: a contiguous matrix on the GPU");
-    TORCH_CHECK(g.size(0) < (1L << 31) && g.size(1) < (1L << 30),
-                "mx4_linear: output gradient: too large");
-}
-
-Tensor grad_input(const Tensor& g, const Tensor& wc, const Tensor& ws,
-                  int64_t K, int64_t dt) {
-    check_grad(g);
-    check_packed(wc, ws, K, "mx4_linear: weight");
-    const int64_t M = g.size(0), N = g.size(1);
-    TORCH_CHECK(wc.size(1) == N && g.device() == wc.device(),
-                "mx4_linear: output gradient does not match the weight");
-    const int gd = dtype_code(g, "mx4_linear: output gradient");
-    c10::DeviceGuard guard(g.device());
-    auto dx = at::empty({M, K}, g.options().dtype(scalar_type(dt)));
-    if (!M || !K) return dx;
-    if (!N) return dx.zero_();
-    const bool aligned = (uintptr_t)g.data_ptr() % 16 == 0;
-    auto work = workspace(mx4::grad_input_bytes(M, N, K, gd, aligned), g);
-    mx4::grad_input(g.data_ptr(), gd, aligned, M, N, K,
-                    wc.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(),
-                    dx.data_ptr(), (int)dt, work.data_ptr(), current_stream());
-    return dx;
-}
-
-Tensor grad_weight(const Tensor& g, const Tensor& xc, const Tensor& xs,
-                   int64_t K, int64_t dt) {
-    check_grad(g);
+// the same from rows held in 4 bits
+Tensor linear_q(const Tensor& xc, const Tensor& xs, int64_t K,
+                const Tensor& wc, const Tensor& ws, const OptTensor& bias,
+                int64_t dt, int64_t form) {
     check_packed(xc, xs, K, "mx4_linear: input");
-    const int64_t M = g.size(0), N = g.size(1);
-    TORCH_CHECK(xc.size(1) == M && g.device() == xc.device(),
-                "mx4_linear: output gradient does not match the input");
-    const int gd = dtype_code(g, "mx4_linear: output gradient");
-    c10::DeviceGuard guard(g.device());
-    auto dw = at::empty({N, K}, g.options().dtype(scalar_type(dt)));
-    if (!N || !K) return dw;
-    if (!M) return dw.zero_();
-    auto work = workspace(mx4::grad_weight_bytes(M, N, K, gd), g);
-    mx4::grad_weight(g.data_ptr(), gd, M, N, K, xc.data_ptr<uint8_t>(),
-                     xs.data_ptr<uint8_t>(), dw.data_ptr(), (int)dt,
-                     work.data_ptr(), current_stream());
-    return dw;
+    check_packed(wc, ws, K, "mx4_linear: weight");
+    CHECK_VALUE(xc.device() == wc.device(), "mx4_linear: one GPU for all");
+    scalar_type(dt);
+    c10::DeviceGuard guard(xc.device());
+    return product_q(xc, xs, K, wc, ws, bias, {xc.size(1), wc.size(1)}, (int)dt,
+                     form);
 }
 
-Tensor col_sum(const Tensor& g, int64_t dt) {
-    check_grad(g);
-    const int64_t M = g.size(0), N = g.size(1);
-    const int gd = dtype_code(g, "mx4_linear: output gradient");
-    c10::DeviceGuard guard(g.device());
-    auto out = at::empty({N}, g.options().dtype(scalar_type(dt)));
-    if (!N) return out;
-    if (!M) return out.zero_();
-    auto work = workspace(mx4::col_sum_bytes(M, N), g);
-    mx4::col_sum(g.data_ptr(), gd, M, N, out.data_ptr(), (int)dt,
-                 work.data_ptr(), current_stream());
-    return out;
+// Q(x) Q(w)^T + bias, and what its gradients want of it
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_train(
+        const Tensor& x, const Tensor& w, const OptTensor& bias) {
+    const int dt = dtype_code(x, "mx4_linear: input");
+    const int wdt = dtype_code(w, "mx4_linear: weight");
+    const Tensor x2 = matrix(x, "mx4_linear: input");
+    const int64_t K = x2.size(1);
+    CHECK_VALUE(w.dim() == 2 && w.size(1) == K, "mx4_linear: input ",
+                x.sizes(), " and weight ", w.sizes(), " do not match");
+    CHECK_VALUE(x.device() == w.device(), "mx4_linear: input on ", x.device(),
+                ", weight on ", w.device());
+    c10::DeviceGuard guard(x.device());
+    Packed pw = pack(matrix(w, "mx4_linear: weight"), wdt);
+    Packed px = pack(x2, dt);
+    Tensor y = product_q(px.codes, px.scales, K, pw.codes, pw.scales, bias,
+                         shape_of(x, w.size(0)), dt, -1);
+    return {y, px.codes, px.scales, pw.codes, pw.scales};
+}
+
+// Gradients of the product: to the input (type dx_dt) where weights are given,
+// to the weight (dw_dt) where rows are, to the bias (db_dt); -1 leaves one out.
+std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
+        const Tensor& grad, const OptTensor& wc, const OptTensor& ws,
+        const OptTensor& xc, const OptTensor& xs, int64_t K, int64_t dx_dt,
+        int64_t dw_dt, int64_t db_dt) {
+    CHECK_VALUE(grad.is_cuda() && grad.dim() >= 1,
+                "mx4_linear: output gradient: rows on the GPU");
+    const int gd = dtype_code(grad, "mx4_linear: output gradient");
+    const int64_t N = grad.size(-1);
+    int64_t M = 1;
+    for (int64_t i = 0; i + 1 < grad.dim(); ++i) M *= grad.size(i);
+    CHECK_VALUE(M < (1L << 31) && N < (1L << 22),
+                "mx4_linear: output gradient: too large");
+    c10::DeviceGuard guard(grad.device());
+    const Tensor g = grad.contiguous();
+    const bool aligned = (uintptr_t)g.data_ptr() % 16 == 0;
+    const hipStream_t stream = current_stream();
+    OptTensor dx, dw, db;
+    auto make = [&](std::vector<int64_t> shape, int64_t dt) {
+        return at::empty(shape, g.options().dtype(scalar_type(dt)));
+    };
+    if (dx_dt >= 0) {
+        check_packed(*wc, *ws, K, "mx4_linear: weight");
+        CHECK_VALUE(wc->size(1) == N && g.device() == wc->device(),
+                    "mx4_linear: output gradient does not match the weight");
+        dx = make(shape_of(grad, K), dx_dt);
+        if (M && K && !N) {
+            dx->zero_();
+        } else if (M && K) {
+            auto work = workspace(mx4::grad_input_bytes(M, N, K, gd, aligned), g);
+            mx4::grad_input(g.data_ptr(), gd, aligned, M, N, K,
+                            wc->data_ptr<uint8_t>(), ws->data_ptr<uint8_t>(),
+                            dx->data_ptr(), (int)dx_dt, work.data_ptr(), stream);
+        }
+    }
+    if (dw_dt >= 0) {
+        check_packed(*xc, *xs, K, "mx4_linear: input");
+        CHECK_VALUE(xc->size(1) == M && g.device() == xc->device(),
+                    "mx4_linear: output gradient does not match the input");
+        dw = make({N, K}, dw_dt);
+        if (N && K && !M) {
+            dw->zero_();
+        } else if (N && K) {
+            auto work = workspace(mx4::grad_weight_bytes(M, N, K, gd), g);
+            mx4::grad_weight(g.data_ptr(), gd, M, N, K, xc->data_ptr<uint8_t>(),
+                             xs->data_ptr<uint8_t>(), dw->data_ptr(),
+                             (int)dw_dt, work.data_ptr(), stream);
+        }
+    }
+    if (db_dt >= 0) {
+        db = make({N}, db_dt);
+        if (N && !M) {
+            db->zero_();
+        } else if (N) {
+            auto work = workspace(mx4::col_sum_bytes(M, N), g);
+            mx4::col_sum(g.data_ptr(), gd, M, N, db->data_ptr(), (int)db_dt,
+                         work.data_ptr(), stream);
+        }
+    }
+    return {dx, dw, db};
 }
 
 // ---------------------------------------------------------------------------
@@ -228,9 +307,11 @@ Tensor col_sum(const Tensor& g, int64_t dt) {
 
 void check_list(const std::vector<Tensor>& ts, const char* what) {
     for (const auto& t : ts) {
-        TORCH_CHECK(t.layout() == at::kStrided && t.is_cuda(), what,
-                    ": dense tensors on the GPU");
-        TORCH_CHECK(t.device() == ts[0].device(), what, ": one GPU for all");
+        CHECK_TYPE(t.layout() == at::kStrided, what, ": dense tensors, not ",
+                   t.layout());
+        CHECK_VALUE(t.device() == ts[0].device(), what, ": tensors on ",
+                    ts[0].device(), " and ", t.device());
+        CHECK_VALUE(t.is_cuda(), what, ": on ", t.device(), ", not on a GPU");
         dtype_code(t, what);
     }
 }
@@ -266,7 +347,7 @@ void check_apart(const std::vector<gradclip::Item>& items) {
 int norm_kind(double p) {
     if (p == 2.0) return gradclip::L2;
     if (p == 1.0) return gradclip::L1;
-    TORCH_CHECK(std::isinf(p) && p > 0, "norm_type: 1, 2 or inf, not ", p);
+    CHECK_VALUE(std::isinf(p) && p > 0, "norm_type: 1, 2 or inf, not ", p);
     return gradclip::LINF;
 }
 
@@ -299,21 +380,22 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
                   const std::vector<Tensor>& outs, double max_norm, double p) {
     const int kind = norm_kind(p);
     TORCH_CHECK(!grads.empty(), "clip_grads_: an empty list");
-    TORCH_CHECK(max_norm >= 0, "clip_grads_: max_norm is negative or NaN");
-    TORCH_CHECK(grads.size() == outs.size(), "clip_grads_: ", grads.size(),
+    CHECK_VALUE(max_norm >= 0, "clip_grads_: max_norm ", max_norm);
+    CHECK_VALUE(grads.size() == outs.size(), "clip_grads_: ", grads.size(),
                 " gradients, ", outs.size(), " outputs");
     check_list(grads, "clip_grads_");
     check_list(outs, "clip_grads_: out");
-    TORCH_CHECK(grads[0].device() == outs[0].device(),
-                "clip_grads_: one GPU for all");
+    CHECK_VALUE(grads[0].device() == outs[0].device(),
+                "clip_grads_: gradients on ", grads[0].device(), ", out on ",
+                outs[0].device());
     c10::DeviceGuard guard(grads[0].device());
     std::vector<gradclip::Item> items;
     std::vector<Tensor> kept;
     items.reserve(grads.size());
     for (size_t i = 0; i < grads.size(); ++i) {
         const Tensor &g = grads[i], &o = outs[i];
-        TORCH_CHECK(g.sizes() == o.sizes(), "clip_grads_: out ", i,
-                    " has another shape");
+        CHECK_VALUE(g.sizes() == o.sizes(), "clip_grads_: out ", o.sizes(),
+                    " for a gradient ", g.sizes());
         TORCH_CHECK(o.is_non_overlapping_and_dense(), "clip_grads_: tensor ",
                     i, " is written and has gaps or shares elements with "
                     "itself");
@@ -335,6 +417,8 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
     gradclip::norm(items, kind, max_norm, norm.data_ptr<float>(),
                    work.data_ptr<double>(), stream);
     gradclip::scale(items, work.data_ptr<double>(), stream);
+    for (const auto& o : outs)           // written behind autograd's back
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     return norm;
 }
 
@@ -343,17 +427,17 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
 void register_mx4(pybind11::module& m) {
     m.def("mx4_quantize", &quantize, "rows to MX4 codes and scales");
     m.def("mx4_dequantize", &dequantize, "MX4 codes and scales to values");
-    namespace py = pybind11;
     m.def("mx4_linear", &linear, "Q(x) W^T + bias", py::arg("x"),
-          py::arg("codes"), py::arg("scales"), py::arg("bias"),
+          py::arg("codes"), py::arg("scales"), py::arg("K"), py::arg("bias"),
           py::arg("form") = -1);
     m.def("mx4_linear_q", &linear_q, "X W^T + bias from 4-bit rows",
           py::arg("xcodes"), py::arg("xscales"), py::arg("K"),
           py::arg("codes"), py::arg("scales"), py::arg("bias"),
           py::arg("dtype"), py::arg("form") = -1);
-    m.def("mx4_grad_input", &grad_input, "g W");
-    m.def("mx4_grad_weight", &grad_weight, "g^T X");
-    m.def("col_sum", &col_sum, "column sums of a matrix");
+    m.def("mx4_linear_train", &linear_train,
+          "Q(x) Q(w)^T + bias, and the rounded x and w");
+    m.def("mx4_linear_backward", &linear_backward,
+          "gradients to the input, the weight and the bias");
     m.def("grad_norm", &grad_norm, "global norm of a list of tensors");
     m.def("clip_grads", &clip_grads,
           "a list scaled to a global norm of at most max_norm; returns the norm");

@@ -181,19 +181,21 @@ void quantize(const void* x, int dt, long rows, long K, long ldx,
 void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
                 long K, void* out, int dt, hipStream_t stream);
 
-// Forms of the product. linear_form() and linear_q_form() choose; each form
-// is right for every size.
+// Forms of the product; linear_form() and linear_q_form() choose. Each is right
+// for every size.
 enum Form : int {
-    ROWS16 = 0,       // 16 x 16 of y a block, its waves share the sum
-    ROWS32 = 1,       // 32 x 32 of y a block, the same
-    ROUNDING = 2,     // tiles; x rounded on its way into LDS
-    TILES128 = 3,     // tiles of 4-bit rows; x rounded before
-    TILES256 = 4,
-    FORMS = 5
+    ROWS16 = 0,       // 16 x 16 of y a block, x rounded by each block
+    ROWS32 = 1,       // 32 x 32, the same
+    ROUNDING = 2,     // tiles of 128 rows, x rounded on its way into LDS
+    HELD16 = 3,       // x rounded before; then the same from 4-bit rows,
+    HELD32 = 4,
+    TILES128 = 5,     // or tiles of them
+    TILES256 = 6,
+    FORMS = 7
 };
 
 // y[M,N] = Q(x) W^T + bias
-int linear_form(long M, long K, long N, int dt, bool aligned);
+int linear_form(long M, long K, long N, bool aligned);
 size_t linear_bytes(int form, long M, long K);        // of workspace
 void linear(const void* x, int dt, long M, long K, long ldx,
             const uint8_t* wc, const uint8_t* ws, long N, const void* bias,

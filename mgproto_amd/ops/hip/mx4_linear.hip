@@ -138,7 +138,7 @@ void launch_rows(const void* x, const uint8_t* xs, long M, long K, long ldx,
             dim3((unsigned)(mt * nt)), dim3(256), 0, stream, x, xs, M, (int)K, \
             (int)steps_of(K), ldx, wc, ws, N, bias, bias_dt, (typename Elem<OT>::T*)y, \
             (int)nt); } while (0)
-    if (form == ROWS16) MX4_L(1);
+    if (form == ROWS16 || form == HELD16) MX4_L(1);
     else MX4_L(2);
     #undef MX4_L
 }
@@ -147,21 +147,42 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace
 
-int linear_form(long M, long K, long N, int dt, bool aligned) {
-    if (M <= 16) return ROWS16;
-    if (M * N <= 1024L * 1024) return ROWS32;
-    if (N <= 512) return ROUNDING;
+// The choice, by the multiplications M K N (at least 16 rows count); times in
+// us, bf16, on an MI355X.
+//
+// Rounding in the blocks saves a launch (4 us) and a pass over x, but every
+// block rounds its rows again: 784x1024->256 5.4 against 9.0 with the rounding
+// before, 64x4096->4096 (2^30) 12.8 against 11.5, 128x4096->4096 22 against 16.
+// Rows that do not start on 16 bytes are read element by element: 777x333->1001
+// (2^28) 17 against 10.
+//
+// Many rows and few columns: x's way from memory counts, and tiles of 128 rows
+// round it on the way: 62720x1024->256 39 against 42, 1003520x256->64 146
+// against 208. With more columns the rows would be rounded again and again
+// (62720x512->512 43 against 36), and a short K leaves nothing to overlap
+// (1003520x64->64 167 against 87).
+int linear_form(long M, long K, long N, bool aligned) {
+    const double work = (double)(M > 16 ? M : 16) * K * N;
+    if (work < (aligned ? 0x1p30 : 0x1p27)) return M <= 16 ? ROWS16 : ROWS32;
+    if (aligned && M >= 4096 && N <= 256 && K >= 256) return ROUNDING;
     return linear_q_form(M, K, N);
 }
 
+// Small blocks share a sum among their waves and read past LDS: 128x4096->4096
+// (2^31) 11.5 against 16.7 us with tiles of 128, 256x4096->4096 20.8 against
+// 16.7. Tiles of 256 take half the bytes a result, but there have to be some for
+// each of 256 units: 8192x4096->16384 (2048 tiles) 262 against 318,
+// 2048x4096->4096 (128 tiles) 34 against 25; with 128 columns half of a tile is
+// empty, 250880x512->128 31 against 24.
 int linear_q_form(long M, long K, long N) {
-    if (M <= 16) return ROWS16;
-    if (M * N <= 1024L * 1024) return ROWS32;
-    return (M + 255) / 256 * ((N + 255) / 256) >= 256 ? TILES256 : TILES128;
+    if (M <= 16) return HELD16;
+    if ((double)M * K * N <= 0x1p31) return HELD32;
+    const long tiles = (M + 255) / 256 * ((N + 255) / 256);
+    return N > 128 && tiles >= 384 ? TILES256 : TILES128;
 }
 
 size_t linear_bytes(int form, long M, long K) {
-    if (form < TILES128) return 0;
+    if (form < HELD16) return 0;
     return up256(code_bytes(M, K)) + scale_bytes(M, K);
 }
 
@@ -174,7 +195,7 @@ void linear(const void* x, int dt, long M, long K, long ldx,
         rounding(x, dt, vec, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream);
         return;
     }
-    if (form > ROUNDING) {
+    if (form >= HELD16) {
         uint8_t* xc = (uint8_t*)work;
         uint8_t* xs = xc + up256(code_bytes(M, K));
         quantize(x, dt, M, K, ldx, xc, xs, stream);
@@ -197,7 +218,7 @@ void linear(const void* x, int dt, long M, long K, long ldx,
 void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
               int bias_dt, void* y, int dt, int form, hipStream_t stream) {
-    if (form >= ROUNDING) {
+    if (form >= TILES128) {
         tiles(xc, xs, M, K, wc, ws, N, bias, bias_dt, y, dt,
               form == TILES256, stream);
         return;

@@ -243,10 +243,10 @@ void tiles(const uint8_t* xc, const uint8_t* xs, long M, long K,
     // 256 units: one block of 147 KB of LDS each, or two of 73 KB
     #define MX4_L(OT) \
         launch_tiles<OT, 256, 256, 2, 4, 4>(xc, xs, M, K, wc, ws, N, bias, \
-                                            bias_dt, y, 256, 2, stream)
+                                            bias_dt, y, 256, 4, stream)
     #define MX4_S(OT) \
         launch_tiles<OT, 128, 128, 2, 2, 4>(xc, xs, M, K, wc, ws, N, bias, \
-                                            bias_dt, y, 512, 4, stream)
+                                            bias_dt, y, 512, 8, stream)
     if (large) {
         if (dt == F32) MX4_L(F32);
         else if (dt == BF16) MX4_L(BF16);

@@ -74,6 +74,13 @@ class MX4Tensor:
         self.shape, self.dtype = shape, dtype
 
     @classmethod
+    def _of(cls, codes, scales, shape, dtype) -> 'MX4Tensor':
+        """From what the kernels made."""
+        q = object.__new__(cls)
+        q.codes, q.scales, q.shape, q.dtype = codes, scales, shape, dtype
+        return q
+
+    @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16) -> 'MX4Tensor':
         """From codes [..., K/2] and scales [..., K/32] in plain order, K a
@@ -121,13 +128,8 @@ class MX4Tensor:
 
 
 def _matrix(x: torch.Tensor) -> torch.Tensor:
-    """[..., K] -> [M, K] with contiguous rows; a view where it can be."""
-    K = x.shape[-1]
-    M = math.prod(x.shape[:-1])
-    x2 = x.reshape(M, K)
-    if K > 1 and x2.stride(1) != 1 or M > 1 and x2.stride(0) < K:
-        x2 = x2.contiguous()
-    return x2
+    """[..., K] -> [M, K]."""
+    return x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
 
 
 def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
@@ -135,13 +137,10 @@ def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
     _check_float(x, 'mx4_quantize')
     if x.dim() < 1:
         raise ValueError('mx4_quantize: a tensor of rows, not a number')
-    x2 = _matrix(x.detach())
-    ext = _ext(x2)
-    if ext is not None:
-        codes, scales = ext.mx4_quantize(x2)
-    else:
-        codes, scales = reference.mx4_quantize(x2)
-    return MX4Tensor(codes, scales, x.shape, x.dtype)
+    ext = _ext(x)
+    codes, scales = (ext.mx4_quantize(x) if ext is not None
+                     else reference.mx4_quantize(_matrix(x.detach())))
+    return MX4Tensor._of(codes, scales, x.shape, x.dtype)
 
 
 def mx4_dequantize(q: MX4Tensor,
@@ -153,64 +152,48 @@ def mx4_dequantize(q: MX4Tensor,
         raise TypeError(f'mx4_dequantize: no values of type {dtype}')
     ext = _ext(q.codes)
     if ext is not None:
-        out = ext.mx4_dequantize(q.codes, q.scales, q.K, _CODE[dtype])
+        out = ext.mx4_dequantize(q.codes, q.scales, q.shape[-1], _CODE[dtype])
     else:
         out = reference.mx4_dequantize(q.codes, q.scales, q.K, dtype)
-    return out.view(q.shape)
+    return out if len(q.shape) == 2 else out.view(q.shape)
 
 
 class _MX4Linear(torch.autograd.Function):
     """weight: a float [N, K] matrix, or None with (wc, ws) held in 4 bits."""
 
     @staticmethod
-    def forward(ctx, x2, weight, wc, ws, bias, train):
-        ext = _ext(x2)
-        K = x2.shape[1]
-        if weight is not None:
-            w2 = weight if weight.stride(1) == 1 or K <= 1 \
-                else weight.contiguous()
-            wc, ws = (ext.mx4_quantize(w2) if ext is not None
-                      else reference.mx4_quantize(w2))
-        need_w = train and weight is not None and ctx.needs_input_grad[1]
+    def forward(ctx, x, weight, wc, ws, bias):
+        ext = _ext(x)
+        K = x.shape[-1]
+        need_x, need_w = ctx.needs_input_grad[:2]
         xc = xs = None
-        if need_w:      # the rounded rows are kept, a quarter of x
-            xc, xs = (ext.mx4_quantize(x2) if ext is not None
-                      else reference.mx4_quantize(x2))
         if ext is None:
-            if xc is None:
-                xc, xs = reference.mx4_quantize(x2)
-            y = reference.mx4_product(xc, xs, wc, ws, K, bias, x2.dtype)
-        elif need_w:
-            y = ext.mx4_linear_q(xc, xs, K, wc, ws, bias, _CODE[x2.dtype])
+            xc, xs = reference.mx4_quantize(_matrix(x))
+            if weight is not None:
+                wc, ws = reference.mx4_quantize(weight)
+            y = reference.mx4_product(xc, xs, wc, ws, K, bias, x.dtype)
+            y = y.view(*x.shape[:-1], wc.shape[1])
+        elif need_w:    # the rounded rows are kept, a quarter of x in bf16
+            y, xc, xs, wc, ws = ext.mx4_linear_train(x, weight, bias)
         else:
-            y = ext.mx4_linear(x2, wc, ws, bias)
-        ctx.save_for_backward(*((xc, xs) if need_w else (None, None)),
-                              *((wc, ws) if train and ctx.needs_input_grad[0]
-                                else (None, None)))
-        ctx.K, ctx.x_dtype = K, x2.dtype
-        ctx.w_dtype = weight.dtype if weight is not None else None
-        ctx.b_dtype = bias.dtype if bias is not None else None
+            if weight is not None:
+                wc, ws = ext.mx4_quantize(weight)
+            y = ext.mx4_linear(x, wc, ws, K, bias)
+        ctx.save_for_backward(*((wc, ws) if need_x else (None, None)),
+                              *((xc, xs) if need_w else (None, None)))
+        ctx.K = K
+        ctx.types = tuple(
+            _CODE[t.dtype] if need else -1 for t, need in
+            zip((x, weight, bias), (need_x, need_w, ctx.needs_input_grad[4])))
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        xc, xs, wc, ws = ctx.saved_tensors
-        g = g.contiguous()
-        ext = _ext(g)
-        dx = dw = db = None
-        if ctx.needs_input_grad[0]:
-            dx = (ext.mx4_grad_input(g, wc, ws, ctx.K, _CODE[ctx.x_dtype])
-                  if ext is not None else
-                  reference.mx4_grad_input(g, wc, ws, ctx.K, ctx.x_dtype))
-        if ctx.needs_input_grad[1]:
-            dw = (ext.mx4_grad_weight(g, xc, xs, ctx.K, _CODE[ctx.w_dtype])
-                  if ext is not None else
-                  reference.mx4_grad_weight(g, xc, xs, ctx.K, ctx.w_dtype))
-        if ctx.needs_input_grad[4]:
-            db = (ext.col_sum(g, _CODE[ctx.b_dtype]) if ext is not None
-                  else g.float().sum(0).to(ctx.b_dtype))
-        return dx, dw, None, None, db, None
+        backward = (reference.mx4_backward if _ext(g) is None
+                    else _ext(g).mx4_linear_backward)
+        dx, dw, db = backward(g, *ctx.saved_tensors, ctx.K, *ctx.types)
+        return dx, dw, None, None, db
 
 
 def mx4_linear(x: torch.Tensor, weight: Union[MX4Tensor, torch.Tensor],
@@ -221,8 +204,16 @@ def mx4_linear(x: torch.Tensor, weight: Union[MX4Tensor, torch.Tensor],
     A NaN or an infinity in a block of x makes its row NaN, one in a block of
     the weight its column. Differentiable once, in x, a float weight and bias.
     """
+    held = type(weight) is MX4Tensor
+    train = torch.is_grad_enabled() and (
+        x.requires_grad or not held and weight.requires_grad
+        or bias is not None and bias.requires_grad)
+    if held and not train and x.is_cuda and len(weight.shape) == 2:
+        ext = _ext(x)                  # refuses what the checks below refuse
+        if ext is not None:
+            return ext.mx4_linear(x, weight.codes, weight.scales,
+                                  weight.shape[1], bias)
     _check_float(x, 'mx4_linear: input')
-    held = isinstance(weight, MX4Tensor)
     if not held:
         _check_float(weight, 'mx4_linear: weight')
     if x.dim() < 1:
@@ -241,9 +232,8 @@ def mx4_linear(x: torch.Tensor, weight: Union[MX4Tensor, torch.Tensor],
         if bias.device != x.device:
             raise ValueError(f'mx4_linear: input on {x.device}, bias on '
                              f'{bias.device}')
-        bias = bias.contiguous()
-    x2 = _matrix(x)
     wc, ws = (weight.codes, weight.scales) if held else (None, None)
-    y = _MX4Linear.apply(x2, None if held else weight, wc, ws, bias,
-                         torch.is_grad_enabled())
-    return y.view(*x.shape[:-1], weight.shape[0])
+    if not train:
+        x, bias = x.detach(), None if bias is None else bias.detach()
+        weight = weight if held else weight.detach()
+    return _MX4Linear.apply(x, None if held else weight, wc, ws, bias)

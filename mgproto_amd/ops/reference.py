@@ -396,13 +396,22 @@ def mx4_product(xc, xs, wc, ws, K: int, bias, dtype) -> torch.Tensor:
     return y.to(dtype)
 
 
-def mx4_grad_input(g, wc, ws, K: int, dtype) -> torch.Tensor:
-    return (g.float() @ mx4_dequantize(wc, ws, K, torch.float32)).to(dtype)
-
-
-def mx4_grad_weight(g, xc, xs, K: int, dtype) -> torch.Tensor:
-    return (g.float().t()
-            @ mx4_dequantize(xc, xs, K, torch.float32)).to(dtype)
+def mx4_backward(g, wc, ws, xc, xs, K: int, dx_type: int, dw_type: int,
+                 db_type: int):
+    """Straight-through gradients; types as codes (0 float32, 1 bfloat16, 2
+    float16), -1 for one that is not wanted."""
+    types = (torch.float32, torch.bfloat16, torch.float16)
+    f = g.reshape(math.prod(g.shape[:-1]), g.shape[-1]).float()
+    dx = dw = db = None
+    if dx_type >= 0:
+        dx = (f @ mx4_dequantize(wc, ws, K, torch.float32)).to(types[dx_type])
+        dx = dx.view(*g.shape[:-1], K)
+    if dw_type >= 0:
+        dw = (f.t() @ mx4_dequantize(xc, xs, K, torch.float32)).to(
+            types[dw_type])
+    if db_type >= 0:
+        db = f.sum(0).to(types[db_type])
+    return dx, dw, db
 
 
 # ---------------------------------------------------------------------------

@@ -143,11 +143,11 @@ def test_refusals(device):
         ops.clip_grads_([t], -1.0)
     with pytest.raises(ValueError, match='max_norm'):
         ops.clip_grads_([t], math.nan)
-    with pytest.raises(TypeError, match='float64'):
+    with pytest.raises(TypeError, match='float64|Double'):
         ops.grad_norm([t.double()])
-    with pytest.raises(TypeError, match='sparse'):
-        ops.grad_norm([torch.eye(3).to_sparse()])
-    with pytest.raises(TypeError, match='NoneType'):
+    with pytest.raises(TypeError, match='[sS]parse'):
+        ops.grad_norm([t, torch.eye(3, device=device).to_sparse()])
+    with pytest.raises(TypeError):
         ops.grad_norm([t, None])
     with pytest.raises(ValueError, match='meta'):
         ops.grad_norm([t, t.to('meta')])

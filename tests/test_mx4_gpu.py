@@ -122,7 +122,7 @@ def test_whole_numbers_are_exact(M, K, N):
         assert torch.equal(dw.double().cpu(), g.t() @ xv)
 
 
-@pytest.mark.parametrize('form', range(5))
+@pytest.mark.parametrize('form', range(7))
 @pytest.mark.parametrize('M,K,N', SIZES + [(260, 1, 260), (129, 384, 70),
                                            (700, 1000, 520)])
 def test_every_form_at_every_size(M, K, N, form):
@@ -138,7 +138,7 @@ def test_every_form_at_every_size(M, K, N, form):
         for lo in (0, 1, 8):
             xd = base[:, lo:lo + K]
             xd.copy_(x)
-            y = ext.mx4_linear(xd, wq.codes, wq.scales, b.cuda(), form)
+            y = ext.mx4_linear(xd, wq.codes, wq.scales, K, b.cuda(), form)
             assert torch.equal(y.cpu(), want.to(dtype))
             base.fill_(math.nan)
         q = ops.mx4_quantize(x.to(dtype).cuda())
@@ -277,10 +277,25 @@ def test_refusals():
     ext = ops._native_or_die()
     qd = q.to('cuda')
     x = torch.randn(4, 64, device='cuda')
+    with pytest.raises(ValueError, match='input on cuda'):
+        ops.mx4_linear(x, q)
+    with pytest.raises(ValueError, match='do not match'):
+        ops.mx4_linear(x[:, :63], qd)
+    with pytest.raises(TypeError, match='Double'):
+        ops.mx4_linear(x.double(), qd)
+    with pytest.raises(ValueError, match='bias'):
+        ops.mx4_linear(x, qd, torch.zeros(7, device='cuda'))
+    with pytest.raises(ValueError, match='bias on cpu'):
+        ops.mx4_linear(x, qd, torch.zeros(8))
+    with pytest.raises(ValueError, match='do not match'):
+        ops.mx4_linear(x, ops.mx4_quantize(torch.zeros(2, 8, 64)).to('cuda'))
     with pytest.raises(RuntimeError, match='do not hold rows'):
-        ext.mx4_linear(x, qd.codes[:, :, :32].contiguous(), qd.scales, None)
+        ext.mx4_linear(x, qd.codes[:, :, :32].contiguous(), qd.scales, 64,
+                       None)
     with pytest.raises(RuntimeError, match='contiguous'):
-        ext.mx4_linear(x.t(), qd.codes, qd.scales, None)
-    with pytest.raises(RuntimeError, match='does not match'):
-        ext.mx4_grad_input(torch.randn(4, 7, device='cuda'), qd.codes,
-                           qd.scales, 64, 0)
+        ext.mx4_linear(x, qd.codes[:, :, ::2], qd.scales, 64, None)
+    with pytest.raises(ValueError, match='no form'):
+        ext.mx4_linear(x, qd.codes, qd.scales, 64, None, 7)
+    with pytest.raises(ValueError, match='does not match'):
+        ext.mx4_linear_backward(torch.randn(4, 7, device='cuda'), qd.codes,
+                                qd.scales, None, None, 64, 0, -1, -1)
