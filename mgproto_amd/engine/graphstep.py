@@ -62,13 +62,13 @@ class GraphedStep:
             ...eager path...
 
     ``stats`` is a dict of DEVICE scalars: loss / ce / mine / aux /
-    n_correct (floats accumulate trainer-side exactly like the eager
+    n_correct / grad_norm (floats accumulate trainer-side exactly like the eager
     path's detached tensors).
     """
 
     def __init__(self, model, aux_criterion, coefs, device, batch_size,
                  img_size, amp_dtype='bf16', warmup_steps=3,
-                 channels_last=True):
+                 channels_last=True, clip_grad_norm=None):
         self.model = model
         self.aux = aux_criterion
         self.coefs = coefs
@@ -76,6 +76,7 @@ class GraphedStep:
         self.batch_size = batch_size
         self.warmup_steps = warmup_steps
         self.amp_dtype = amp_dtype
+        self.clip_grad_norm = clip_grad_norm
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.broken = False          # capture failed -> permanent eager
         self._sig = None
@@ -90,7 +91,7 @@ class GraphedStep:
                                       device=device)
         z = lambda: torch.zeros((), device=device)  # noqa: E731
         self.stats = {'loss': z(), 'ce': z(), 'mine': z(), 'aux': z(),
-                      'n_correct': z()}
+                      'n_correct': z(), 'grad_norm': z()}
 
     # ------------------------------------------------------------------
     def _signature(self, optimizer, use_mine, em_active):
@@ -141,6 +142,10 @@ class GraphedStep:
         loss.backward()
         if reducer is not None:
             reducer.finalize()
+        if self.clip_grad_norm is not None:
+            from .trainer import clip_optimizer_grads
+            self.stats['grad_norm'].copy_(
+                clip_optimizer_grads(optimizer, self.clip_grad_norm))
         optimizer.step()
         if em_active:
             self.model.update_GMM()

@@ -22,6 +22,7 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from .. import ops
 from ..utils.helpers import list_of_distances
 
 
@@ -34,6 +35,16 @@ def _amp_ctx(device, amp_dtype):
         dt = torch.bfloat16 if amp_dtype == 'bf16' else torch.float16
         return torch.autocast(device_type='cuda', dtype=dt)
     return contextlib.nullcontext()
+
+
+def clip_optimizer_grads(optimizer, max_norm: float):
+    """Scales the gradients of the optimizer's parameters to a global norm of
+    at most ``max_norm``; the norm before, as a device scalar. After a
+    distributed reduction every rank has the same gradients and gets the same
+    factor."""
+    return ops.clip_grads_([p.grad for g in optimizer.param_groups
+                            for p in g['params'] if p.grad is not None],
+                           max_norm)
 
 
 class EMRunner:
@@ -69,7 +80,8 @@ def _training(model, dataloader, optimizer=None, aux_criterion=None,
               use_mine=False, update_GMM=False, class_specific=True,
               coefs=None, log=print, device=None, amp_dtype='bf16',
               em_runner: Optional[EMRunner] = None, metrics=None,
-              comm=None, print_every=20, reducer=None, graph_step=None):
+              comm=None, print_every=20, reducer=None, graph_step=None,
+              clip_grad_norm=None):
     device = device or next(_unwrap(model).parameters()).device
     m = _unwrap(model)
     start = time.time()
@@ -113,6 +125,7 @@ def _training(model, dataloader, optimizer=None, aux_criterion=None,
                                      use_mine=use_mine)
             loss, cross_entropy = st['loss'], st['ce']
             mine_loss, aux_loss = st['mine'], st['aux']
+            grad_norm = st['grad_norm']
             n_examples += target.numel()
             n_correct += st['n_correct']
             n_batches += 1
@@ -156,6 +169,8 @@ def _training(model, dataloader, optimizer=None, aux_criterion=None,
             with timer.phase('optimizer'):
                 if reducer is not None:
                     reducer.finalize()  # drain async all-reduces before step
+                if clip_grad_norm is not None:
+                    grad_norm = clip_optimizer_grads(optimizer, clip_grad_norm)
                 optimizer.step()
 
             # EM update (reference train_and_test.py:61-63; update_interval=1)
@@ -187,7 +202,9 @@ def _training(model, dataloader, optimizer=None, aux_criterion=None,
                              'train/mine': float(mine_loss),
                              'train/aux': float(aux_loss),
                              'train/acc': acc,
-                             'train/mem_ratio': float(full_ratio)})
+                             'train/mem_ratio': float(full_ratio),
+                             **({'train/grad_norm': float(grad_norm)}
+                                if clip_grad_norm is not None else {})})
 
     if em_runner is not None:
         em_runner.sync()

@@ -18,6 +18,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import ops
+
 
 def _usable(x: torch.Tensor, conv: nn.Conv2d) -> bool:
     # Measured on the flagship step: plain hipBLASLt matmul on these
@@ -56,7 +58,85 @@ def conv1x1(x: torch.Tensor, conv: nn.Conv2d) -> torch.Tensor:
 
 class GemmConv2d(nn.Conv2d):
     """Drop-in nn.Conv2d that takes the hipBLASLt GEMM path for stride-1
-    1x1 convs on channels-last bf16 inputs (state dict unchanged)."""
+    1x1 convs on channels-last bf16 inputs (state dict unchanged), or the
+    4-bit product where ``use_mx4`` asked for it."""
+
+    mx4 = None          # None, 'train' or 'held'
 
     def forward(self, x):
+        if self.mx4 is not None:
+            return self._mx4_forward(x)
         return conv1x1(x, self)
+
+    # ------------------------------------------------------------ 4-bit form
+    def _mx4_pack(self):
+        w = self.weight.detach()
+        q = ops.mx4_quantize(w.reshape(self.out_channels, -1))
+        # not in the state dict: made from the weight again where that changes
+        self.register_buffer('_mx4_codes', q.codes, persistent=False)
+        self.register_buffer('_mx4_scales', q.scales, persistent=False)
+        self._mx4_version = _version(self.weight)
+
+    def _mx4_weight(self):
+        if self.mx4 == 'train':
+            return self.weight.view(self.out_channels, -1)
+        if (self.training and torch.is_grad_enabled()
+                and self.weight.requires_grad):
+            raise RuntimeError(
+                'this 1x1 convolution holds its weight in 4 bits and cannot '
+                'train it: use_mx4(model, train=True), or freeze the weight')
+        if self._mx4_version != _version(self.weight):
+            self._mx4_pack()
+        return ops.MX4Tensor(self._mx4_codes, self._mx4_scales,
+                             (self.out_channels, self.in_channels))
+
+    def _mx4_forward(self, x):
+        kind = x.device.type
+        if torch.is_autocast_enabled(kind):
+            x = x.to(torch.get_autocast_dtype(kind))
+        sh, sw = self.stride
+        # NHWC rows: a view of a channels-last tensor, strided ones copied
+        rows = x[:, :, ::sh, ::sw].permute(0, 2, 3, 1)
+        y = ops.mx4_linear(rows, self._mx4_weight(), self.bias)
+        return y.permute(0, 3, 1, 2)                   # channels_last NCHW
+
+
+def _version(w: torch.Tensor) -> int:
+    return -1 if w.is_inference() else w._version
+
+
+def use_mx4(module: nn.Module, train: bool = False) -> int:
+    """Turns the 1x1 convolutions of ``module`` to 4-bit products
+    (``ops.mx4_linear``: weights and inputs rounded to MX blocks along the
+    channels, fp32 sums). Returns how many there are.
+
+    ``train=False`` rounds the weights now and holds them in 4 bits, for
+    inference; a later in-place update of a weight (an optimizer's, or
+    ``load_state_dict``) rounds it again, one through ``.data`` is not seen.
+    ``train=True`` rounds them in every forward, with straight-through
+    gradients to the float weights: fine-tuning for the former. The state dict
+    stays what it was either way. ``use_mx4(model.features)`` leaves the
+    add-on layers, which the densities read, in full precision."""
+    n = 0
+    for m in module.modules():
+        if not isinstance(m, GemmConv2d) or not _plain_1x1(m):
+            continue
+        m.mx4 = 'train' if train else 'held'
+        if not train:
+            m._mx4_pack()
+        n += 1
+    return n
+
+
+def no_mx4(module: nn.Module):
+    """The reverse of ``use_mx4``."""
+    for m in module.modules():
+        if isinstance(m, GemmConv2d) and m.mx4 is not None:
+            if m.mx4 == 'held':
+                del m._mx4_codes, m._mx4_scales
+            m.mx4 = None
+
+
+def _plain_1x1(conv: nn.Conv2d) -> bool:
+    return (conv.kernel_size == (1, 1) and conv.padding == (0, 0)
+            and conv.groups == 1)

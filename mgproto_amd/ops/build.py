@@ -5,6 +5,7 @@ Usage: ``python -m mgproto_amd.ops.build``. Cross-compiles on CPU-only boxes
 travels with repo snapshots.
 """
 
+import glob
 import os
 import shutil
 import sys
@@ -45,6 +46,19 @@ def build_cpu(verbose: bool = False) -> str:
     return CPU_OUT
 
 
+def _drop_stale(build_dir: str):
+    """Objects older than a header: the generated ninja file knows only their
+    sources."""
+    newest = max((os.path.getmtime(h) for h in
+                  glob.glob(os.path.join(_HERE, 'hip', '*.h'))), default=0)
+    for src in SRC:
+        with open(src) as f:
+            local = '#include "' in f.read()
+        obj = os.path.join(build_dir, os.path.basename(src)[:-4] + '.cuda.o')
+        if local and os.path.isfile(obj) and os.path.getmtime(obj) < newest:
+            os.remove(obj)
+
+
 def build(verbose: bool = False) -> str:
     os.environ.setdefault('PYTORCH_ROCM_ARCH', 'gfx950')
     os.environ.setdefault('MAX_JOBS', '8')
@@ -52,6 +66,7 @@ def build(verbose: bool = False) -> str:
 
     build_dir = os.path.join(_HERE, 'hip', 'build')
     os.makedirs(build_dir, exist_ok=True)
+    _drop_stale(build_dir)
     mod = load(name='_mgproto_hip',
                sources=SRC,
                build_directory=build_dir,

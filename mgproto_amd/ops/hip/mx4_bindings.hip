@@ -250,7 +250,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
     const int64_t N = grad.size(-1);
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < grad.dim(); ++i) M *= grad.size(i);
-    CHECK_VALUE(M < (1L << 31) && N < (1L << 22),
+    CHECK_VALUE(M < (1L << 23) && N < (1L << 22),
                 "mx4_linear: output gradient: too large");
     c10::DeviceGuard guard(grad.device());
     const Tensor g = grad.contiguous();

@@ -115,6 +115,11 @@ void values_t_kernel(const uint8_t* __restrict__ codes,
 // steps of all parts; with more than one split C is fp32 [splits][M][N].
 // LDS rows are 128 bytes; 16-byte piece c of row r lies at c ^ key(r), so
 // that the 16 rows which a read takes at once fall on different banks.
+static __device__ __forceinline__ int a_key(int r) { return (r ^ (r >> 3 & 1)) & 7; }
+static __device__ __forceinline__ int b_key(int r) {      // runs of 4, 16 apart
+    return ((r & 3) | (r >> 4 & 1) << 2) ^ (r >> 5 & 1);
+}
+
 template <int OT>
 __global__ __launch_bounds__(256)
 void product_nt_kernel(const unsigned short* __restrict__ A, long lda,
@@ -124,26 +129,31 @@ void product_nt_kernel(const unsigned short* __restrict__ A, long lda,
                        typename Elem<OT>::T* __restrict__ C) {
     using T = typename Elem<OT>::T;
     __shared__ __attribute__((aligned(16))) unsigned short lds[2][2][BT * BK];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const long m0 = (long)blockIdx.x * BT, n0 = (long)blockIdx.y * BT;
     const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
     const long per = Kc / BK, steps = per * P;
     const long s_lo = steps * blockIdx.z / gridDim.z;
     const long s_hi = steps * (blockIdx.z + 1) / gridDim.z;
+    const int lasta = (int)min((long)BT, M - m0) - 1;
+    const int lastb = (int)min((long)BT, N - n0) - 1;
 
+    // offsets in a tile stay below 2^31: rows are at most 2^22 elements here,
+    // 2^31 / 256 along M (checked by the caller)
     auto stage = [&](long s, int buf) {
         const long p = s / per, k0 = (s - p * per) * BK;
-        const unsigned short* a = A + p * part_stride + k0;
-        const unsigned short* b = B + k0;
+        const unsigned short* a = A + p * part_stride + m0 * lda + k0;
+        const unsigned short* b = B + n0 * ldb + k0;
         #pragma unroll
         for (int q = 0; q < 4; ++q) {          // 1 KB: 8 rows a wave's call
             const int call = wave * 4 + q;
             const int r = call * 8 + (lane >> 3), c = lane & 7;
-            const int ca = c ^ ((r >> 1) & 7);
-            const int cn = c ^ (((r >> 4) & 3) | ((r >> 1) & 1) << 2);
-            copy16_to_lds(a + min(m0 + r, M - 1) * lda + ca * 8, &lds[buf][0][call * 512]);
-            copy16_to_lds(b + min(n0 + r, N - 1) * ldb + cn * 8, &lds[buf][1][call * 512]);
+            copy16_to_lds(a, (unsigned)(min(r, lasta) * lda * 2) + (c ^ a_key(r)) * 16,
+                          lds_address(&lds[buf][0][call * 512]));
+            copy16_to_lds(b, (unsigned)(min(r, lastb) * ldb * 2) + (c ^ b_key(r)) * 16,
+                          lds_address(&lds[buf][1][call * 512]));
         }
     };
 
@@ -158,7 +168,7 @@ void product_nt_kernel(const unsigned short* __restrict__ A, long lda,
     for (long s = s_lo; s < s_hi; ++s, buf ^= 1) {
         // the pieces of this step have to be there, and every wave has to be
         // done with the other buffer before it is filled again
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wait_copies<0>();
         __syncthreads();
         if (s + 1 < s_hi) stage(s + 1, buf ^ 1);
         #pragma unroll
@@ -169,14 +179,13 @@ void product_nt_kernel(const unsigned short* __restrict__ A, long lda,
             for (int i = 0; i < 4; ++i) {
                 const int r = wm + i * 16 + r16;
                 a[i] = *reinterpret_cast<const bf16x8*>(
-                    &lds[buf][0][r * BK + (c ^ ((r >> 1) & 7)) * 8]);
+                    &lds[buf][0][r * BK + (c ^ a_key(r)) * 8]);
             }
             #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = wn + (r16 >> 2) * 16 + j * 4 + (r16 & 3);
                 b[j] = *reinterpret_cast<const bf16x8*>(
-                    &lds[buf][1][r * BK
-                        + (c ^ (((r >> 4) & 3) | ((r >> 1) & 1) << 2)) * 8]);
+                    &lds[buf][1][r * BK + (c ^ b_key(r)) * 8]);
             }
             #pragma unroll
             for (int i = 0; i < 4; ++i)

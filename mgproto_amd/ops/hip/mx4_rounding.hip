@@ -54,14 +54,15 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
             const int s = call / CALLS, c = call % CALLS;
             if (2 * k + s >= steps) break;
             const int r = c * 16 + (lane >> 2);
-            copy16_to_lds(wc + ((size_t)(2 * k + s) * N + n0 + min(r, lastw)) * 64
-                              + ((lane & 3) ^ w_key<FN>(r)) * 16,
-                          wl[buf][s] + c * 1024);
+            copy16_to_lds(wc + ((size_t)(2 * k + s) * N + n0) * 64,
+                          min(r, lastw) * 64 + ((lane & 3) ^ w_key<FN>(r)) * 16,
+                          lds_address(wl[buf][s]) + c * 1024);
         }
         if ((k & 1) == 0 && wave < BN / 64) {    // four steps' scales
             const int r = wave * 64 + lane;
-            copy16_to_lds(ws + ((size_t)(k >> 1) * N + n0 + min(r, lastw)) * 16,
-                          wsl[k >> 1 & 1] + wave * 1024);
+            copy16_to_lds(ws + ((size_t)(k >> 1) * N + n0) * 16,
+                          min(r, lastw) * 16,
+                          lds_address(wsl[k >> 1 & 1]) + wave * 1024);
         }
     };
     u32x4 raw[UNITS][W];
@@ -135,7 +136,7 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     // Waits until a buffer's bytes have arrived and no wave reads the other
     // one any more, and sends for the next.
     auto turn = [&](int k) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        wait_copies<0>();
         __syncthreads();
         if (k + 1 < turns) {
             send_w(k + 1, (k + 1) & 1);

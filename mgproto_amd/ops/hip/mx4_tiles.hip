@@ -38,8 +38,9 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
     static_assert(BM % (16 * WAVES) == 0 && BN % (16 * WAVES) == 0 &&
                   R % (64 * WAVES) == 0 && BM % 64 == 0 &&
                   FM % (XQ + WQ) == 0 && S >= 3, "whole copies");
-    // the ring of codes, and two buffers of scales
-    __shared__ __attribute__((aligned(16))) uint8_t lds[S * R * 64 + 2 * R * 16];
+    // The ring of codes, and as many buffers of scales: where a tile is one
+    // step long, every step brings its own.
+    __shared__ __attribute__((aligned(16))) uint8_t lds[S * (R * 64 + R * 16)];
     uint8_t* const scales = lds + S * R * 64;
     const unsigned to = lds_address(lds);
     const int lane = threadIdx.x & 63;
@@ -95,7 +96,7 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
             copy16_to_lds(call < BM / 64 ? lxs : lws, (unsigned)so[q],
                           to + S * R * 64 + lc * (R * 16) + call * 1024);
         }
-        lxs += M * 16, lws += N * 16, lc ^= 1;
+        lxs += M * 16, lws += N * 16, lc = lc == S - 1 ? 0 : lc + 1;
     };
     auto send_codes = [&](int buf, int q) {       // one copy of XQ + WQ
         if (q < XQ)
@@ -182,7 +183,7 @@ void tiles_kernel(const uint8_t* __restrict__ xc, const uint8_t* __restrict__ xs
                 #pragma unroll
                 for (int i = 0; i < FM; ++i)
                     xb[i] = *reinterpret_cast<const int*>(s + xsp + i * 256);
-                sbuf ^= 1;
+                sbuf = sbuf == S - 1 ? 0 : sbuf + 1;
             } else {                              // the next byte of each
                 #pragma unroll
                 for (int j = 0; j < FN; ++j) wb[j] = (unsigned)wb[j] >> 8;
@@ -240,7 +241,7 @@ void launch_tiles(const uint8_t* xc, const uint8_t* xs, long M, long K,
 void tiles(const uint8_t* xc, const uint8_t* xs, long M, long K,
            const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
            int bias_dt, void* y, int dt, bool large, hipStream_t stream) {
-    // 256 units: one block of 147 KB of LDS each, or two of 73 KB
+    // 256 units: one block with all 160 KB of LDS each, or two
     #define MX4_L(OT) \
         launch_tiles<OT, 256, 256, 2, 4, 4>(xc, xs, M, K, wc, ws, N, bias, \
                                             bias_dt, y, 256, 4, stream)

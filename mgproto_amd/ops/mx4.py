@@ -171,7 +171,8 @@ class _MX4Linear(torch.autograd.Function):
             xc, xs = reference.mx4_quantize(_matrix(x))
             if weight is not None:
                 wc, ws = reference.mx4_quantize(weight)
-            y = reference.mx4_product(xc, xs, wc, ws, K, bias, x.dtype)
+            with torch.autocast(x.device.type, enabled=False):
+                y = reference.mx4_product(xc, xs, wc, ws, K, bias, x.dtype)
             y = y.view(*x.shape[:-1], wc.shape[1])
         elif need_w:    # the rounded rows are kept, a quarter of x in bf16
             y, xc, xs, wc, ws = ext.mx4_linear_train(x, weight, bias)
@@ -190,9 +191,14 @@ class _MX4Linear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        backward = (reference.mx4_backward if _ext(g) is None
-                    else _ext(g).mx4_linear_backward)
-        dx, dw, db = backward(g, *ctx.saved_tensors, ctx.K, *ctx.types)
+        ext = _ext(g)
+        if ext is not None:
+            dx, dw, db = ext.mx4_linear_backward(g, *ctx.saved_tensors, ctx.K,
+                                                 *ctx.types)
+        else:
+            with torch.autocast(g.device.type, enabled=False):
+                dx, dw, db = reference.mx4_backward(g, *ctx.saved_tensors,
+                                                    ctx.K, *ctx.types)
         return dx, dw, None, None, db
 
 

@@ -8,7 +8,8 @@
   activating prototypes with their mixture prior, peak activation, latent
   location and receptive-field bounding box in input pixels,
 * optional hipGraph capture of the forward for fixed-batch low-latency
-  serving (same machinery as the training-step capture).
+  serving (same machinery as the training-step capture);
+* ``weights='mx4'``: the backbone's 1x1 convolutions as 4-bit products.
 
 ``create_app`` exposes it over FastAPI (POST /predict with an image file;
 GET /healthz, /model_info).
@@ -20,12 +21,19 @@ from typing import List, Optional
 import torch
 import torch.nn.functional as F
 
+from .models import use_mx4
 from .utils.receptive_field import compute_rf_prototype
 
 
 class InferenceEngine:
-    def __init__(self, model, device=None, amp: bool = True):
+    def __init__(self, model, device=None, amp: bool = True,
+                 weights: str = 'float'):
+        if weights not in ('float', 'mx4'):
+            raise ValueError(f"weights 'float' or 'mx4', not {weights!r}")
         self.model = model.eval()
+        self.weights = weights
+        if weights == 'mx4':
+            use_mx4(self.model.features)
         self.device = device or next(model.parameters()).device
         self.amp = amp and self.device.type == 'cuda'
         self._graph = None
@@ -152,6 +160,7 @@ def create_app(engine: InferenceEngine, class_names: Optional[List[str]] = None)
                 'num_prototypes': m.num_prototypes,
                 'prototypes_per_class': m.num_prototypes_per_class,
                 'img_size': m.img_size,
+                'weights': engine.weights,
                 'graph_captured': engine._graph is not None}
 
     @app.post('/predict')

@@ -109,6 +109,7 @@ class Settings:
     last_layer_optimizer_lr: float = last_layer_optimizer_lr
     coefs: Dict[str, float] = field(default_factory=lambda: dict(coefs))
     joint_lr_gamma: float = 0.4
+    clip_grad_norm: Optional[float] = None  # global gradient norm at most this
     joint_lr_decay_epochs: Optional[List[int]] = None  # None -> per-arch table
 
     # schedule
@@ -125,6 +126,7 @@ class Settings:
     em_stream: bool = True           # run the EM update on a side HIP stream
     hip_graph: bool = True           # capture the whole training step in a hipGraph
     grad_bucket_mb: int = 50         # RCCL all-reduce bucket size (xGMI-tuned)
+    mx4: bool = False                # 4-bit 1x1 convs in the backbone (train)
     native_ops: str = 'auto'         # 'auto' | 'force' | 'off' — HIP kernel dispatch
 
     def lr_decay_epochs(self) -> List[int]:

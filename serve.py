@@ -31,6 +31,8 @@ def main():
     ap.add_argument('--port', type=int, default=8000)
     ap.add_argument('--capture-batch', type=int, default=0,
                     help='hipGraph-capture the forward at this batch size')
+    ap.add_argument('--weights', choices=('float', 'mx4'), default='float',
+                    help='mx4: the backbone\'s 1x1 convolutions in 4 bits')
     args = ap.parse_args()
 
     device = torch.device('cuda', 0) if torch.cuda.is_available() \
@@ -58,7 +60,7 @@ def main():
     if device.type == 'cuda':
         model.features = model.features.to(memory_format=torch.channels_last)
 
-    engine = InferenceEngine(model, device)
+    engine = InferenceEngine(model, device, weights=args.weights)
     if args.capture_batch and device.type == 'cuda':
         engine.capture(args.capture_batch)
 

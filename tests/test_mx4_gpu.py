@@ -147,6 +147,24 @@ def test_every_form_at_every_size(M, K, N, form):
         assert torch.equal(y.cpu(), want.to(dtype))
 
 
+@pytest.mark.parametrize('form', [2, 5, 6])
+@pytest.mark.parametrize('K', [32, 200, 330, 520])
+def test_more_tiles_than_blocks(K, form):
+    # every block walks over several tiles, of 1, 2, 3 and 5 steps
+    M, N = 66000, 530
+    ext = ops._native_or_die()
+    x = GRID[torch.randint(0, 8, (M, K))].float().cuda()
+    w = GRID[torch.randint(0, 8, (N, K))].float().cuda()
+    x[torch.rand(M, K, device='cuda') < 0.3] *= -4
+    w[::3] *= -0.5
+    want = (ops.mx4_quantize(x).dequantize()
+            @ ops.mx4_quantize(w).dequantize().t())      # exact in fp32, too
+    wq = ops.mx4_quantize(w)
+    for _ in range(3):
+        y = ext.mx4_linear(x, wq.codes, wq.scales, K, None, form)
+        assert torch.equal(y, want)
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('M', [1, 40, 3000])
 def test_strides_and_alignments_of_rows(dtype, M):

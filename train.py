@@ -107,12 +107,22 @@ def main():
                              'chain (main.py:98-104) instead of the fused '
                              'one-homography approximation — pick this for '
                              'training-parity comparisons')
+    parser.add_argument('--clip-grad-norm', type=float, default=None,
+                        help='scale the gradients of a step to a global norm '
+                             'of at most this')
+    parser.add_argument('--mx4', action='store_true',
+                        help='train with the backbone\'s 1x1 convolutions '
+                             'rounded to 4 bits (straight-through gradients), '
+                             'for serve.py --weights mx4')
     args = parser.parse_args()
+    if args.clip_grad_norm is not None and not args.clip_grad_norm > 0:
+        parser.error('--clip-grad-norm takes a positive number')
 
     cfg = Settings(base_architecture=args.arch, aux_loss=args.aux_loss,
                    sz_embedding=args.aux_emb_sz, mem_capacity=args.mem_sz,
                    mine_K=args.mine_level,
-                   fast_augment=not args.faithful_aug)
+                   fast_augment=not args.faithful_aug,
+                   clip_grad_norm=args.clip_grad_norm, mx4=args.mx4)
     if args.addon:
         cfg.add_on_layers_type = args.addon
     if os.environ.get('MGPROTO_TINY_TEST') == '1':
@@ -186,6 +196,11 @@ def main():
     if device.type == 'cuda' and cfg.channels_last:
         ppnet.features = ppnet.features.to(memory_format=torch.channels_last)
 
+    if cfg.mx4:
+        from mgproto_amd.models import use_mx4
+        n = use_mx4(ppnet.features, train=True)
+        log(f'4-bit 1x1 convolutions: {n}')
+
     aux_criterion = build_aux_loss(args.aux_loss, nb_classes=cfg.num_classes,
                                    sz_embed=args.aux_emb_sz, mrg=0.1,
                                    beta=32).to(device)
@@ -225,7 +240,8 @@ def main():
         graph_step = GraphedStep(ppnet, aux_criterion, cfg.coefs, device,
                                  cfg.train_batch_size, cfg.img_size,
                                  amp_dtype=cfg.amp_dtype,
-                                 channels_last=cfg.channels_last)
+                                 channels_last=cfg.channels_last,
+                                 clip_grad_norm=cfg.clip_grad_norm)
         log('hipGraph training step: enabled')
 
     reducer = None
@@ -313,7 +329,7 @@ def main():
             ppnet, train_loader, optimizer, aux_criterion=aux_criterion,
             use_mine=use_mining, update_GMM=update_GMM, coefs=cfg.coefs,
             log=log, em_runner=em_runner, reducer=reducer,
-            graph_step=graph_step, **kw)
+            graph_step=graph_step, clip_grad_norm=cfg.clip_grad_norm, **kw)
 
         if args.ood_eval:
             accu, _ = tnt.test(ppnet, (test_loader, ood1_loader, ood2_loader),
