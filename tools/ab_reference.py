@@ -33,6 +33,9 @@ _REF = None
 
 def load_reference(path='/root/reference'):
     """Import the reference's model + losses modules with import stubs."""
+    if not os.path.isfile(os.path.join(path, 'model.py')):
+        import unittest
+        raise unittest.SkipTest(f'no reference checkout in {path}')
     global _REF
     if _REF is not None:
         return _REF
