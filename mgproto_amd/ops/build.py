@@ -21,6 +21,8 @@ SRC = [os.path.join(_HERE, 'hip', 'mgproto_kernels.hip'),
        os.path.join(_HERE, 'hip', 'mx4_tiles.hip'),
        os.path.join(_HERE, 'hip', 'mx4_rounding.hip'),
        os.path.join(_HERE, 'hip', 'mx4_grad.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_grad_input.hip'),
+       os.path.join(_HERE, 'hip', 'mx4_grad_weight.hip'),
        os.path.join(_HERE, 'hip', 'grad_clip.hip'),
        os.path.join(_HERE, 'hip', 'mx4_bindings.hip')]
 # no packed fp32 instructions: some of their forms give wrong results on this

@@ -243,61 +243,53 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_train(
 std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
         const Tensor& grad, const OptTensor& wc, const OptTensor& ws,
         const OptTensor& xc, const OptTensor& xs, int64_t K, int64_t dx_dt,
-        int64_t dw_dt, int64_t db_dt) {
+        int64_t dw_dt, int64_t db_dt, int64_t form) {
     CHECK_VALUE(grad.is_cuda() && grad.dim() >= 1,
                 "mx4_linear: output gradient: rows on the GPU");
-    const int gd = dtype_code(grad, "mx4_linear: output gradient");
-    const int64_t N = grad.size(-1);
-    int64_t M = 1;
-    for (int64_t i = 0; i + 1 < grad.dim(); ++i) M *= grad.size(i);
-    CHECK_VALUE(M < (1L << 23) && N < (1L << 22),
+    CHECK_VALUE(form >= -1 && form <= 1, "mx4_linear: no form ", form);
+    mx4::GradArgs a{};
+    a.g_dt = dtype_code(grad, "mx4_linear: output gradient");
+    a.N = grad.size(-1), a.M = 1, a.K = K;
+    for (int64_t i = 0; i + 1 < grad.dim(); ++i) a.M *= grad.size(i);
+    CHECK_VALUE(a.M < (1L << 31) && a.N < (1L << 22),
                 "mx4_linear: output gradient: too large");
-    c10::DeviceGuard guard(grad.device());
-    const Tensor g = grad.contiguous();
-    const bool aligned = (uintptr_t)g.data_ptr() % 16 == 0;
-    const hipStream_t stream = current_stream();
-    OptTensor dx, dw, db;
-    auto make = [&](std::vector<int64_t> shape, int64_t dt) {
-        return at::empty(shape, g.options().dtype(scalar_type(dt)));
-    };
     if (dx_dt >= 0) {
         check_packed(*wc, *ws, K, "mx4_linear: weight");
-        CHECK_VALUE(wc->size(1) == N && g.device() == wc->device(),
+        CHECK_VALUE(wc->size(1) == a.N && grad.device() == wc->device(),
                     "mx4_linear: output gradient does not match the weight");
-        dx = make(shape_of(grad, K), dx_dt);
-        if (M && K && !N) {
-            dx->zero_();
-        } else if (M && K) {
-            auto work = workspace(mx4::grad_input_bytes(M, N, K, gd, aligned), g);
-            mx4::grad_input(g.data_ptr(), gd, aligned, M, N, K,
-                            wc->data_ptr<uint8_t>(), ws->data_ptr<uint8_t>(),
-                            dx->data_ptr(), (int)dx_dt, work.data_ptr(), stream);
-        }
+        a.wc = wc->data_ptr<uint8_t>(), a.ws = ws->data_ptr<uint8_t>();
     }
     if (dw_dt >= 0) {
         check_packed(*xc, *xs, K, "mx4_linear: input");
-        CHECK_VALUE(xc->size(1) == M && g.device() == xc->device(),
+        CHECK_VALUE(xc->size(1) == a.M && grad.device() == xc->device(),
                     "mx4_linear: output gradient does not match the input");
-        dw = make({N, K}, dw_dt);
-        if (N && K && !M) {
-            dw->zero_();
-        } else if (N && K) {
-            auto work = workspace(mx4::grad_weight_bytes(M, N, K, gd), g);
-            mx4::grad_weight(g.data_ptr(), gd, M, N, K, xc->data_ptr<uint8_t>(),
-                             xs->data_ptr<uint8_t>(), dw->data_ptr(),
-                             (int)dw_dt, work.data_ptr(), stream);
-        }
+        a.xc = xc->data_ptr<uint8_t>(), a.xs = xs->data_ptr<uint8_t>();
     }
-    if (db_dt >= 0) {
-        db = make({N}, db_dt);
-        if (N && !M) {
-            db->zero_();
-        } else if (N) {
-            auto work = workspace(mx4::col_sum_bytes(M, N), g);
-            mx4::col_sum(g.data_ptr(), gd, M, N, db->data_ptr(), (int)db_dt,
-                         work.data_ptr(), stream);
-        }
-    }
+    c10::DeviceGuard guard(grad.device());
+    const Tensor g = grad.contiguous();
+    OptTensor dx, dw, db;
+    // a sum over nothing is 0
+    auto make = [&](std::vector<int64_t> shape, int64_t dt, int64_t over,
+                    OptTensor& t, void*& ptr, int& code) {
+        if (dt < 0) return;
+        t = at::empty(shape, g.options().dtype(scalar_type(dt)));
+        code = (int)dt;
+        if (!t->numel()) return;
+        if (over) ptr = t->data_ptr();
+        else t->zero_();
+    };
+    make(shape_of(grad, K), dx_dt, a.N, dx, a.dx, a.dx_dt);
+    make({a.N, K}, dw_dt, a.M, dw, a.dw, a.dw_dt);
+    make({a.N}, db_dt, a.M, db, a.db, a.db_dt);
+    if (!a.dx && !a.dw && !a.db) return {dx, dw, db};
+    a.K = std::max<int64_t>(K, 1);        // only db is left where K is 0
+    a.g = g.data_ptr();
+    a.aligned = (uintptr_t)a.g % 16 == 0;
+    Tensor work;
+    if (const size_t bytes = mx4::grads_bytes(a, (int)form))
+        work = workspace(bytes, g);
+    mx4::grads(a, (int)form, work.defined() ? work.data_ptr() : nullptr,
+               current_stream());
     return {dx, dw, db};
 }
 
@@ -437,7 +429,10 @@ void register_mx4(pybind11::module& m) {
     m.def("mx4_linear_train", &linear_train,
           "Q(x) Q(w)^T + bias, and the rounded x and w");
     m.def("mx4_linear_backward", &linear_backward,
-          "gradients to the input, the weight and the bias");
+          "gradients to the input, the weight and the bias", py::arg("grad"),
+          py::arg("codes"), py::arg("scales"), py::arg("xcodes"),
+          py::arg("xscales"), py::arg("K"), py::arg("dx_dtype"),
+          py::arg("dw_dtype"), py::arg("db_dtype"), py::arg("form") = -1);
     m.def("grad_norm", &grad_norm, "global norm of a list of tensors");
     m.def("clip_grads", &clip_grads,
           "a list scaled to a global norm of at most max_norm; returns the norm");

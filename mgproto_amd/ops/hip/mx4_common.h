@@ -207,20 +207,20 @@ void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
               int bias_dt, void* y, int dt, int form, hipStream_t stream);
 
-// dx[M,K] = g[M,N] W[N,K] and dw[N,K] = g[M,N]^T X[M,K]; each states the
-// bytes of workspace that it wants
-size_t grad_input_bytes(long M, long N, long K, int g_dt, bool g_aligned);
-void grad_input(const void* g, int g_dt, bool g_aligned, long M, long N,
-                long K, const uint8_t* wc, const uint8_t* ws, void* dx,
-                int dx_dt, void* work, hipStream_t stream);
-size_t grad_weight_bytes(long M, long N, long K, int g_dt);
-void grad_weight(const void* g, int g_dt, long M, long N, long K,
-                 const uint8_t* xc, const uint8_t* xs, void* dw, int dw_dt,
-                 void* work, hipStream_t stream);
-
-// out[n] = sum_m g[m,n]
-size_t col_sum_bytes(long M, long N);
-void col_sum(const void* g, int g_dt, long M, long N, void* out, int out_dt,
-             void* work, hipStream_t stream);
+// The gradients that are wanted of the product: dx[M,K] = g[M,N] W[N,K],
+// dw[N,K] = g^T X[M,K], db[N] = sum_m g; none of M, N, K is 0. `aligned`: g starts
+// on 16 bytes. Form 0 is the one of small products, 1 that of large ones, -1
+// chooses.
+struct GradArgs {
+    const void* g;
+    int g_dt;
+    bool aligned;
+    long M, N, K;
+    const uint8_t *wc, *ws, *xc, *xs;
+    void *dx, *dw, *db;                  // null where not wanted
+    int dx_dt, dw_dt, db_dt;
+};
+size_t grads_bytes(const GradArgs& a, int form);      // of workspace
+void grads(const GradArgs& a, int form, void* work, hipStream_t stream);
 
 }  // namespace mx4

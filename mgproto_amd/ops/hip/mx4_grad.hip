@@ -2,415 +2,434 @@
 //   dx[M,K] = g[M,N] W[N,K],   dw[N,K] = g[M,N]^T X[M,K],   db[n] = sum_m g.
 //
 // Every MX4 value is exact in bf16, so the held operand is read as bf16 and
-// both products run on v_mfma_f32_16x16x32_bf16 with fp32 sums. g is taken
-// whole: a wider type is cut into bf16 parts by truncation (two for fp16's 11
-// bits, three for fp32's 24), whose sum is g exactly, and the parts' products
-// are added in the same sums.
+// both products run on bf16 matrix instructions with fp32 sums
+// (mx4_grad_input.hip, mx4_grad_weight.hip). g is taken whole: a wider type is
+// cut into bf16 parts by truncation (two for fp16's 11 bits, three for fp32's
+// 24), whose sum is g exactly, and the parts' products are added in the same
+// sums. Small products, where every launch counts, take one kernel of plain
+// fp32 arithmetic instead.
 
 #include <hip/hip_runtime.h>
 
-#include "mx4_common.h"
-#include "mx4_linear.h"
+#include <algorithm>
+
+#include "mx4_grad.h"
 
 namespace mx4 {
 namespace {
 
-constexpr int BT = 128, BK = 64;      // tile of the output, step of the sum
-
 int parts_of(int dt) { return dt == BF16 ? 1 : dt == F16 ? 2 : 3; }
-long up64(long v) { return (v + 63) / 64 * 64; }
-size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // part p of v: eight bits of its significand each time
-static __device__ __forceinline__ unsigned short part_of(float v, int p) {
+static __device__ __forceinline__ unsigned part_of(float v, int p) {
     unsigned b = __float_as_uint(v);
     if ((b & 0x7f800000u) == 0x7f800000u) {       // infinity or NaN: whole in
         if (p) return 0;                          // the first part
-        return (unsigned short)((b >> 16) | ((b & 0x7fffffu) ? 0x40u : 0u));
+        return (b >> 16) | ((b & 0x7fffffu) ? 0x40u : 0u);
     }
     for (int i = 0; i < p; ++i) {
         v -= __uint_as_float(b & 0xffff0000u);    // exact
         b = __float_as_uint(v);
     }
-    return (unsigned short)(b >> 16);
+    return b >> 16;
 }
 
 // ---------------------------------------------------------------------------
-// operands laid out for the product: rows along the summed axis, zeros up to
-// a multiple of 64
+// operands laid out for the tiles
 // ---------------------------------------------------------------------------
 
-// g [R, C] -> out [P][R][Cp]
-template <int DT>
+// g [M, N] -> parts of it, 8 elements a thread: STEPPED [P][Np/32][M][32], else
+// [P][M][Np]; zeros behind column N
+template <int DT, bool STEPPED>
 __global__ __launch_bounds__(256)
-void parts_kernel(const typename Elem<DT>::T* __restrict__ g, long R, long C,
-                  long Cp, int P, unsigned short* __restrict__ out) {
-    const long total = R * Cp, step = (long)gridDim.x * 256;
+void parts_kernel(const typename Elem<DT>::T* __restrict__ g, long M, int N,
+                  int Np, int P, u32x4* __restrict__ out) {
+    const int upr = Np / 8;
+    const long total = M * upr, step = (long)gridDim.x * 256;
     for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
-        const long r = t / Cp, c = t - r * Cp;
-        const float v = c < C ? (float)g[r * C + c] : 0.f;
-        for (int p = 0; p < P; ++p) out[p * total + t] = part_of(v, p);
+        const long m = t / upr;
+        const int u = (int)(t - m * upr), n = u * 8;
+        float v[8];
+        #pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = n + i < N ? (float)g[m * N + n + i] : 0.f;
+        const long at = STEPPED ? ((long)(u >> 2) * M + m) * 4 + (u & 3) : t;
+        for (int p = 0; p < P; ++p) {
+            u32x4 o;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[i] = part_of(v[2 * i], p) | part_of(v[2 * i + 1], p) << 16;
+            out[p * total + at] = o;
+        }
     }
 }
 
-// g [R, C] -> out [P][C][Rp]
-template <int DT>
-__global__ __launch_bounds__(256)
-void parts_t_kernel(const typename Elem<DT>::T* __restrict__ g, long R, long C,
-                    long Rp, int P, unsigned short* __restrict__ out) {
-    __shared__ float tile[64][65];
-    const long r0 = (long)blockIdx.x * 64, c0 = (long)blockIdx.y * 64;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    for (int i = ty; i < 64; i += 4) {
-        const long r = r0 + i, c = c0 + tx;
-        tile[i][tx] = r < R && c < C ? (float)g[r * C + c] : 0.f;
-    }
-    __syncthreads();
-    for (int i = ty; i < 64; i += 4) {
-        const long c = c0 + i;
-        if (c >= C) break;
-        for (int p = 0; p < P; ++p)
-            out[((long)p * C + c) * Rp + r0 + tx] = part_of(tile[tx][i], p);
-    }
-}
-
-// 4-bit rows [R, K] -> out [K][Rp]
+// 4-bit rows [R, K] -> [ceil(R/32)][K][32] bf16, zeros behind row R
 __global__ __launch_bounds__(256)
 void values_t_kernel(const uint8_t* __restrict__ codes,
                      const uint8_t* __restrict__ scales, long R, long K,
-                     long Rp, __bf16* __restrict__ out) {
-    __shared__ float tile[64][65];
-    const long r0 = (long)blockIdx.x * 64, k0 = (long)blockIdx.y * 64;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    {   // 8 codes a thread, 32 rows at a time
-        const int u = threadIdx.x & 7, rr = threadIdx.x >> 3;
-        const int k = (int)k0 + u * 8;
-        for (int i = rr; i < 64; i += 32) {
-            const long r = r0 + i;
-            unsigned c = 0, byte = 0;
-            if (r < R) {                       // 64 divides a step
-                c = reinterpret_cast<const unsigned*>(codes)[
-                    ((size_t)(k >> 7) * R + r) * 16 + (k >> 3 & 15)];
-                byte = scales[scale_at(R, r, k >> 5)];
-            }
-            float f[8];
-            values8(c, byte, f);
-            #pragma unroll
-            for (int e = 0; e < 8; ++e) tile[i][u * 8 + e] = f[e];
+                     __bf16* __restrict__ out) {
+    __shared__ float tile[32][129];
+    const long r0 = (long)blockIdx.x * 32, k0 = (long)blockIdx.y * 128;
+    #pragma unroll
+    for (int q = 0; q < 2; ++q) {       // 32 rows of 16 words
+        const int w = q * 256 + threadIdx.x, i = w >> 4, u = w & 15;
+        const long r = r0 + i;
+        unsigned c = 0, byte = 0;
+        if (r < R) {
+            c = reinterpret_cast<const unsigned*>(codes)[
+                ((size_t)blockIdx.y * R + r) * 16 + u];
+            byte = scales[scale_at(R, r, (int)(k0 >> 5) + (u >> 2))];
         }
+        float f[8];
+        values8(c, byte, f);
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) tile[i][u * 8 + e] = f[e];
     }
     __syncthreads();
-    for (int i = ty; i < 64; i += 4) {
-        const long k = k0 + i;
-        if (k >= K) break;
-        out[k * Rp + r0 + tx] = (__bf16)tile[tx][i];
+    #pragma unroll
+    for (int q = 0; q < 2; ++q) {       // 128 columns of 4 pieces of 8
+        const int w = q * 256 + threadIdx.x, k = w >> 2, p = w & 3;
+        if (k0 + k >= K) break;
+        u32x4 o;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __bf16 lo = (__bf16)tile[p * 8 + 2 * i][k];
+            const __bf16 hi = (__bf16)tile[p * 8 + 2 * i + 1][k];
+            o[i] = __builtin_bit_cast(unsigned short, lo)
+                | (unsigned)__builtin_bit_cast(unsigned short, hi) << 16;
+        }
+        reinterpret_cast<u32x4*>(out)[((long)blockIdx.x * K + k0 + k) * 4 + p] = o;
     }
 }
 
 // ---------------------------------------------------------------------------
-// C[M,N] = sum_p A_p[M,Kc] B[N,Kc]^T, rows of multiples of 64 elements
+// sums of partial results
 // ---------------------------------------------------------------------------
 
-// Grid (row tiles, column tiles, splits). A split sums its share of the
-// steps of all parts; with more than one split C is fp32 [splits][M][N].
-// LDS rows are 128 bytes; 16-byte piece c of row r lies at c ^ key(r), so
-// that the 16 rows which a read takes at once fall on different banks.
-static __device__ __forceinline__ int a_key(int r) { return (r ^ (r >> 3 & 1)) & 7; }
-static __device__ __forceinline__ int b_key(int r) {      // runs of 4, 16 apart
-    return ((r & 3) | (r >> 4 & 1) << 2) ^ (r >> 5 & 1);
-}
-
-template <int OT>
-__global__ __launch_bounds__(256)
-void product_nt_kernel(const unsigned short* __restrict__ A, long lda,
-                       long part_stride, int P,
-                       const unsigned short* __restrict__ B, long ldb,
-                       long M, long N, long Kc,
-                       typename Elem<OT>::T* __restrict__ C) {
-    using T = typename Elem<OT>::T;
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2][2][BT * BK];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r16 = lane & 15, g = lane >> 4;
-    const long m0 = (long)blockIdx.x * BT, n0 = (long)blockIdx.y * BT;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    const long per = Kc / BK, steps = per * P;
-    const long s_lo = steps * blockIdx.z / gridDim.z;
-    const long s_hi = steps * (blockIdx.z + 1) / gridDim.z;
-    const int lasta = (int)min((long)BT, M - m0) - 1;
-    const int lastb = (int)min((long)BT, N - n0) - 1;
-
-    // offsets in a tile stay below 2^31: rows are at most 2^22 elements here,
-    // 2^31 / 256 along M (checked by the caller)
-    auto stage = [&](long s, int buf) {
-        const long p = s / per, k0 = (s - p * per) * BK;
-        const unsigned short* a = A + p * part_stride + m0 * lda + k0;
-        const unsigned short* b = B + n0 * ldb + k0;
-        #pragma unroll
-        for (int q = 0; q < 4; ++q) {          // 1 KB: 8 rows a wave's call
-            const int call = wave * 4 + q;
-            const int r = call * 8 + (lane >> 3), c = lane & 7;
-            copy16_to_lds(a, (unsigned)(min(r, lasta) * lda * 2) + (c ^ a_key(r)) * 16,
-                          lds_address(&lds[buf][0][call * 512]));
-            copy16_to_lds(b, (unsigned)(min(r, lastb) * ldb * 2) + (c ^ b_key(r)) * 16,
-                          lds_address(&lds[buf][1][call * 512]));
-        }
-    };
-
-    f32x4 acc[4][4];
-    #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
-
-    if (s_lo < s_hi) stage(s_lo, 0);
-    int buf = 0;
-    for (long s = s_lo; s < s_hi; ++s, buf ^= 1) {
-        // the pieces of this step have to be there, and every wave has to be
-        // done with the other buffer before it is filled again
-        wait_copies<0>();
-        __syncthreads();
-        if (s + 1 < s_hi) stage(s + 1, buf ^ 1);
-        #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            bf16x8 a[4], b[4];
-            const int c = kk * 4 + g;
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = wm + i * 16 + r16;
-                a[i] = *reinterpret_cast<const bf16x8*>(
-                    &lds[buf][0][r * BK + (c ^ a_key(r)) * 8]);
-            }
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = wn + (r16 >> 2) * 16 + j * 4 + (r16 & 3);
-                b[j] = *reinterpret_cast<const bf16x8*>(
-                    &lds[buf][1][r * BK + (c ^ b_key(r)) * 8]);
-            }
-            #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        b[j], a[i], acc[i][j], 0, 0, 0);
-        }
-    }
-
-    // a lane holds 16 consecutive columns of each of its 4 rows
-    T* out = C + (gridDim.z > 1 ? (long)blockIdx.z * M * N : 0);
-    const bool vec = N % 4 == 0;
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long m = m0 + wm + i * 16 + r16;
-        if (m >= M) continue;
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long n = n0 + wn + g * 16 + j * 4;
-            if (n >= N) continue;
-            T* q = out + m * N + n;
-            union { T v[4]; u32x2 u[sizeof(T) / 2]; } o;
-            #pragma unroll
-            for (int r = 0; r < 4; ++r) o.v[r] = from_f32<OT>(acc[i][j][r]);
-            if (vec) {
-                #pragma unroll
-                for (int r = 0; r < (int)sizeof(T) / 2; ++r)
-                    reinterpret_cast<u32x2*>(q)[r] = o.u[r];
-            } else {
-                #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < N) q[r] = o.v[r];
-            }
-        }
-    }
-}
-
-// out[i] = sum of the splits, in their order
+// 64 results a block; its four waves sum a quarter of the parts each
 template <int OT>
 __global__ __launch_bounds__(256)
 void join_kernel(const float* __restrict__ part, int S, long n,
                  typename Elem<OT>::T* __restrict__ out) {
-    const long step = (long)gridDim.x * 256;
-    for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < n; t += step) {
-        float v = 0.f;
-        for (int s = 0; s < S; ++s) v += part[s * n + t];
-        out[t] = from_f32<OT>(v);
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+    const long i = (long)blockIdx.x * 64 + lane;
+    const int lo = S * q / 4, hi = S * (q + 1) / 4;
+    float v = 0.f;
+    if (i < n) {
+        #pragma unroll 8
+        for (int s = lo; s < hi; ++s) v += part[s * n + i];
+    }
+    red[q][lane] = v;
+    __syncthreads();
+    if (q == 0 && i < n)
+        out[i] = from_f32<OT>((red[0][lane] + red[1][lane])
+                              + (red[2][lane] + red[3][lane]));
+}
+
+// Sums over rows: W lanes side by side take 8 columns each, 256 / W rows at a
+// time; part[chunk][n]
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256)
+void col_sum_kernel(const typename Elem<DT>::T* __restrict__ g, long M, int N,
+                    int W, long rows, float* __restrict__ part) {
+    constexpr int E = DT == F32 ? 2 : 1;
+    __shared__ float red[256][9];
+    const int x = threadIdx.x & (W - 1), y = threadIdx.x / W, Y = 256 / W;
+    const long n = ((long)blockIdx.x * W + x) * 8;
+    const long lo = blockIdx.y * rows, hi = min(lo + rows, M);
+    float v[8] = {};
+    if (n < N) {
+        #pragma unroll 4
+        for (long m = lo + y; m < hi; m += Y) {
+            u32x4 u[E];
+            const typename Elem<DT>::T* p = g + m * N + n;
+            if (VEC && n + 8 <= N) {
+                #pragma unroll
+                for (int e = 0; e < E; ++e)
+                    u[e] = reinterpret_cast<const u32x4*>(p)[e];
+            } else {
+                load8_tail<DT>(p, (int)min((long)8, N - n), u);
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (DT == F32) {
+                    v[i] += __uint_as_float(u[0][i]);
+                    v[4 + i] += __uint_as_float(u[1][i]);
+                } else {
+                    const unsigned w = u[0][i];
+                    v[2 * i] += DT == BF16 ? __uint_as_float(w << 16)
+                                           : (float)as_f16x2(w).x;
+                    v[2 * i + 1] += DT == BF16 ? __uint_as_float(w & 0xffff0000u)
+                                               : (float)as_f16x2(w).y;
+                }
+            }
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) red[threadIdx.x][i] = v[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < W * 8; i += 256) {
+        const long c = (long)blockIdx.x * W * 8 + i;
+        if (c >= N) break;
+        float s = 0.f;
+        for (int k = 0; k < Y; ++k) s += red[k * W + (i >> 3)][i & 7];
+        part[blockIdx.y * (long)N + c] = s;
     }
 }
 
-unsigned grid_for(long total) {
-    const long blocks = (total + 255) / 256;
-    return (unsigned)(blocks < 256 * 32 ? blocks : 256 * 32);
+struct Sums { int W, chunks; long rows; unsigned gx; };
+Sums sums(long M, long N) {
+    Sums s;
+    s.W = 1;
+    while (s.W < 256 && s.W * 8 < N) s.W *= 2;
+    s.gx = (unsigned)((N + s.W * 8 - 1) / (s.W * 8));
+    // enough blocks for the card, at least 16 rows a lane
+    const long least = 256 / s.W * 16, most = std::max<long>(1, 1024 / s.gx);
+    s.rows = std::max(least, (M + most - 1) / most);
+    s.chunks = (int)((M + s.rows - 1) / s.rows);
+    return s;
 }
 
-// Splits of the sum: enough blocks for two on each of 256 units, each split
-// at least 4 steps long.
-int splits_for(long M, long N, long steps) {
-    const long tiles = ((M + BT - 1) / BT) * ((N + BT - 1) / BT);
-    long s = (512 + tiles - 1) / tiles;
-    if (s > steps / 4) s = steps / 4;
-    if (s > 64) s = 64;
-    return s < 1 ? 1 : (int)s;
+// ---------------------------------------------------------------------------
+// small products
+// ---------------------------------------------------------------------------
+
+struct Small {
+    const void* g;
+    long M, N, K;
+    int g_dt;
+    const uint8_t *wc, *ws, *xc, *xs;    // of the results that are wanted
+    void *dx, *dw, *db;
+    int dx_dt, dw_dt, db_dt;
+    int dx_blocks, dw_blocks, kb;        // kb: blocks along K
+};
+
+static __device__ __forceinline__ float load_g(const Small& a, long i) {
+    if (a.g_dt == F32) return reinterpret_cast<const float*>(a.g)[i];
+    if (a.g_dt == BF16) return (float)reinterpret_cast<const __bf16*>(a.g)[i];
+    return (float)reinterpret_cast<const _Float16*>(a.g)[i];
+}
+static __device__ __forceinline__ void store_any(void* p, int dt, long i, float v) {
+    if (dt == F32) reinterpret_cast<float*>(p)[i] = v;
+    else if (dt == BF16) reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
+    else reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 
-size_t split_bytes(long M, long N, long steps) {
-    const int S = splits_for(M, N, steps);
-    return S > 1 ? up256((size_t)S * M * N * 4) : 0;
+// out[a, k] = sum_b g(a, b) V[b, k] for 4 values of a and 64 of k a block: 8
+// lanes take 8 columns each, the 32 groups of them every 32nd b, joined in
+// order. g(a, b) lies at a * ga + b * gb.
+constexpr int SA = 4;
+static __device__ void small_product(const Small& p, long A, long B, long ga,
+                                     long gb, const uint8_t* codes,
+                                     const uint8_t* scales, void* out, int dt,
+                                     int block) {
+    __shared__ float red[32][SA][65];
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
+    const long a0 = (long)(block / p.kb) * SA, k = (long)(block % p.kb) * 64 + x * 8;
+    float v[SA][8] = {};
+    if (k < p.K) {
+        #pragma unroll 4
+        for (long b = y; b < B; b += 32) {
+            const unsigned c = reinterpret_cast<const unsigned*>(codes)[
+                ((size_t)(k >> 7) * B + b) * 16 + (k >> 3 & 15)];
+            const unsigned byte = scales[scale_at(B, b, (int)(k >> 5))];
+            float gv[SA], f[8];
+            #pragma unroll
+            for (int i = 0; i < SA; ++i)
+                gv[i] = load_g(p, min(a0 + i, A - 1) * ga + b * gb);
+            values8(c, byte, f);
+            #pragma unroll
+            for (int i = 0; i < SA; ++i)
+                #pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[i][e] = __builtin_fmaf(gv[i], f[e], v[i][e]);
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < SA; ++i)
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) red[y][i][x * 8 + e] = v[i][e];
+    __syncthreads();
+    const int i = threadIdx.x >> 6, e = threadIdx.x & 63;
+    const long a = a0 + i, kk = (long)(block % p.kb) * 64 + e;
+    if (a >= A || kk >= p.K) return;
+    float s = 0.f;
+    #pragma unroll
+    for (int q = 0; q < 32; ++q) s += red[q][i][e];
+    store_any(out, dt, a * p.K + kk, s);
 }
 
-void product_nt(const unsigned short* A, long lda, long part_stride, int P,
-                const unsigned short* B, long ldb, long M, long N, long Kc,
-                void* out, int dt, float* part, hipStream_t stream) {
-    const int S = splits_for(M, N, Kc / BK * P);
-    const dim3 grid((unsigned)((M + BT - 1) / BT),
-                    (unsigned)((N + BT - 1) / BT), (unsigned)S);
-    #define MX4_P(DT, C) \
-        hipLaunchKernelGGL((product_nt_kernel<DT>), grid, dim3(256), 0, \
-                           stream, A, lda, part_stride, P, B, ldb, M, N, Kc, \
-                           (typename Elem<DT>::T*)(C))
-    if (S == 1) {
-        if (dt == F32) MX4_P(F32, out);
-        else if (dt == BF16) MX4_P(BF16, out);
-        else MX4_P(F16, out);
+__global__ __launch_bounds__(256)
+void small_grads_kernel(const Small p) {
+    int block = blockIdx.x;
+    if (block < p.dx_blocks) {
+        small_product(p, p.M, p.N, p.N, 1, p.wc, p.ws, p.dx, p.dx_dt, block);
         return;
     }
-    MX4_P(F32, part);
-    #undef MX4_P
-    const long n = M * N;
+    block -= p.dx_blocks;
+    if (block < p.dw_blocks) {
+        small_product(p, p.N, p.M, 1, p.N, p.xc, p.xs, p.dw, p.dw_dt, block);
+        return;
+    }
+    block -= p.dw_blocks;
+    // 64 columns, every fourth row a wave
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+    const long n = (long)block * 64 + lane;
+    float v = 0.f;
+    if (n < p.N) {
+        #pragma unroll 4
+        for (long m = q; m < p.M; m += 4) v += load_g(p, m * p.N + n);
+    }
+    red[q][lane] = v;
+    __syncthreads();
+    if (q == 0 && n < p.N)
+        store_any(p.db, p.db_dt, n, (red[0][lane] + red[1][lane])
+                                    + (red[2][lane] + red[3][lane]));
+}
+
+// ---------------------------------------------------------------------------
+
+unsigned grid_for(long total) {
+    return (unsigned)std::min<long>((total + 255) / 256, 256 * 32);
+}
+
+bool dx_in_place(const GradArgs& a) {
+    return a.g_dt == BF16 && a.aligned && a.N % 32 == 0;
+}
+bool dw_in_place(const GradArgs& a) {
+    return a.g_dt == BF16 && a.aligned && a.N % 8 == 0;
+}
+
+// One launch against five to nine of 4 us: the plain arithmetic keeps up to
+// 2^24 multiplications (83x200x65 fp32: 13 us of backward against 42; 2^25, as
+// 3136x128x64, 28 against 31).
+bool small(const GradArgs& a) {
+    return (double)a.M * a.N * a.K <= 0x1p24 && std::max(a.M, a.N) <= 4096;
+}
+
+template <bool STEPPED>
+void launch_parts(const GradArgs& a, int Np, void* out, hipStream_t stream) {
+    const long total = a.M * (Np / 8);
+    #define MX4_G(DT) \
+        hipLaunchKernelGGL((parts_kernel<DT, STEPPED>), dim3(grid_for(total)), \
+                           dim3(256), 0, stream, \
+                           (const typename Elem<DT>::T*)a.g, a.M, (int)a.N, Np, \
+                           parts_of(a.g_dt), (u32x4*)out)
+    if (a.g_dt == F32) MX4_G(F32);
+    else if (a.g_dt == BF16) MX4_G(BF16);
+    else MX4_G(F16);
+    #undef MX4_G
+}
+
+size_t dx_bytes(const GradArgs& a) {
+    const long Np = up32(a.N);
+    const int P = parts_of(a.g_dt);
+    return up256((size_t)a.K * Np * 2)
+        + (dx_in_place(a) ? 0 : up256((size_t)P * a.M * Np * 2))
+        + grad_input_partial(a.M, a.K, Np / 32 * P);
+}
+
+size_t dw_bytes(const GradArgs& a) {
+    const int P = parts_of(a.g_dt);
+    return (dw_in_place(a) ? 0 : up256((size_t)P * a.M * ((a.N + 7) / 8 * 8) * 2))
+        + grad_weight_partial(a.M, a.N, a.K, P);
+}
+
+size_t db_bytes(const GradArgs& a) {
+    return up256((size_t)sums(a.M, a.N).chunks * a.N * 4);
+}
+
+// W^T is written once as bf16 (W is small beside g, or the product large)
+void run_dx(const GradArgs& a, char* at, hipStream_t stream) {
+    const long Np = up32(a.N);
+    const int P = parts_of(a.g_dt);
+    __bf16* wt = (__bf16*)at;
+    at += up256((size_t)a.K * Np * 2);
+    hipLaunchKernelGGL(values_t_kernel,
+                       dim3((unsigned)(Np / 32), (unsigned)steps_of(a.K)),
+                       dim3(256), 0, stream, a.wc, a.ws, a.N, a.K, wt);
+    if (dx_in_place(a)) {
+        grad_input_tiles(a.g, 64, a.N * 2, 1, (int)(Np / 32), wt, a.M, a.K, a.dx,
+                         a.dx_dt, at, stream);
+        return;
+    }
+    char* parts = at;
+    at += up256((size_t)P * a.M * Np * 2);
+    launch_parts<true>(a, (int)Np, parts, stream);
+    grad_input_tiles(parts, (size_t)a.M * 64, 64, P, (int)(Np / 32), wt, a.M, a.K,
+                     a.dx, a.dx_dt, at, stream);
+}
+
+void run_dw(const GradArgs& a, char* at, hipStream_t stream) {
+    const int P = parts_of(a.g_dt);
+    if (dw_in_place(a)) {
+        grad_weight_tiles(a.g, a.N, 0, 1, a.M, a.N, a.K, a.xc, a.xs, a.dw,
+                          a.dw_dt, at, stream);
+        return;
+    }
+    const long Np = (a.N + 7) / 8 * 8;
+    const size_t part = (size_t)a.M * Np * 2;
+    launch_parts<false>(a, (int)Np, at, stream);
+    grad_weight_tiles(at, Np, part, P, a.M, a.N, a.K, a.xc, a.xs, a.dw, a.dw_dt,
+                      at + up256(P * part), stream);
+}
+
+void run_db(const GradArgs& a, char* at, hipStream_t stream) {
+    const Sums s = sums(a.M, a.N);
+    const dim3 grid(s.gx, (unsigned)s.chunks);
+    const bool vec = a.aligned && a.N % 8 == 0;
+    #define MX4_S(DT, V) \
+        hipLaunchKernelGGL((col_sum_kernel<DT, V>), grid, dim3(256), 0, stream, \
+                           (const typename Elem<DT>::T*)a.g, a.M, (int)a.N, s.W, \
+                           s.rows, (float*)at)
+    #define MX4_V(DT) do { if (vec) MX4_S(DT, true); else MX4_S(DT, false); } while (0)
+    if (a.g_dt == F32) MX4_V(F32);
+    else if (a.g_dt == BF16) MX4_V(BF16);
+    else MX4_V(F16);
+    #undef MX4_V
+    #undef MX4_S
+    join((const float*)at, s.chunks, a.N, a.db, a.db_dt, stream);
+}
+
+}  // namespace
+
+void join(const float* part, int S, long n, void* out, int dt,
+          hipStream_t stream) {
+    const dim3 grid((unsigned)((n + 63) / 64));
     #define MX4_J(DT) \
-        hipLaunchKernelGGL((join_kernel<DT>), dim3(grid_for(n)), dim3(256), \
-                           0, stream, part, S, n, (typename Elem<DT>::T*)out)
+        hipLaunchKernelGGL((join_kernel<DT>), grid, dim3(256), 0, stream, part, \
+                           S, n, (typename Elem<DT>::T*)out)
     if (dt == F32) MX4_J(F32);
     else if (dt == BF16) MX4_J(BF16);
     else MX4_J(F16);
     #undef MX4_J
 }
 
-// ---------------------------------------------------------------------------
-// column sums
-// ---------------------------------------------------------------------------
-
-constexpr int SUM_ROWS = 512;
-
-template <int DT>
-__global__ __launch_bounds__(256)
-void col_sum_kernel(const typename Elem<DT>::T* __restrict__ g, long M, long N,
-                    float* __restrict__ part) {
-    __shared__ float red[4][64];
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const long n = (long)blockIdx.x * 64 + tx;
-    const long lo = (long)blockIdx.y * SUM_ROWS;
-    const long hi = min(lo + SUM_ROWS, M);
-    float v = 0.f;
-    if (n < N)
-        for (long m = lo + ty; m < hi; m += 4) v += (float)g[m * N + n];
-    red[ty][tx] = v;
-    __syncthreads();
-    if (ty == 0 && n < N)
-        part[blockIdx.y * N + n] =
-            (red[0][tx] + red[1][tx]) + (red[2][tx] + red[3][tx]);
+size_t grads_bytes(const GradArgs& a, int form) {
+    if (form < 0 ? small(a) : form == 0) return 0;
+    // one after the other on the stream: the same bytes serve all
+    return std::max({a.dx ? dx_bytes(a) : 0, a.dw ? dw_bytes(a) : 0,
+                     a.db ? db_bytes(a) : 0});
 }
 
-}  // namespace
-
-size_t col_sum_bytes(long M, long N) {
-    return up256((size_t)((M + SUM_ROWS - 1) / SUM_ROWS) * N * 4);
-}
-
-void col_sum(const void* g, int g_dt, long M, long N, void* out, int out_dt,
-             void* work, hipStream_t stream) {
-    const int S = (int)((M + SUM_ROWS - 1) / SUM_ROWS);
-    float* part = (float*)work;
-    const dim3 grid((unsigned)((N + 63) / 64), (unsigned)S);
-    #define MX4_S(DT) \
-        hipLaunchKernelGGL((col_sum_kernel<DT>), grid, dim3(256), 0, stream, \
-                           (const typename Elem<DT>::T*)g, M, N, part)
-    if (g_dt == F32) MX4_S(F32);
-    else if (g_dt == BF16) MX4_S(BF16);
-    else MX4_S(F16);
-    #undef MX4_S
-    #define MX4_J(DT) \
-        hipLaunchKernelGGL((join_kernel<DT>), dim3(grid_for(N)), dim3(256), \
-                           0, stream, part, S, N, (typename Elem<DT>::T*)out)
-    if (out_dt == F32) MX4_J(F32);
-    else if (out_dt == BF16) MX4_J(BF16);
-    else MX4_J(F16);
-    #undef MX4_J
-}
-
-// dx = g W: W^T is written once as [K][Np] bf16; g is read in place where its
-// rows allow it, and copied into padded bf16 parts elsewhere
-static bool in_place(long N, int g_dt, bool g_aligned) {
-    return g_dt == BF16 && g_aligned && N % 64 == 0;
-}
-
-size_t grad_input_bytes(long M, long N, long K, int g_dt, bool g_aligned) {
-    const long Np = up64(N);
-    const int P = parts_of(g_dt);
-    size_t b = up256((size_t)K * Np * 2);
-    if (!in_place(N, g_dt, g_aligned)) b += up256((size_t)P * M * Np * 2);
-    return b + split_bytes(M, K, Np / BK * P);
-}
-
-void grad_input(const void* g, int g_dt, bool g_aligned, long M, long N,
-                long K, const uint8_t* wc, const uint8_t* ws, void* dx,
-                int dx_dt, void* work, hipStream_t stream) {
-    const long Np = up64(N);
-    const int P = parts_of(g_dt);
-    char* at = (char*)work;
-    __bf16* wt = (__bf16*)at;
-    at += up256((size_t)K * Np * 2);
-    hipLaunchKernelGGL(values_t_kernel,
-                       dim3((unsigned)(Np / 64), (unsigned)((K + 63) / 64)),
-                       dim3(256), 0, stream, wc, ws, N, K, Np, wt);
-    const unsigned short* a = (const unsigned short*)g;
-    if (!in_place(N, g_dt, g_aligned)) {
-        unsigned short* parts = (unsigned short*)at;
-        at += up256((size_t)P * M * Np * 2);
-        #define MX4_G(DT) \
-            hipLaunchKernelGGL((parts_kernel<DT>), dim3(grid_for(M * Np)), \
-                               dim3(256), 0, stream, \
-                               (const typename Elem<DT>::T*)g, M, N, Np, P, parts)
-        if (g_dt == F32) MX4_G(F32);
-        else if (g_dt == BF16) MX4_G(BF16);
-        else MX4_G(F16);
-        #undef MX4_G
-        a = parts;
+void grads(const GradArgs& a, int form, void* work, hipStream_t stream) {
+    if (form < 0 ? small(a) : form == 0) {
+        Small p{a.g, a.M, a.N, a.K, a.g_dt, a.wc, a.ws, a.xc, a.xs, a.dx, a.dw,
+                a.db, a.dx_dt, a.dw_dt, a.db_dt, 0, 0, (int)((a.K + 63) / 64)};
+        p.dx_blocks = a.dx ? (int)((a.M + SA - 1) / SA) * p.kb : 0;
+        p.dw_blocks = a.dw ? (int)((a.N + SA - 1) / SA) * p.kb : 0;
+        const int db = a.db ? (int)((a.N + 63) / 64) : 0;
+        hipLaunchKernelGGL(small_grads_kernel,
+                           dim3((unsigned)(p.dx_blocks + p.dw_blocks + db)),
+                           dim3(256), 0, stream, p);
+        return;
     }
-    product_nt(a, Np, M * Np, P, (const unsigned short*)wt, Np, M, K, Np, dx,
-               dx_dt, (float*)at, stream);
-}
-
-// dw = g^T X: both turned so that rows lie along M
-size_t grad_weight_bytes(long M, long N, long K, int g_dt) {
-    const long Mp = up64(M);
-    const int P = parts_of(g_dt);
-    return up256((size_t)K * Mp * 2) + up256((size_t)P * N * Mp * 2) +
-           split_bytes(N, K, Mp / BK * P);
-}
-
-void grad_weight(const void* g, int g_dt, long M, long N, long K,
-                 const uint8_t* xc, const uint8_t* xs, void* dw, int dw_dt,
-                 void* work, hipStream_t stream) {
-    const long Mp = up64(M);
-    const int P = parts_of(g_dt);
-    char* at = (char*)work;
-    __bf16* xt = (__bf16*)at;
-    at += up256((size_t)K * Mp * 2);
-    unsigned short* gt = (unsigned short*)at;
-    at += up256((size_t)P * N * Mp * 2);
-    hipLaunchKernelGGL(values_t_kernel,
-                       dim3((unsigned)(Mp / 64), (unsigned)((K + 63) / 64)),
-                       dim3(256), 0, stream, xc, xs, M, K, Mp, xt);
-    const dim3 grid((unsigned)(Mp / 64), (unsigned)((N + 63) / 64));
-    #define MX4_G(DT) \
-        hipLaunchKernelGGL((parts_t_kernel<DT>), grid, dim3(256), 0, stream, \
-                           (const typename Elem<DT>::T*)g, M, N, Mp, P, gt)
-    if (g_dt == F32) MX4_G(F32);
-    else if (g_dt == BF16) MX4_G(BF16);
-    else MX4_G(F16);
-    #undef MX4_G
-    product_nt(gt, Mp, N * Mp, P, (const unsigned short*)xt, Mp, N, K, Mp, dw,
-               dw_dt, (float*)at, stream);
+    if (a.dx) run_dx(a, (char*)work, stream);
+    if (a.dw) run_dw(a, (char*)work, stream);
+    if (a.db) run_db(a, (char*)work, stream);
 }
 
 }  // namespace mx4

@@ -147,6 +147,72 @@ def test_every_form_at_every_size(M, K, N, form):
         assert torch.equal(y.cpu(), want.to(dtype))
 
 
+@pytest.mark.parametrize('form', [0, 1])
+@pytest.mark.parametrize('M,K,N', SIZES + [
+    (260, 1, 260), (129, 384, 70), (700, 1000, 520), (2500, 300, 260),
+    (5000, 64, 64), (3001, 128, 128), (4099, 30, 300), (1500, 513, 24),
+    (40, 600, 2000)])
+def test_every_gradient_form_at_every_size(M, K, N, form):
+    # whole numbers: sums of up to 5000 products of at most 4 x 6 are exact
+    ext = ops._native_or_die()
+    x = GRID[torch.randint(0, 8, (M, K))] * (torch.randint(0, 2, (M, K)) * 2 - 1)
+    w = GRID[torch.randint(0, 8, (N, K))] * (torch.randint(0, 2, (N, K)) * 2 - 1)
+    g = torch.randint(-4, 5, (M, N)).double()
+    xv, wv = values(x.float()), values(w.float())
+    dx, dw, db = g @ wv, g.t() @ xv, g.sum(0)
+    xq, wq = (ops.mx4_quantize(t.float().cuda()) for t in (x, w))
+    for code, dtype in enumerate(DTYPES):
+        base = torch.full((M * N + 3,), math.nan, dtype=dtype, device='cuda')
+        for lo in (0, 3):                  # on 16 bytes, and not
+            gd = base[lo:lo + M * N].view(M, N)
+            gd.copy_(g)
+            got = ext.mx4_linear_backward(
+                gd, wq.codes, wq.scales, xq.codes, xq.scales, K, code,
+                (code + 1) % 3, (code + 2) % 3, form)
+            for t, want, c in zip(got, (dx, dw, db),
+                                  (code, (code + 1) % 3, (code + 2) % 3)):
+                assert torch.equal(t.cpu(), want.to(DTYPES[c])), (dtype, lo, c)
+            base.fill_(math.nan)
+
+
+@pytest.mark.parametrize('form', [0, 1])
+def test_gradients_at_the_ends_of_the_scales(form):
+    # each value has to come out of bf16 as it is, subnormal ones too
+    ext = ops._native_or_die()
+    e = torch.arange(-127, 126, 4).double()
+    x = GRID.repeat(4)[None, :] * torch.exp2(e)[:, None]        # rows of 32
+    x[:, 0] = 6.0 * torch.exp2(e)
+    q = ops.mx4_quantize(x.float().cuda())
+    eye = torch.eye(len(e))
+    for g, want in ((eye, values(x.float())),):
+        _, dw, _ = ext.mx4_linear_backward(
+            g.cuda(), None, None, q.codes, q.scales, 32, -1, 0, -1, form)
+        assert torch.equal(dw.double().cpu(), want)
+        dx, _, _ = ext.mx4_linear_backward(
+            g.cuda(), q.codes, q.scales, None, None, 32, 0, -1, -1, form)
+        assert torch.equal(dx.double().cpu(), want)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('M,K,N', [(70, 130, 40), (3000, 200, 300)])
+def test_infinities_in_the_output_gradient(M, K, N, dtype):
+    # they reach the rows and columns that the formula gives them, as they are
+    x = GRID[torch.randint(1, 8, (M, K))].float().cuda()
+    w = GRID[torch.randint(1, 8, (N, K))].float().cuda()
+    g = torch.zeros(M, N)
+    g[M - 1, 5], g[2, N - 1], g[7, 7] = math.inf, -math.inf, math.nan
+    xd, wd = x.to(dtype).requires_grad_(), w.requires_grad_()
+    y = ops.mx4_linear(xd, wd)
+    dx, dw = torch.autograd.grad(y, (xd, wd), g.to(dtype).cuda())
+    want = torch.zeros(M, K)
+    want[M - 1], want[2], want[7] = math.inf, -math.inf, math.nan
+    assert torch.equal(dx.float().cpu().nan_to_num(1, 2, 3),
+                       want.nan_to_num(1, 2, 3))
+    want = torch.zeros(N, K)
+    want[5], want[N - 1], want[7] = math.inf, -math.inf, math.nan
+    assert torch.equal(dw.cpu().nan_to_num(1, 2, 3), want.nan_to_num(1, 2, 3))
+
+
 @pytest.mark.parametrize('form', [2, 5, 6])
 @pytest.mark.parametrize('K', [32, 200, 330, 520])
 def test_more_tiles_than_blocks(K, form):
