@@ -107,25 +107,46 @@ void values_t_kernel(const uint8_t* __restrict__ codes,
 // sums of partial results
 // ---------------------------------------------------------------------------
 
-// 64 results a block; its four waves sum a quarter of the parts each
+// 16 results a block; 16 groups of lanes sum a sixteenth of the parts each
 template <int OT>
 __global__ __launch_bounds__(256)
-void join_kernel(const float* __restrict__ part, int S, long n,
-                 typename Elem<OT>::T* __restrict__ out) {
-    __shared__ float red[4][64];
-    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
-    const long i = (long)blockIdx.x * 64 + lane;
-    const int lo = S * q / 4, hi = S * (q + 1) / 4;
+void join_few_kernel(const float* __restrict__ part, int S, long n,
+                     typename Elem<OT>::T* __restrict__ out) {
+    __shared__ float red[16][17];
+    const int x = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const long i = (long)blockIdx.x * 16 + x;
+    const int lo = S * q / 16, hi = S * (q + 1) / 16;
     float v = 0.f;
     if (i < n) {
         #pragma unroll 8
         for (int s = lo; s < hi; ++s) v += part[s * n + i];
     }
-    red[q][lane] = v;
+    red[q][x] = v;
     __syncthreads();
-    if (q == 0 && i < n)
-        out[i] = from_f32<OT>((red[0][lane] + red[1][lane])
-                              + (red[2][lane] + red[3][lane]));
+    if (q || i >= n) return;
+    float s = 0.f;
+    #pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k][x];
+    out[i] = from_f32<OT>(s);
+}
+
+// 4 results a thread
+template <int OT>
+__global__ __launch_bounds__(256)
+void join_many_kernel(const f32x4* __restrict__ part, int S, long n4,
+                      typename Elem<OT>::T* __restrict__ out) {
+    using T = typename Elem<OT>::T;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    f32x4 v = {0, 0, 0, 0};
+    #pragma unroll 8
+    for (int s = 0; s < S; ++s) v += part[s * n4 + i];
+    union { T t[4]; u32x2 u[sizeof(T) / 2]; } o;
+    #pragma unroll
+    for (int r = 0; r < 4; ++r) o.t[r] = from_f32<OT>(v[r]);
+    #pragma unroll
+    for (int r = 0; r < (int)sizeof(T) / 2; ++r)
+        reinterpret_cast<u32x2*>(out + i * 4)[r] = o.u[r];
 }
 
 // Sums over rows: W lanes side by side take 8 columns each, 256 / W rows at a
@@ -398,10 +419,17 @@ void run_db(const GradArgs& a, char* at, hipStream_t stream) {
 
 void join(const float* part, int S, long n, void* out, int dt,
           hipStream_t stream) {
-    const dim3 grid((unsigned)((n + 63) / 64));
-    #define MX4_J(DT) \
-        hipLaunchKernelGGL((join_kernel<DT>), grid, dim3(256), 0, stream, part, \
-                           S, n, (typename Elem<DT>::T*)out)
+    // (fresh results start on 16 bytes; views of a larger tensor do not occur)
+    const bool many = n % 4 == 0 && n >= 65536;
+    #define MX4_J(DT) do { \
+        if (many) \
+            hipLaunchKernelGGL((join_many_kernel<DT>), \
+                dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, \
+                (const f32x4*)part, S, n / 4, (typename Elem<DT>::T*)out); \
+        else \
+            hipLaunchKernelGGL((join_few_kernel<DT>), \
+                dim3((unsigned)((n + 15) / 16)), dim3(256), 0, stream, part, S, \
+                n, (typename Elem<DT>::T*)out); } while (0)
     if (dt == F32) MX4_J(F32);
     else if (dt == BF16) MX4_J(BF16);
     else MX4_J(F16);

@@ -3,7 +3,7 @@
 // The sum runs over rows, so both operands are wanted across their rows. g's
 // rows go into LDS as they are, past the registers; X's codes, a quarter of
 // that, go there as codes and are written beside as bf16 (every value is exact
-// in it) one step ahead. ds_read_b64_tr_b16 then gives a lane four rows of one
+// in it) two steps ahead. ds_read_b64_tr_b16 then gives a lane four rows of one
 // column: two of them are its operand, in the same order on both sides. So
 // neither operand is ever turned in memory.
 //
@@ -21,7 +21,8 @@
 namespace mx4 {
 namespace {
 
-constexpr int S = 4;            // buffers of g and of codes
+constexpr int S = 5;            // buffers of g and of codes
+constexpr int XS = 3;           // of X as bf16
 constexpr int ROWS = 32;        // of a step
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -60,8 +61,9 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
     constexpr int XQ = (XC + WAVES - 1) / WAVES;
     constexpr int PER = GC + XQ;
     constexpr int STAGE = ROWS * GB + XC * 1024;
-    static_assert(ROWS * GB % (1024 * WAVES) == 0, "whole copies");
-    __shared__ __attribute__((aligned(16))) uint8_t lds[S * STAGE + 2 * ROWS * XB];
+    static_assert(ROWS * GB % (1024 * WAVES) == 0 &&
+                  ROWS * TK / 8 % THREADS == 0, "whole copies, whole words");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[S * STAGE + XS * ROWS * XB];
     uint8_t* const xl = lds + S * STAGE;
     const unsigned to = lds_address(lds);
     const int lane = threadIdx.x & 63;
@@ -119,27 +121,37 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
         if (++lm == per) lm = 0, ++lp;
     };
 
-    // the codes of a step as bf16: 8 of them a thread at a time
-    constexpr int WORDS = ROWS * TK / 8;
-    auto expand = [&](int buf, int to_x, long m0) {
+    // the codes of a step as bf16: 8 of them a thread at a time, fetched before
+    // the matrix instructions of a step and written behind them
+    constexpr int WORDS = ROWS * TK / 8 / THREADS;
+    unsigned code[WORDS], byte[WORDS];
+    auto fetch = [&](int buf) {
         const uint8_t* cl = lds + buf * STAGE + ROWS * GB;
         #pragma unroll
-        for (int q = 0; q < (WORDS + THREADS - 1) / THREADS; ++q) {
+        for (int q = 0; q < WORDS; ++q) {
             const int w = q * THREADS + threadIdx.x;
-            if (WORDS % THREADS && w >= WORDS) break;
             const int m = w / (TK / 8), k8 = w % (TK / 8);   // row, 8 columns
             const int k = (int)(k0 & 127) + k8 * 8;          // from a 128 on
-            const unsigned code = *reinterpret_cast<const unsigned*>(
+            const int b = (((int)k0 + k8 * 8) & 511) >> 5;
+            code[q] = *reinterpret_cast<const unsigned*>(
                 cl + (k >> 7) * 2048 + m * 64 + (k & 127) / 2);
-            const int b = ((int)k0 + k8 * 8 & 511) >> 5;
-            const unsigned byte = cl[(XC - 1) * 1024 + m * 16 + (b & 3) * 4 + (b >> 2)];
-            const float s = scale_f32(byte);
+            byte[q] = cl[(XC - 1) * 1024 + m * 16 + (b & 3) * 4 + (b >> 2)];
+        }
+    };
+    auto expand = [&](int to_x, long m0) {
+        #pragma unroll
+        for (int q = 0; q < WORDS; ++q) {
+            const int w = q * THREADS + threadIdx.x;
+            const int m = w / (TK / 8), k8 = w % (TK / 8);
+            const float s = scale_f32(byte[q]);
+            const unsigned c = code[q];
             u32x4 v;
-            v.x = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0));
-            v.y = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1));
-            v.z = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2));
-            v.w = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3));
-            if (byte == 255u) v = (u32x4){0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+            v.x = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0));
+            v.y = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1));
+            v.z = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2));
+            v.w = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3));
+            if (byte[q] == 255u)
+                v = (u32x4){0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
             if (m0 + m >= M) v = (u32x4){0, 0, 0, 0};
             *reinterpret_cast<u32x4*>(
                 xl + to_x * (ROWS * XB) + m * XB
@@ -165,50 +177,81 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
         #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
 
-    #pragma unroll
-    for (int b = 0; b < S - 1; ++b) {
-        if (b) sent();
-        send(b);
-    }
-    wait_copies<0>();
-    __syncthreads();
-    expand(0, 0, (long)(s0 % per) * ROWS);
-    int buf = 0, xbuf = 0, cm = s0 % per;
-    for (int s = s0; s < s1; ++s) {
-        // The copies of the step behind this one have arrived, this step's X is
-        // written, and every wave is done with the buffers of the step before.
-        wait_copies<(S - 3) * PER>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+    // rows of g that are not there, in the buffer of step `m` of a part
+    auto clear_tail = [&](int buf, int m) {
+        if ((long)(m + 1) * ROWS <= M) return;
         uint8_t* gl = lds + buf * STAGE;
-        const int free = buf == 0 ? S - 1 : buf - 1;
-        buf = buf == S - 1 ? 0 : buf + 1;
-        if ((long)(cm + 1) * ROWS > M) {          // rows that are not there
-            const int have = (int)(M - (long)cm * ROWS);
-            for (int i = have * (GB / 16) + threadIdx.x; i < ROWS * (GB / 16);
-                 i += THREADS)
-                reinterpret_cast<u32x4*>(gl)[i] = (u32x4){0, 0, 0, 0};
-            __syncthreads();
-        }
-        if (++cm == per) cm = 0;
-        sent();
-        send(free);
+        const int have = (int)(M - (long)m * ROWS);
+        for (int i = have * (GB / 16) + threadIdx.x; i < ROWS * (GB / 16);
+             i += THREADS)
+            reinterpret_cast<u32x4*>(gl)[i] = (u32x4){0, 0, 0, 0};
+        __syncthreads();
+    };
+    bf16x8 b[FN], av[FM];
+    // the first reads of a step, made while the step before still computes
+    auto begin = [&](int buf, int xbuf) {
+        const uint8_t* gl = lds + buf * STAGE;
         const uint8_t* xp = xl + xbuf * (ROWS * XB);
-        expand(buf, xbuf ^ 1, (long)cm * ROWS);   // (the last one is not read)
-        bf16x8 b[FN];
         #pragma unroll
         for (int j = 0; j < FN; ++j)
             b[j] = read_across(x_at(xp, 0, wn / 16 + j), x_at(xp, 1, wn / 16 + j));
         #pragma unroll
+        for (int i = 0; i < 2; ++i)
+            av[i] = read_across(g_at(gl, 0, wm / 16 + i), g_at(gl, 1, wm / 16 + i));
+    };
+
+    auto turn = [](int v, int n) { return v == n - 1 ? 0 : v + 1; };
+    #pragma unroll
+    for (int i = 0; i < S - 1; ++i) {
+        if (i) sent();
+        send(i);
+    }
+    int cm = s0 % per;                   // step of its part
+    wait_copies<0>();
+    __syncthreads();
+    fetch(0);
+    expand(0, (long)cm * ROWS);
+    fetch(1);
+    expand(1, (long)turn(cm, per) * ROWS);
+    clear_tail(0, cm);
+    __syncthreads();
+    begin(0, 0);
+    int buf = 0, xbuf = 0;
+    for (int s = s0; s < s1; ++s) {
+        // The copies of the two steps behind this one have arrived, the next
+        // step's X is written, and every wave is done with the buffers of the
+        // step before.
+        wait_copies<(S - 4) * PER>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const uint8_t* gl = lds + buf * STAGE;
+        const int free = buf == 0 ? S - 1 : buf - 1;
+        buf = turn(buf, S), xbuf = turn(xbuf, XS), cm = turn(cm, per);
+        clear_tail(buf, cm);
+        sent();
+        send(free);
+        // X of the step after the next (behind the end it is not read); reads
+        // two fragments ahead of the matrix instructions
+        fetch(turn(buf, S));
+        #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            const bf16x8 a = read_across(g_at(gl, 0, wm / 16 + i),
-                                         g_at(gl, 1, wm / 16 + i));
+            if (i + 2 < FM)
+                av[i + 2] = read_across(g_at(gl, 0, wm / 16 + i + 2),
+                                        g_at(gl, 1, wm / 16 + i + 2));
             #pragma unroll
             for (int j = 0; j < FN; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    b[j], a, acc[i][j], 0, 0, 0);
+                    b[j], av[i], acc[i][j], 0, 0, 0);
         }
-        xbuf ^= 1;
+        begin(buf, xbuf);
+        expand(turn(xbuf, XS), (long)turn(cm, per) * ROWS);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * WORDS, 0);
+        #pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            if (i + 2 < FM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            if (i == FM - 1) __builtin_amdgcn_sched_group_barrier(0x100, 2 * FN + 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, FN, 0);
+        }
     }
     wait_copies<0>();      // no copy is under way when LDS is given up
 
