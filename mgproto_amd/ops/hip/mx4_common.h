@@ -47,8 +47,8 @@ static __device__ __forceinline__ typename Elem<DT>::T from_f32(float v) {
     return (typename Elem<DT>::T)v;
 }
 
-// 2^(byte-127) as a float; 2^-127 lies below the normal numbers. Byte 255
-// gives an infinity here, callers deal with it before.
+// 2^(byte-127) as a float; 2^-127 lies below the normal numbers, and byte 255
+// gives an infinity.
 static __device__ __forceinline__ float scale_f32(unsigned byte) {
     return __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }

@@ -167,20 +167,26 @@ void grad_input_kernel(const uint8_t* __restrict__ a, size_t a_step,
     wait_copies<0>();      // no copy is under way when LDS is given up
 }
 
-// A tile of 256 x 256 halves the bytes a result; it has to be there for each
-// of 256 units. Few columns: 256 x 64.
-struct Plan { int bm, bn, splits; };
+// The tile that ends first: rounds over the blocks that fit, times the cycles of
+// a step (of all blocks on a unit). 15680x512 (sum 2048): 256 x 256 50 us, 256 x
+// 128 36, 128 x 128 43. Few columns: 256 x 64.
+struct Plan { int bm, bn, slots, splits; };
 Plan plan(long M, long K, long steps) {
-    auto tiles = [&](int a, int b) {
-        return ((M + a - 1) / a) * ((K + b - 1) / b);
-    };
-    Plan p{128, 128, 1};
-    if (K <= 64) p = {256, 64, 1};
-    else if (K > 128 && tiles(256, 256) >= 192) p = {256, 256, 1};
-    // a long sum with few tiles is split, at least 8 steps each
-    const long have = tiles(p.bm, p.bn), want = p.bn == 256 ? 256 : 512;
-    if (have * 2 <= want)
-        p.splits = (int)std::max<long>(1, std::min(want / have, steps / 8));
+    static const struct { int bm, bn, slots, cycles; } T[] = {
+        {256, 256, 256, 1260}, {256, 128, 256, 780}, {128, 128, 512, 1380},
+        {256, 64, 512, 1000}};
+    Plan p{};
+    double best = 0;
+    for (const auto& t : T) {
+        const long have = ((M + t.bm - 1) / t.bm) * ((K + t.bn - 1) / t.bn);
+        const double cost = (double)((have + t.slots - 1) / t.slots) * t.cycles;
+        if (p.bm && cost >= best) continue;
+        best = cost;
+        p = {t.bm, t.bn, t.slots, 1};
+        // a long sum with few tiles is split, at least 8 steps each
+        if (have * 4 <= t.slots)
+            p.splits = (int)std::max<long>(1, std::min(t.slots / have, steps / 8));
+    }
     return p;
 }
 
@@ -202,12 +208,13 @@ void grad_input_tiles(const void* a, size_t a_step, size_t a_row, int parts,
     const int total = mt * nt * p.splits;
     #define MX4_G(OT, BM, BN, WM, WN) \
         hipLaunchKernelGGL((grad_input_kernel<OT, BM, BN, WM, WN>), \
-            dim3(std::min((total + 7) / 8 * 8, BN == 256 ? 256 : 512)), \
+            dim3(std::min((total + 7) / 8 * 8, p.slots)), \
             dim3(64 * WM * WN), 0, stream, (const uint8_t*)a, a_step, a_row, \
             steps, per, (const uint8_t*)b, M, K, (typename Elem<OT>::T*)out, mt, \
             nt, p.splits, 4)
     #define MX4_T(OT) do { \
         if (p.bn == 256) MX4_G(OT, 256, 256, 2, 4); \
+        else if (p.bm == 256 && p.bn == 128) MX4_G(OT, 256, 128, 4, 2); \
         else if (p.bn == 128) MX4_G(OT, 128, 128, 2, 2); \
         else MX4_G(OT, 256, 64, 4, 1); } while (0)
     if (odt == F32) MX4_T(F32);

@@ -139,6 +139,7 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
         }
     };
     auto expand = [&](int to_x, long m0) {
+        const bool tail = m0 + ROWS > M;
         #pragma unroll
         for (int q = 0; q < WORDS; ++q) {
             const int w = q * THREADS + threadIdx.x;
@@ -150,25 +151,28 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
             v.y = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1));
             v.z = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2));
             v.w = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3));
-            if (byte[q] == 255u)
-                v = (u32x4){0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-            if (m0 + m >= M) v = (u32x4){0, 0, 0, 0};
+            if (tail && m0 + m >= M) v = (u32x4){0, 0, 0, 0};
             *reinterpret_cast<u32x4*>(
                 xl + to_x * (ROWS * XB) + m * XB
                 + (((k8 >> 1) ^ row_key<XB>(m)) << 5) + (k8 & 1) * 16) = v;
         }
     };
 
-    // Where this lane reads: rows g*8 + r16/4 (and 4 more), columns 4 (r16 & 3)
-    // of a fragment, whose 32 bytes are one piece.
+    // Where this lane reads: rows g*8 + r16/4 (and 4 more, which have the same
+    // key), columns 4 (r16 & 3) of a fragment, whose 32 bytes are one piece.
     const int row0 = g * 8 + (r16 >> 2), in = (r16 & 3) * 8;
-    auto g_at = [&](const uint8_t* p, int h, int piece) {
-        const int m = row0 + h * 4;
-        return p + m * GB + ((piece ^ row_key<GB>(m)) << 5) + in;
+    int ga[FM], xa[FN];
+    #pragma unroll
+    for (int i = 0; i < FM; ++i)
+        ga[i] = row0 * GB + (((wm / 16 + i) ^ row_key<GB>(row0)) << 5) + in;
+    #pragma unroll
+    for (int j = 0; j < FN; ++j)
+        xa[j] = row0 * XB + (((wn / 16 + j) ^ row_key<XB>(row0)) << 5) + in;
+    auto g_frag = [&](const uint8_t* p, int i) {
+        return read_across(p + ga[i], p + ga[i] + 4 * GB);
     };
-    auto x_at = [&](const uint8_t* p, int h, int piece) {
-        const int m = row0 + h * 4;
-        return p + m * XB + ((piece ^ row_key<XB>(m)) << 5) + in;
+    auto x_frag = [&](const uint8_t* p, int j) {
+        return read_across(p + xa[j], p + xa[j] + 4 * XB);
     };
 
     f32x4 acc[FM][FN];
@@ -194,10 +198,10 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
         const uint8_t* xp = xl + xbuf * (ROWS * XB);
         #pragma unroll
         for (int j = 0; j < FN; ++j)
-            b[j] = read_across(x_at(xp, 0, wn / 16 + j), x_at(xp, 1, wn / 16 + j));
+            b[j] = x_frag(xp, j);
         #pragma unroll
         for (int i = 0; i < 2; ++i)
-            av[i] = read_across(g_at(gl, 0, wm / 16 + i), g_at(gl, 1, wm / 16 + i));
+            av[i] = g_frag(gl, i);
     };
 
     auto turn = [](int v, int n) { return v == n - 1 ? 0 : v + 1; };
@@ -236,8 +240,7 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
         #pragma unroll
         for (int i = 0; i < FM; ++i) {
             if (i + 2 < FM)
-                av[i + 2] = read_across(g_at(gl, 0, wm / 16 + i + 2),
-                                        g_at(gl, 1, wm / 16 + i + 2));
+                av[i + 2] = g_frag(gl, i + 2);
             #pragma unroll
             for (int j = 0; j < FN; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(

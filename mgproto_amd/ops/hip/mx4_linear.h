@@ -13,19 +13,17 @@ static __device__ __forceinline__ i32x8 wide(i32x4 v) {
     return (i32x8){v.x, v.y, v.z, v.w, 0, 0, 0, 0};
 }
 
-// the values of 8 codes under one scale byte
+// The values of 8 codes under one scale byte. (Byte 255 becomes an infinite
+// scale here, which the conversion takes for not a number, as it should.)
 static __device__ __forceinline__ void values8(unsigned c, unsigned byte,
                                                float (&f)[8]) {
-    const float s = byte == 255u ? 1.f : scale_f32(byte);
+    const float s = scale_f32(byte);
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
     const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
     const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
     const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
-    const float nan = __uint_as_float(0x7fc00000u);
     f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
     f[4] = d.x; f[5] = d.y; f[6] = e.x; f[7] = e.y;
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = byte == 255u ? nan : f[i];
 }
 
 // 16 bytes a lane from memory into LDS, past the registers: lane i's, from
