@@ -3,6 +3,8 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <tuple>
@@ -104,13 +106,19 @@ Tensor workspace(size_t bytes, const Tensor& like) {
                      like.options().dtype(at::kByte));
 }
 
-struct Packed { Tensor codes, scales; };
+struct Packed {               // room for the blocks of a matrix
+    Tensor codes, scales;
+    explicit Packed(const Tensor& x2) {
+        const int64_t R = x2.size(0), K = x2.size(1);
+        auto opt = x2.options().dtype(at::kByte);
+        codes = at::empty({mx4::steps_of(K), R, 64}, opt);
+        scales = at::empty({mx4::chunks_of(K), R, 16}, opt);
+    }
+};
 
 Packed pack(const Tensor& x2, int dt) {
     const int64_t R = x2.size(0), K = x2.size(1);
-    auto opt = x2.options().dtype(at::kByte);
-    Packed p{at::empty({mx4::steps_of(K), R, 64}, opt),
-             at::empty({mx4::chunks_of(K), R, 16}, opt)};
+    Packed p(x2);
     mx4::quantize(x2.data_ptr(), dt, R, K, row_stride(x2),
                   p.codes.data_ptr<uint8_t>(), p.scales.data_ptr<uint8_t>(),
                   current_stream());
@@ -231,8 +239,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_train(
     CHECK_VALUE(x.device() == w.device(), "mx4_linear: input on ", x.device(),
                 ", weight on ", w.device());
     c10::DeviceGuard guard(x.device());
-    Packed pw = pack(matrix(w, "mx4_linear: weight"), wdt);
-    Packed px = pack(x2, dt);
+    const Tensor w2 = matrix(w, "mx4_linear: weight");
+    Packed pw(w2), px(x2);
+    mx4::quantize_two(
+        w2.data_ptr(), wdt, w2.size(0), row_stride(w2),
+        pw.codes.data_ptr<uint8_t>(), pw.scales.data_ptr<uint8_t>(),
+        x2.data_ptr(), dt, x2.size(0), row_stride(x2),
+        px.codes.data_ptr<uint8_t>(), px.scales.data_ptr<uint8_t>(), K,
+        current_stream());
     Tensor y = product_q(px.codes, px.scales, K, pw.codes, pw.scales, bias,
                          shape_of(x, w.size(0)), dt, -1);
     return {y, px.codes, px.scales, pw.codes, pw.scales};
@@ -291,6 +305,96 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
     mx4::grads(a, (int)form, work.defined() ? work.data_ptr() : nullptr,
                current_stream());
     return {dx, dw, db};
+}
+
+// The differentiable product. The node is native: a small layer's step is
+// bound by the host, and a Python node costs it twice what this one does.
+// The weight is w, or held in 4 bits (wc, ws).
+struct LinearNode : public torch::autograd::Function<LinearNode> {
+    using Context = torch::autograd::AutogradContext;
+    using List = torch::autograd::variable_list;
+
+    static Tensor forward(Context* ctx, const Tensor& x, const OptTensor& w,
+                          const OptTensor& bias, const OptTensor& wc,
+                          const OptTensor& ws, int64_t K) {
+        const bool need_x = x.requires_grad();
+        const bool need_w = w.has_value() && w->requires_grad();
+        const bool need_b = bias.has_value() && bias->requires_grad();
+        Tensor y, xc, xs, c = wc.value_or(Tensor()), s = ws.value_or(Tensor());
+        if (need_w) {        // the rounded rows are kept, a quarter of bf16
+            std::tie(y, xc, xs, c, s) = linear_train(x, *w, bias);
+        } else {
+            if (w.has_value()) std::tie(c, s) = quantize(*w);
+            y = linear(x, c, s, K, bias, -1);
+        }
+        if (!need_x) c = s = Tensor();
+        ctx->save_for_backward({c, s, xc, xs});
+        auto code = [](const Tensor& t) {
+            return (int64_t)dtype_code(t, "mx4_linear");
+        };
+        ctx->saved_data["K"] = K;
+        ctx->saved_data["types"] = std::vector<int64_t>{
+            need_x ? code(x) : -1, need_w ? code(*w) : -1,
+            need_b ? code(*bias) : -1};
+        return y;
+    }
+
+    static List backward(Context* ctx, List grads) {
+        const bool again = at::GradMode::is_enabled() &&
+                           grads[0].requires_grad();
+        const List t = ctx->get_saved_variables();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        List out(6);
+        {
+            at::AutoGradMode off(false);
+            const auto [dx, dw, db] = linear_backward(
+                grads[0], t[0], t[1], t[2], t[3],
+                ctx->saved_data["K"].toInt(), types[0], types[1], types[2], -1);
+            out[0] = dx.value_or(Tensor());
+            out[1] = dw.value_or(Tensor());
+            out[2] = db.value_or(Tensor());
+        }
+        if (again) {         // a second derivative is refused where it is taken
+            for (auto& d : out) {
+                if (!d.defined()) continue;
+                auto refuse = std::make_shared<torch::autograd::DelayedError>(
+                    "mx4_linear is differentiable once", 1);
+                d = (*refuse)(List{d.detach().set_requires_grad(true)})[0];
+            }
+        }
+        return out;
+    }
+};
+
+bool needs_grad(const Tensor& x, const OptTensor& w, const OptTensor& bias) {
+    return at::GradMode::is_enabled() &&
+           (x.requires_grad() || (w.has_value() && w->requires_grad()) ||
+            (bias.has_value() && bias->requires_grad()));
+}
+
+// Q(x) W^T + bias, held weights
+Tensor linear_held(const Tensor& x, const Tensor& wc, const Tensor& ws,
+                   int64_t K, const OptTensor& bias, int64_t form) {
+    if (needs_grad(x, c10::nullopt, bias) && form < 0)
+        return LinearNode::apply(x, c10::nullopt, bias, wc, ws, K);
+    return linear(x, wc, ws, K, bias, form);
+}
+
+// Q(x) Q(w)^T + bias, a float weight
+Tensor linear_float(const Tensor& x, const Tensor& w, const OptTensor& bias) {
+    dtype_code(x, "mx4_linear: input");
+    dtype_code(w, "mx4_linear: weight");
+    CHECK_VALUE(x.dim() >= 1, "mx4_linear: input: rows, not a number");
+    CHECK_VALUE(w.dim() == 2 && w.size(1) == x.size(-1), "mx4_linear: input ",
+                x.sizes(), " and weight ", w.sizes(), " do not match");
+    CHECK_VALUE(x.device() == w.device(), "mx4_linear: input on ", x.device(),
+                ", weight on ", w.device());
+    check_bias(bias, w.size(0), x);
+    if (needs_grad(x, w, bias))
+        return LinearNode::apply(x, w, bias, c10::nullopt, c10::nullopt,
+                                 x.size(-1));
+    const auto [c, s] = quantize(w);
+    return linear(x, c, s, x.size(-1), bias, -1);
 }
 
 // ---------------------------------------------------------------------------
@@ -419,13 +523,14 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
 void register_mx4(pybind11::module& m) {
     m.def("mx4_quantize", &quantize, "rows to MX4 codes and scales");
     m.def("mx4_dequantize", &dequantize, "MX4 codes and scales to values");
-    m.def("mx4_linear", &linear, "Q(x) W^T + bias", py::arg("x"),
+    m.def("mx4_linear", &linear_held, "Q(x) W^T + bias", py::arg("x"),
           py::arg("codes"), py::arg("scales"), py::arg("K"), py::arg("bias"),
           py::arg("form") = -1);
     m.def("mx4_linear_q", &linear_q, "X W^T + bias from 4-bit rows",
           py::arg("xcodes"), py::arg("xscales"), py::arg("K"),
           py::arg("codes"), py::arg("scales"), py::arg("bias"),
           py::arg("dtype"), py::arg("form") = -1);
+    m.def("mx4_linear_float", &linear_float, "Q(x) Q(w)^T + bias");
     m.def("mx4_linear_train", &linear_train,
           "Q(x) Q(w)^T + bias, and the rounded x and w");
     m.def("mx4_linear_backward", &linear_backward,

@@ -141,6 +141,20 @@ static __device__ __forceinline__ unsigned codes8(const u32x4* u, float s) {
     return r;
 }
 
+// 8 elements at p, which need not start on 16 bytes: the memory pipe takes any
+// address in one load. With this and store_piece, fp32 5000x777->777 takes 21 us;
+// 41 with single elements.
+template <int DT>
+static __device__ __forceinline__ void load8(const typename Elem<DT>::T* p,
+                                             u32x4* u) {
+    struct __attribute__((packed, aligned(sizeof(*p)))) Any {
+        u32x4 v[DT == F32 ? 2 : 1];
+    };
+    const Any a = *reinterpret_cast<const Any*>(p);
+    u[0] = a.v[0];
+    if constexpr (DT == F32) u[1] = a.v[1];
+}
+
 // n <= 8 elements at p, the rest zero, as codes8 takes them
 template <int DT>
 static __device__ __forceinline__ void load8_tail(
@@ -157,6 +171,31 @@ static __device__ __forceinline__ void load8_tail(
             const unsigned hi = 2 * i + 1 < n ? q[2 * i + 1] : 0;
             u[0][i] = lo | (hi << 16);
         }
+    }
+}
+
+// W consecutive elements, 8 or 16 bytes of them at a time
+template <class T, int W>
+union Piece {
+    static constexpr int B = W * sizeof(T) % 16 ? 8 : 16;   // bytes a store
+    typedef unsigned Word __attribute__((ext_vector_type(B / 4)));
+    T v[W];
+    Word u[W * sizeof(T) / B];
+};
+// whole where n >= W elements are left for it, wherever q points
+template <class T, int W>
+static __device__ __forceinline__ void store_piece(T* q, const Piece<T, W>& o,
+                                                   long n) {
+    using P = Piece<T, W>;
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { typename P::Word u; };
+    if (n >= W) {
+        #pragma unroll
+        for (int i = 0; i < (int)(W * sizeof(T)) / P::B; ++i)
+            reinterpret_cast<Any*>(q)[i].u = o.u[i];
+    } else {
+        #pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (e < n) q[e] = o.v[e];
     }
 }
 
@@ -177,6 +216,12 @@ static __device__ __forceinline__ size_t scale_at(long R, long row, int b) {
 
 void quantize(const void* x, int dt, long rows, long K, long ldx,
               uint8_t* codes, uint8_t* scales, hipStream_t stream);
+
+// two matrices of K columns in one launch
+void quantize_two(const void* x, int dt, long rows, long ldx, uint8_t* codes,
+                  uint8_t* scales, const void* x2, int dt2, long rows2,
+                  long ldx2, uint8_t* codes2, uint8_t* scales2, long K,
+                  hipStream_t stream);
 
 void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
                 long K, void* out, int dt, hipStream_t stream);

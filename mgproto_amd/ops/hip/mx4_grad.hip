@@ -34,6 +34,24 @@ static __device__ __forceinline__ unsigned part_of(float v, int p) {
     return b >> 16;
 }
 
+// what load8 gave
+template <int DT>
+static __device__ __forceinline__ void floats8(const u32x4* u, float* f) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == F32) {
+            f[i] = __uint_as_float(u[0][i]);
+            f[4 + i] = __uint_as_float(u[1][i]);
+        } else {
+            const unsigned w = u[0][i];
+            f[2 * i] = DT == BF16 ? __uint_as_float(w << 16)
+                                  : (float)as_f16x2(w).x;
+            f[2 * i + 1] = DT == BF16 ? __uint_as_float(w & 0xffff0000u)
+                                      : (float)as_f16x2(w).y;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------
 // operands laid out for the tiles
 // ---------------------------------------------------------------------------
@@ -49,10 +67,12 @@ void parts_kernel(const typename Elem<DT>::T* __restrict__ g, long M, int N,
     for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
         const long m = t / upr;
         const int u = (int)(t - m * upr), n = u * 8;
+        const typename Elem<DT>::T* q = g + m * N + n;
+        u32x4 raw[DT == F32 ? 2 : 1];
+        if (n + 8 <= N) load8<DT>(q, raw);
+        else load8_tail<DT>(q, N - n, raw);
         float v[8];
-        #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = n + i < N ? (float)g[m * N + n + i] : 0.f;
+        floats8<DT>(raw, v);
         const long at = STEPPED ? ((long)(u >> 2) * M + m) * 4 + (u & 3) : t;
         for (int p = 0; p < P; ++p) {
             u32x4 o;
@@ -151,7 +171,7 @@ void join_many_kernel(const f32x4* __restrict__ part, int S, long n4,
 
 // Sums over rows: W lanes side by side take 8 columns each, 256 / W rows at a
 // time; part[chunk][n]
-template <int DT, bool VEC>
+template <int DT>
 __global__ __launch_bounds__(256)
 void col_sum_kernel(const typename Elem<DT>::T* __restrict__ g, long M, int N,
                     int W, long rows, float* __restrict__ part) {
@@ -166,26 +186,12 @@ void col_sum_kernel(const typename Elem<DT>::T* __restrict__ g, long M, int N,
         for (long m = lo + y; m < hi; m += Y) {
             u32x4 u[E];
             const typename Elem<DT>::T* p = g + m * N + n;
-            if (VEC && n + 8 <= N) {
-                #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    u[e] = reinterpret_cast<const u32x4*>(p)[e];
-            } else {
-                load8_tail<DT>(p, (int)min((long)8, N - n), u);
-            }
+            if (n + 8 <= N) load8<DT>(p, u);
+            else load8_tail<DT>(p, (int)(N - n), u);
+            float f[8];
+            floats8<DT>(u, f);
             #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (DT == F32) {
-                    v[i] += __uint_as_float(u[0][i]);
-                    v[4 + i] += __uint_as_float(u[1][i]);
-                } else {
-                    const unsigned w = u[0][i];
-                    v[2 * i] += DT == BF16 ? __uint_as_float(w << 16)
-                                           : (float)as_f16x2(w).x;
-                    v[2 * i + 1] += DT == BF16 ? __uint_as_float(w & 0xffff0000u)
-                                               : (float)as_f16x2(w).y;
-                }
-            }
+            for (int i = 0; i < 8; ++i) v[i] += f[i];
         }
     }
     #pragma unroll
@@ -401,16 +407,13 @@ void run_dw(const GradArgs& a, char* at, hipStream_t stream) {
 void run_db(const GradArgs& a, char* at, hipStream_t stream) {
     const Sums s = sums(a.M, a.N);
     const dim3 grid(s.gx, (unsigned)s.chunks);
-    const bool vec = a.aligned && a.N % 8 == 0;
-    #define MX4_S(DT, V) \
-        hipLaunchKernelGGL((col_sum_kernel<DT, V>), grid, dim3(256), 0, stream, \
+    #define MX4_S(DT) \
+        hipLaunchKernelGGL((col_sum_kernel<DT>), grid, dim3(256), 0, stream, \
                            (const typename Elem<DT>::T*)a.g, a.M, (int)a.N, s.W, \
                            s.rows, (float*)at)
-    #define MX4_V(DT) do { if (vec) MX4_S(DT, true); else MX4_S(DT, false); } while (0)
-    if (a.g_dt == F32) MX4_V(F32);
-    else if (a.g_dt == BF16) MX4_V(BF16);
-    else MX4_V(F16);
-    #undef MX4_V
+    if (a.g_dt == F32) MX4_S(F32);
+    else if (a.g_dt == BF16) MX4_S(BF16);
+    else MX4_S(F16);
     #undef MX4_S
     join((const float*)at, s.chunks, a.N, a.db, a.db_dt, stream);
 }

@@ -260,7 +260,6 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
 
     // a lane holds 4 consecutive columns of row n of each fragment
     T* out = c + (splits > 1 ? (size_t)z * N * K : 0);
-    const bool vec = K % 4 == 0;
     #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const long n = n0 + wm + i * 16 + r16;
@@ -268,20 +267,10 @@ void grad_weight_kernel(const uint8_t* __restrict__ gv, long row, size_t part,
         #pragma unroll
         for (int j = 0; j < FN; ++j) {
             const long k = k0 + wn + j * 16 + g * 4;
-            T* q = out + n * K + k;
-            union { T v[4]; u32x2 u[sizeof(T) / 2]; } o;
+            Piece<T, 4> o;
             #pragma unroll
             for (int r = 0; r < 4; ++r) o.v[r] = from_f32<OT>(acc[i][j][r]);
-            if (vec) {
-                if (k >= K) continue;
-                #pragma unroll
-                for (int r = 0; r < (int)sizeof(T) / 2; ++r)
-                    reinterpret_cast<u32x2*>(q)[r] = o.u[r];
-            } else {
-                #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (k + r < K) q[r] = o.v[r];
-            }
+            store_piece(out + n * K + k, o, K - k);
         }
     }
 }

@@ -94,7 +94,7 @@ static __device__ __forceinline__ void load_bias(float (&b)[4 * FN],
 }
 
 // Rows m, m + 16, ... of y from column n on: 4*FN consecutive columns a lane.
-// Pieces of 16 bytes where rows start on them, single elements elsewhere.
+// Pieces of 16 bytes, wherever a row starts; single elements at its end.
 template <int OT, int FM, int FN>
 static __device__ __forceinline__ void store_rows(
         const f32x4 (&acc)[FM][FN], typename Elem<OT>::T* y, long M, long N,
@@ -102,7 +102,6 @@ static __device__ __forceinline__ void store_rows(
     using T = typename Elem<OT>::T;
     constexpr int PER = OT == F32 ? 1 : (FN % 2 ? 1 : 2);   // tiles a piece
     constexpr int W = 4 * PER;                              // columns a piece
-    const bool vec = N % W == 0;
     #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const long row = m + i * 16;
@@ -111,22 +110,11 @@ static __device__ __forceinline__ void store_rows(
         for (int j = 0; j < FN; j += PER) {
             const long c = n + j * 4;
             T* q = y + row * N + c;
-            union { T v[W]; u32x2 h[W * sizeof(T) / 8]; } o;
+            Piece<T, W> o;
             #pragma unroll
             for (int r = 0; r < W; ++r)
                 o.v[r] = from_f32<OT>(acc[i][j + r / 4][r % 4] + b[j * 4 + r]);
-            if (vec) {
-                if (c >= N) continue;
-                if constexpr (W * sizeof(T) == 16)
-                    *reinterpret_cast<u32x4*>(q) =
-                        (u32x4){o.h[0].x, o.h[0].y, o.h[1].x, o.h[1].y};
-                else
-                    *reinterpret_cast<u32x2*>(q) = o.h[0];
-            } else {
-                #pragma unroll
-                for (int r = 0; r < W; ++r)
-                    if (c + r < N) q[r] = o.v[r];
-            }
+            store_piece(q, o, N - c);
         }
     }
 }
@@ -136,7 +124,7 @@ void tiles(const uint8_t* xc, const uint8_t* xs, long M, long K,
            const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
            int bias_dt, void* y, int dt, bool large, hipStream_t stream);
 // mx4_rounding.hip
-void rounding(const void* x, int dt, bool vec, long M, long K, long ldx,
+void rounding(const void* x, int dt, long M, long K, long ldx,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
               int bias_dt, void* y, hipStream_t stream);
 

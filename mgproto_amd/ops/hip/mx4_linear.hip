@@ -21,15 +21,14 @@ namespace {
 constexpr int CODES = -1;     // x is held in 4 bits already
 
 // One block of x: loaded, rounded; codes and scale byte stay in this lane.
-template <int DT, bool VEC>
+template <int DT>
 static __device__ __forceinline__ i32x4 round_block(
         const typename Elem<DT>::T* row, int kb, int K, int& byte) {
     constexpr int W = DT == F32 ? 2 : 1;
     u32x4 u[4 * W];
-    if (VEC && kb + 32 <= K) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(row + kb);
+    if (kb + 32 <= K) {
         #pragma unroll
-        for (int i = 0; i < 4 * W; ++i) u[i] = p[i];
+        for (int i = 0; i < 4; ++i) load8<DT>(row + kb + i * 8, u + i * W);
     } else {
         #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -45,7 +44,7 @@ static __device__ __forceinline__ i32x4 round_block(
 
 // FM x FN tiles of 16 x 16 a block. Its four waves take every fourth step of
 // 128 each and are joined in LDS, in their order.
-template <int AT, bool VEC, int OT, int FM, int FN>
+template <int AT, int OT, int FM, int FN>
 __global__ __launch_bounds__(256)
 void linear_rows_kernel(const void* __restrict__ xv,
                         const uint8_t* __restrict__ xs, long M, int K, int steps,
@@ -92,7 +91,7 @@ void linear_rows_kernel(const void* __restrict__ xv,
                 xb[i] = xs[scale_at(M, xrow[i], s * 4 + g)];
             } else {
                 using E = typename Elem<AT == CODES ? F32 : AT>::T;
-                x[i] = round_block<AT == CODES ? F32 : AT, VEC>(
+                x[i] = round_block<AT == CODES ? F32 : AT>(
                     reinterpret_cast<const E*>(xv) + xrow[i] * ldx,
                     s * 128 + g * 32, K, xb[i]);
             }
@@ -127,14 +126,14 @@ void linear_rows_kernel(const void* __restrict__ xv,
     store_rows<OT, FM, FN>(acc, y, M, N, m0 + r16, n0 + g * (4 * FN), b);
 }
 
-template <int AT, bool VEC, int OT>
+template <int AT, int OT>
 void launch_rows(const void* x, const uint8_t* xs, long M, long K, long ldx,
                  const uint8_t* wc, const uint8_t* ws, long N,
                  const void* bias, int bias_dt, void* y, int form,
                  hipStream_t stream) {
     #define MX4_L(F) do { \
         const long mt = (M + 16 * F - 1) / (16 * F), nt = (N + 16 * F - 1) / (16 * F); \
-        hipLaunchKernelGGL((linear_rows_kernel<AT, VEC, OT, F, F>), \
+        hipLaunchKernelGGL((linear_rows_kernel<AT, OT, F, F>), \
             dim3((unsigned)(mt * nt)), dim3(256), 0, stream, x, xs, M, (int)K, \
             (int)steps_of(K), ldx, wc, ws, N, bias, bias_dt, (typename Elem<OT>::T*)y, \
             (int)nt); } while (0)
@@ -153,8 +152,6 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 // Rounding in the blocks saves a launch (4 us) and a pass over x, but every
 // block rounds its rows again: 784x1024->256 5.4 against 9.0 with the rounding
 // before, 64x4096->4096 (2^30) 12.8 against 11.5, 128x4096->4096 22 against 16.
-// Rows that do not start on 16 bytes are read element by element: 777x333->1001
-// (2^28) 17 against 10.
 //
 // Many rows and few columns: x's way from memory counts, and tiles of 128 rows
 // round it on the way: 62720x1024->256 39 against 42, 1003520x256->64 146
@@ -163,7 +160,7 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 // (1003520x64->64 167 against 87).
 int linear_form(long M, long K, long N, bool aligned) {
     const double work = (double)(M > 16 ? M : 16) * K * N;
-    if (work < (aligned ? 0x1p30 : 0x1p27)) return M <= 16 ? ROWS16 : ROWS32;
+    if (work < 0x1p30) return M <= 16 ? ROWS16 : ROWS32;
     if (aligned && M >= 4096 && N <= 256 && K >= 256) return ROUNDING;
     return linear_q_form(M, K, N);
 }
@@ -189,10 +186,8 @@ size_t linear_bytes(int form, long M, long K) {
 void linear(const void* x, int dt, long M, long K, long ldx,
             const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
             int bias_dt, void* y, int form, void* work, hipStream_t stream) {
-    const int es = dt == F32 ? 4 : 2;
-    const bool vec = (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0;
     if (form == ROUNDING) {
-        rounding(x, dt, vec, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream);
+        rounding(x, dt, M, K, ldx, wc, ws, N, bias, bias_dt, y, stream);
         return;
     }
     if (form >= HELD16) {
@@ -203,15 +198,9 @@ void linear(const void* x, int dt, long M, long K, long ldx,
         return;
     }
     #define MX4_ARGS x, nullptr, M, K, ldx, wc, ws, N, bias, bias_dt, y, form, stream
-    if (vec) {
-        if (dt == F32) launch_rows<F32, true, F32>(MX4_ARGS);
-        else if (dt == BF16) launch_rows<BF16, true, BF16>(MX4_ARGS);
-        else launch_rows<F16, true, F16>(MX4_ARGS);
-    } else {
-        if (dt == F32) launch_rows<F32, false, F32>(MX4_ARGS);
-        else if (dt == BF16) launch_rows<BF16, false, BF16>(MX4_ARGS);
-        else launch_rows<F16, false, F16>(MX4_ARGS);
-    }
+    if (dt == F32) launch_rows<F32, F32>(MX4_ARGS);
+    else if (dt == BF16) launch_rows<BF16, BF16>(MX4_ARGS);
+    else launch_rows<F16, F16>(MX4_ARGS);
     #undef MX4_ARGS
 }
 
@@ -224,9 +213,9 @@ void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
         return;
     }
     #define MX4_ARGS xc, xs, M, K, 0, wc, ws, N, bias, bias_dt, y, form, stream
-    if (dt == F32) launch_rows<CODES, true, F32>(MX4_ARGS);
-    else if (dt == BF16) launch_rows<CODES, true, BF16>(MX4_ARGS);
-    else launch_rows<CODES, true, F16>(MX4_ARGS);
+    if (dt == F32) launch_rows<CODES, F32>(MX4_ARGS);
+    else if (dt == BF16) launch_rows<CODES, BF16>(MX4_ARGS);
+    else launch_rows<CODES, F16>(MX4_ARGS);
     #undef MX4_ARGS
 }
 

@@ -16,16 +16,24 @@ namespace {
 
 constexpr int ROWS = 4;       // pieces a wave has under way
 
+struct Rows {                 // of one matrix, and where its blocks go
+    const void* x;
+    long R, ldx;
+    uint8_t *codes, *scales;
+    int dt;
+};
+
 // LPR lanes hold a row's piece: 64 of them 512 elements, 16 of them 128
-template <int DT, bool VEC, int LPR>
-__global__ __launch_bounds__(256)
-void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long R, int K,
-                     int steps, long ldx, uint8_t* __restrict__ codes,
-                     uint8_t* __restrict__ scales, int chunks) {
+template <int DT, int LPR>
+static __device__ __forceinline__ void quantize_rows(const Rows& a, int K,
+                                                     int steps, int chunks,
+                                                     long block) {
     constexpr int W = DT == F32 ? 2 : 1;
     constexpr int RPW = 64 / LPR;                // rows side by side
+    const typename Elem<DT>::T* x = (const typename Elem<DT>::T*)a.x;
+    const long R = a.R;
     const int lane = threadIdx.x & 63, sub = lane % LPR;
-    const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long wave = block * 4 + (threadIdx.x >> 6);
     const int chunk = (int)(wave % chunks);
     const long row0 = wave / chunks * (RPW * ROWS) + lane / LPR;
     const int k = chunk * 512 + sub * 8, s = k >> 7;
@@ -33,14 +41,9 @@ void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long R, int K,
     #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const long row = row0 + i * RPW;
-        const typename Elem<DT>::T* p = x + min(row, R - 1) * ldx + k;
-        if (VEC && k + 8 <= K) {
-            #pragma unroll
-            for (int e = 0; e < W; ++e)
-                u[i][e] = reinterpret_cast<const u32x4*>(p)[e];
-        } else {
-            load8_tail<DT>(p, K - k, u[i]);
-        }
+        const typename Elem<DT>::T* p = x + min(row, R - 1) * a.ldx + k;
+        if (k + 8 <= K) load8<DT>(p, u[i]);
+        else load8_tail<DT>(p, K - k, u[i]);
     }
     #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
@@ -57,15 +60,36 @@ void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long R, int K,
         }
         if (row >= R) continue;
         if (s < steps)
-            reinterpret_cast<unsigned*>(codes)[
+            reinterpret_cast<unsigned*>(a.codes)[
                 ((size_t)s * R + row) * 16 + (sub & 15)] = byte == 255u ? 0u : c;
         if (sub < 16 && (sub & 3) == 0)
-            reinterpret_cast<unsigned*>(scales)[
+            reinterpret_cast<unsigned*>(a.scales)[
                 ((size_t)chunk * R + row) * 4 + (sub >> 2)] = four;
     }
 }
 
-template <int DT, bool VEC, int LPR>
+template <int DT, int LPR>
+__global__ __launch_bounds__(256)
+void quantize_kernel(const Rows a, int K, int steps, int chunks) {
+    quantize_rows<DT, LPR>(a, K, steps, chunks, blockIdx.x);
+}
+
+// Two matrices of the same row length, the first in the first blocks: one
+// launch less for a training step, which rounds the weight and the rows.
+template <int LPR>
+__global__ __launch_bounds__(256)
+void quantize_two_kernel(const Rows a, const Rows b, unsigned first, int K,
+                         int steps, int chunks) {
+    const bool is_a = blockIdx.x < first;
+    const Rows& r = is_a ? a : b;
+    const long block = is_a ? blockIdx.x : blockIdx.x - first;
+    if (r.dt == F32) quantize_rows<F32, LPR>(r, K, steps, chunks, block);
+    else if (r.dt == BF16)
+        quantize_rows<BF16, LPR>(r, K, steps, chunks, block);
+    else quantize_rows<F16, LPR>(r, K, steps, chunks, block);
+}
+
+template <int DT, int LPR>
 __global__ __launch_bounds__(256)
 void dequantize_kernel(const uint8_t* __restrict__ codes,
                        const uint8_t* __restrict__ scales, long R, int K,
@@ -90,21 +114,12 @@ void dequantize_kernel(const uint8_t* __restrict__ codes,
     for (int i = 0; i < ROWS; ++i) {
         const long row = row0 + i * RPW;
         if (row >= R) continue;
-        union { T v[8]; u32x4 u[sizeof(T) / 2]; } o;
+        Piece<T, 8> o;
         float f[8];
         values8(c[i], byte[i], f);
         #pragma unroll
         for (int e = 0; e < 8; ++e) o.v[e] = from_f32<DT>(f[e]);
-        T* q = out + row * K + k;
-        if (VEC) {
-            #pragma unroll
-            for (int e = 0; e < (int)sizeof(T) / 2; ++e)
-                reinterpret_cast<u32x4*>(q)[e] = o.u[e];
-        } else {
-            #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (k + e < K) q[e] = o.v[e];
-        }
+        store_piece(out + row * K + k, o, K - k);
     }
 }
 
@@ -120,51 +135,58 @@ unsigned blocks_for(long R, long K, bool shortrow) {
 void quantize(const void* x, int dt, long rows, long K, long ldx,
               uint8_t* codes, uint8_t* scales, hipStream_t stream) {
     if (rows == 0 || K == 0) return;
-    const int es = dt == F32 ? 4 : 2;
-    const bool vec = (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0;
     const bool shortrow = K <= 128;
+    const Rows a{x, rows, ldx, codes, scales, dt};
     const dim3 grid(blocks_for(rows, K, shortrow));
-    #define MX4_Q(DT, V, L) \
-        hipLaunchKernelGGL((quantize_kernel<DT, V, L>), grid, dim3(256), 0, \
-                           stream, (const typename Elem<DT>::T*)x, rows, \
-                           (int)K, (int)steps_of(K), ldx, codes, scales, \
-                           (int)chunks_of(K))
-    #define MX4_L(DT, V) do { if (shortrow) MX4_Q(DT, V, 16); \
-                              else MX4_Q(DT, V, 64); } while (0)
-    if (vec) {
-        if (dt == F32) MX4_L(F32, true);
-        else if (dt == BF16) MX4_L(BF16, true);
-        else MX4_L(F16, true);
-    } else {
-        if (dt == F32) MX4_L(F32, false);
-        else if (dt == BF16) MX4_L(BF16, false);
-        else MX4_L(F16, false);
-    }
+    #define MX4_Q(DT, L) \
+        hipLaunchKernelGGL((quantize_kernel<DT, L>), grid, dim3(256), 0, stream, \
+                           a, (int)K, (int)steps_of(K), (int)chunks_of(K))
+    #define MX4_L(DT) do { if (shortrow) MX4_Q(DT, 16); \
+                           else MX4_Q(DT, 64); } while (0)
+    if (dt == F32) MX4_L(F32);
+    else if (dt == BF16) MX4_L(BF16);
+    else MX4_L(F16);
     #undef MX4_L
+    #undef MX4_Q
+}
+
+void quantize_two(const void* x, int dt, long rows, long ldx, uint8_t* codes,
+                  uint8_t* scales, const void* x2, int dt2, long rows2,
+                  long ldx2, uint8_t* codes2, uint8_t* scales2, long K,
+                  hipStream_t stream) {
+    if (K == 0 || rows == 0 || rows2 == 0) {
+        quantize(x, dt, rows, K, ldx, codes, scales, stream);
+        quantize(x2, dt2, rows2, K, ldx2, codes2, scales2, stream);
+        return;
+    }
+    const bool shortrow = K <= 128;
+    const Rows a{x, rows, ldx, codes, scales, dt};
+    const Rows b{x2, rows2, ldx2, codes2, scales2, dt2};
+    const unsigned first = blocks_for(rows, K, shortrow);
+    const dim3 grid(first + blocks_for(rows2, K, shortrow));
+    #define MX4_Q(L) \
+        hipLaunchKernelGGL((quantize_two_kernel<L>), grid, dim3(256), 0, stream, \
+                           a, b, first, (int)K, (int)steps_of(K), \
+                           (int)chunks_of(K))
+    if (shortrow) MX4_Q(16);
+    else MX4_Q(64);
     #undef MX4_Q
 }
 
 void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
                 long K, void* out, int dt, hipStream_t stream) {
     if (rows == 0 || K == 0) return;
-    const bool vec = K % 8 == 0;     // fresh outputs start on 16 bytes
     const bool shortrow = K <= 128;
     const dim3 grid(blocks_for(rows, K, shortrow));
-    #define MX4_D(DT, V, L) \
-        hipLaunchKernelGGL((dequantize_kernel<DT, V, L>), grid, dim3(256), 0, \
+    #define MX4_D(DT, L) \
+        hipLaunchKernelGGL((dequantize_kernel<DT, L>), grid, dim3(256), 0, \
                            stream, codes, scales, rows, (int)K, \
                            (typename Elem<DT>::T*)out, (int)chunks_of(K))
-    #define MX4_L(DT, V) do { if (shortrow) MX4_D(DT, V, 16); \
-                              else MX4_D(DT, V, 64); } while (0)
-    if (vec) {
-        if (dt == F32) MX4_L(F32, true);
-        else if (dt == BF16) MX4_L(BF16, true);
-        else MX4_L(F16, true);
-    } else {
-        if (dt == F32) MX4_L(F32, false);
-        else if (dt == BF16) MX4_L(BF16, false);
-        else MX4_L(F16, false);
-    }
+    #define MX4_L(DT) do { if (shortrow) MX4_D(DT, 16); \
+                           else MX4_D(DT, 64); } while (0)
+    if (dt == F32) MX4_L(F32);
+    else if (dt == BF16) MX4_L(BF16);
+    else MX4_L(F16);
     #undef MX4_L
     #undef MX4_D
 }

@@ -16,7 +16,7 @@
 namespace mx4 {
 namespace {
 
-template <int DT, bool VEC, int BM, int BN, int WM, int WN>
+template <int DT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN)
 void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
                      int steps, long ldx, const uint8_t* __restrict__ wc,
@@ -73,13 +73,8 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
             const int u = q * THREADS + tid, r = u >> 5;
             const int at = k * 256 + (u & 31) * 8;
             const typename Elem<DT>::T* p = x0 + min(r, lastx) * ldx + at;
-            if (VEC && at + 8 <= K) {
-                #pragma unroll
-                for (int i = 0; i < W; ++i)
-                    raw[q][i] = reinterpret_cast<const u32x4*>(p)[i];
-            } else {
-                load8_tail<DT>(p, K - at, raw[q]);
-            }
+            if (at + 8 <= K) load8<DT>(p, raw[q]);
+            else load8_tail<DT>(p, K - at, raw[q]);
         }
     };
     auto store_x = [&](int buf) {
@@ -165,14 +160,14 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     store_rows<DT, FM, FN>(acc, y, M, N, m0 + wm + r16, n, b);
 }
 
-template <int DT, bool VEC, int BM, int BN, int WM, int WN>
+template <int DT, int BM, int BN, int WM, int WN>
 void launch_rounding(const void* x, long M, long K, long ldx,
                      const uint8_t* wc, const uint8_t* ws, long N,
                      const void* bias, int bias_dt, void* y,
                      hipStream_t stream) {
     using T = typename Elem<DT>::T;
     const int mt = (int)((M + BM - 1) / BM), nt = (int)((N + BN - 1) / BN);
-    hipLaunchKernelGGL((rounding_kernel<DT, VEC, BM, BN, WM, WN>),
+    hipLaunchKernelGGL((rounding_kernel<DT, BM, BN, WM, WN>),
                        dim3((unsigned)(mt * nt)), dim3(64 * WM * WN), 0, stream,
                        (const T*)x, M, (int)K, (int)steps_of(K), ldx, wc, ws, N,
                        bias, bias_dt, (T*)y, nt, mt * nt);
@@ -180,24 +175,20 @@ void launch_rounding(const void* x, long M, long K, long ldx,
 
 }  // namespace
 
-void rounding(const void* x, int dt, bool vec, long M, long K, long ldx,
+void rounding(const void* x, int dt, long M, long K, long ldx,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
               int bias_dt, void* y, hipStream_t stream) {
-    #define MX4_T(DT, V, BN, WM, WN) \
-        launch_rounding<DT, V, 128, BN, WM, WN>(x, M, K, ldx, wc, ws, N, bias, \
-                                                bias_dt, y, stream)
-    #define MX4_V(DT, BN, WM, WN) do { \
-        if (vec) MX4_T(DT, true, BN, WM, WN); \
-        else MX4_T(DT, false, BN, WM, WN); } while (0)
+    #define MX4_T(DT, BN, WM, WN) \
+        launch_rounding<DT, 128, BN, WM, WN>(x, M, K, ldx, wc, ws, N, bias, \
+                                             bias_dt, y, stream)
     #define MX4_D(BN, WM, WN) do { \
-        if (dt == F32) MX4_V(F32, BN, WM, WN); \
-        else if (dt == BF16) MX4_V(BF16, BN, WM, WN); \
-        else MX4_V(F16, BN, WM, WN); } while (0)
+        if (dt == F32) MX4_T(F32, BN, WM, WN); \
+        else if (dt == BF16) MX4_T(BF16, BN, WM, WN); \
+        else MX4_T(F16, BN, WM, WN); } while (0)
     if (N > 128) MX4_D(256, 2, 4);
     else if (N > 64) MX4_D(128, 4, 2);
     else MX4_D(64, 8, 1);
     #undef MX4_D
-    #undef MX4_V
     #undef MX4_T
 }
 

@@ -159,46 +159,32 @@ def mx4_dequantize(q: MX4Tensor,
 
 
 class _MX4Linear(torch.autograd.Function):
-    """weight: a float [N, K] matrix, or None with (wc, ws) held in 4 bits."""
+    """The PyTorch form; that of GPU tensors is native. weight: a float [N, K]
+    matrix, or None with (wc, ws) held in 4 bits."""
 
     @staticmethod
     def forward(ctx, x, weight, wc, ws, bias):
-        ext = _ext(x)
         K = x.shape[-1]
         need_x, need_w = ctx.needs_input_grad[:2]
-        xc = xs = None
-        if ext is None:
-            xc, xs = reference.mx4_quantize(_matrix(x))
-            if weight is not None:
-                wc, ws = reference.mx4_quantize(weight)
-            with torch.autocast(x.device.type, enabled=False):
-                y = reference.mx4_product(xc, xs, wc, ws, K, bias, x.dtype)
-            y = y.view(*x.shape[:-1], wc.shape[1])
-        elif need_w:    # the rounded rows are kept, a quarter of x in bf16
-            y, xc, xs, wc, ws = ext.mx4_linear_train(x, weight, bias)
-        else:
-            if weight is not None:
-                wc, ws = ext.mx4_quantize(weight)
-            y = ext.mx4_linear(x, wc, ws, K, bias)
+        xc, xs = reference.mx4_quantize(_matrix(x))
+        if weight is not None:
+            wc, ws = reference.mx4_quantize(weight)
+        with torch.autocast(x.device.type, enabled=False):
+            y = reference.mx4_product(xc, xs, wc, ws, K, bias, x.dtype)
         ctx.save_for_backward(*((wc, ws) if need_x else (None, None)),
                               *((xc, xs) if need_w else (None, None)))
         ctx.K = K
         ctx.types = tuple(
             _CODE[t.dtype] if need else -1 for t, need in
             zip((x, weight, bias), (need_x, need_w, ctx.needs_input_grad[4])))
-        return y
+        return y.view(*x.shape[:-1], wc.shape[1])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        ext = _ext(g)
-        if ext is not None:
-            dx, dw, db = ext.mx4_linear_backward(g, *ctx.saved_tensors, ctx.K,
-                                                 *ctx.types)
-        else:
-            with torch.autocast(g.device.type, enabled=False):
-                dx, dw, db = reference.mx4_backward(g, *ctx.saved_tensors,
-                                                    ctx.K, *ctx.types)
+        with torch.autocast(g.device.type, enabled=False):
+            dx, dw, db = reference.mx4_backward(g, *ctx.saved_tensors, ctx.K,
+                                                *ctx.types)
         return dx, dw, None, None, db
 
 
@@ -211,14 +197,13 @@ def mx4_linear(x: torch.Tensor, weight: Union[MX4Tensor, torch.Tensor],
     the weight its column. Differentiable once, in x, a float weight and bias.
     """
     held = type(weight) is MX4Tensor
-    train = torch.is_grad_enabled() and (
-        x.requires_grad or not held and weight.requires_grad
-        or bias is not None and bias.requires_grad)
-    if held and not train and x.is_cuda and len(weight.shape) == 2:
+    if isinstance(x, torch.Tensor) and x.is_cuda:
         ext = _ext(x)                  # refuses what the checks below refuse
-        if ext is not None:
+        if ext is not None and held and len(weight.shape) == 2:
             return ext.mx4_linear(x, weight.codes, weight.scales,
                                   weight.shape[1], bias)
+        if ext is not None and isinstance(weight, torch.Tensor):
+            return ext.mx4_linear_float(x, weight, bias)
     _check_float(x, 'mx4_linear: input')
     if not held:
         _check_float(weight, 'mx4_linear: weight')
@@ -239,7 +224,4 @@ def mx4_linear(x: torch.Tensor, weight: Union[MX4Tensor, torch.Tensor],
             raise ValueError(f'mx4_linear: input on {x.device}, bias on '
                              f'{bias.device}')
     wc, ws = (weight.codes, weight.scales) if held else (None, None)
-    if not train:
-        x, bias = x.detach(), None if bias is None else bias.detach()
-        weight = weight if held else weight.detach()
     return _MX4Linear.apply(x, None if held else weight, wc, ws, bias)

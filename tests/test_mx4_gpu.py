@@ -363,6 +363,21 @@ def test_refusals():
     x = torch.randn(4, 64, device='cuda')
     with pytest.raises(ValueError, match='input on cuda'):
         ops.mx4_linear(x, q)
+    w = torch.randn(8, 64, device='cuda')
+    with pytest.raises(ValueError, match='do not match'):
+        ops.mx4_linear(x[:, :63], w)
+    with pytest.raises(ValueError, match='do not match'):
+        ops.mx4_linear(x, w[0])
+    with pytest.raises(TypeError, match='weight'):
+        ops.mx4_linear(x, w.double())
+    with pytest.raises(TypeError, match='weight'):
+        ops.mx4_linear(x, [w])
+    with pytest.raises(ValueError, match='weight on cpu'):
+        ops.mx4_linear(x, w.cpu())
+    with pytest.raises(ValueError, match='bias'):
+        ops.mx4_linear(x, w, torch.zeros(7, device='cuda'))
+    with pytest.raises(TypeError, match='bias'):
+        ops.mx4_linear(x, w, torch.zeros(8, device='cuda').double())
     with pytest.raises(ValueError, match='do not match'):
         ops.mx4_linear(x[:, :63], qd)
     with pytest.raises(TypeError, match='Double'):
@@ -383,3 +398,61 @@ def test_refusals():
     with pytest.raises(ValueError, match='does not match'):
         ext.mx4_linear_backward(torch.randn(4, 7, device='cuda'), qd.codes,
                                 qd.scales, None, None, 64, 0, -1, -1)
+
+
+@pytest.mark.parametrize('held', [False, True])
+@pytest.mark.parametrize('wants', ['x', 'b', 'xb', 'w', 'xw', 'wb', 'xwb'])
+def test_each_set_of_leaves_has_its_gradients(held, wants):
+    if held and 'w' in wants:
+        pytest.skip('held weights have no gradient')
+    M, K, N = 70, 136, 40
+    x, b = torch.randn(2, M // 2, K), torch.randn(N)
+    w, g = torch.randn(N, K), torch.randn(2, M // 2, N)
+    every = {'x': x.cuda(), 'w': w.cuda(), 'b': b.cuda().bfloat16()}
+    leaves = [every[c].requires_grad_() for c in wants]
+    weight = ops.mx4_quantize(every['w']) if held else every['w']
+    y = ops.mx4_linear(every['x'], weight, every['b'])
+    assert torch.equal(
+        y, ops.mx4_linear(every['x'].detach(),
+                          weight if held else weight.detach(),
+                          every['b'].detach()))
+    got = dict(zip(wants, torch.autograd.grad(y, leaves, g.cuda())))
+    g64 = g.reshape(M, N).double()
+    xv, wv = values(x.reshape(M, K)), values(w)
+    want = {'x': (g64 @ wv, g64.abs() @ wv.abs(), N),
+            'w': (g64.t() @ xv, g64.abs().t() @ xv.abs(), M),
+            'b': (g64.sum(0), g64.abs().sum(0), M)}
+    for c in wants:
+        assert got[c].dtype == every[c].dtype and got[c].shape == every[c].shape
+        v, mass, n = want[c]
+        assert_close(got[c].reshape(v.shape), v, mass, n)
+    with pytest.raises(RuntimeError):       # its tensors are freed
+        torch.autograd.grad(y, leaves, g.cuda())
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 64, device='cuda', requires_grad=True)
+    w = torch.randn(8, 64, device='cuda', requires_grad=True)
+    g = torch.randn(4, 8, device='cuda', requires_grad=True)
+    dx, dw = torch.autograd.grad(ops.mx4_linear(x, w), (x, w), g,
+                                 create_graph=True)
+    for d in (dx, dw):
+        with pytest.raises(RuntimeError, match='once'):
+            d.sum().backward(retain_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(d.sum(), g, retain_graph=True)
+
+
+def test_checkpointing_and_saved_tensor_hooks():
+    from torch.utils.checkpoint import checkpoint
+    x = torch.randn(96, 128, device='cuda', requires_grad=True)
+    w = torch.randn(64, 128, device='cuda', requires_grad=True)
+    want = torch.autograd.grad(ops.mx4_linear(x, w).square().sum(), (x, w))
+    y = checkpoint(lambda a, b: ops.mx4_linear(a, b).square(), x, w,
+                   use_reentrant=False)
+    for a, b in zip(torch.autograd.grad(y.sum(), (x, w)), want):
+        assert torch.equal(a, b)
+    with torch.autograd.graph.save_on_cpu():
+        y = ops.mx4_linear(x, w).square()
+    for a, b in zip(torch.autograd.grad(y.sum(), (x, w)), want):
+        assert torch.equal(a, b)
