@@ -16,16 +16,26 @@ struct Item {            // one dense tensor; dtypes as in mx4_common.h
 
 enum Norm : int { L2 = 0, L1 = 1, LINF = 2 };
 
-// doubles that a call wants
-size_t workspace_doubles(const std::vector<Item>& items);
+// A list, laid out for its launches.
+class List {
+public:
+    explicit List(const std::vector<Item>& items);
+    ~List();
+    List(const List&) = delete;
+    List& operator=(const List&) = delete;
 
-// norm[0] = the norm; work[0] = the factor min(1, max_norm / (norm + 1e-6)),
-// where max_norm >= 0
-void norm(const std::vector<Item>& items, int kind, double max_norm,
-          float* norm, double* work, hipStream_t stream);
+    // doubles that a call wants
+    size_t workspace_doubles() const;
+    // norm[0] = the norm
+    void norm(int kind, float* norm, double* work, hipStream_t stream) const;
+    // the same, and dst = src * min(1, max_norm / (norm + 1e-6)), max_norm >= 0
+    void clip(int kind, double max_norm, float* norm, double* work,
+              hipStream_t stream) const;
 
-// dst = src * work[0], after norm()
-void scale(const std::vector<Item>& items, const double* work,
-           hipStream_t stream);
+private:
+    struct Data;
+    Data* d;
+    int sums(int kind, double* part, hipStream_t stream) const;
+};
 
 }  // namespace gradclip

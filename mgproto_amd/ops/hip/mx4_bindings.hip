@@ -465,10 +465,11 @@ Tensor grad_norm(const std::vector<Tensor>& grads, double p) {
         items.push_back({c.data_ptr(), nullptr, c.numel(), dt, dt});
     }
     auto norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-    auto work = at::empty({(int64_t)gradclip::workspace_doubles(items)},
+    const gradclip::List list(items);
+    auto work = at::empty({(int64_t)list.workspace_doubles()},
                           norm.options().dtype(at::kDouble));
-    gradclip::norm(items, kind, 0.0, norm.data_ptr<float>(),
-                   work.data_ptr<double>(), current_stream());
+    list.norm(kind, norm.data_ptr<float>(), work.data_ptr<double>(),
+              current_stream());
     return norm;
 }
 
@@ -507,12 +508,11 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
     }
     check_apart(items);
     auto norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-    auto work = at::empty({(int64_t)gradclip::workspace_doubles(items)},
+    const gradclip::List list(items);
+    auto work = at::empty({(int64_t)list.workspace_doubles()},
                           norm.options().dtype(at::kDouble));
-    const hipStream_t stream = current_stream();
-    gradclip::norm(items, kind, max_norm, norm.data_ptr<float>(),
-                   work.data_ptr<double>(), stream);
-    gradclip::scale(items, work.data_ptr<double>(), stream);
+    list.clip(kind, max_norm, norm.data_ptr<float>(), work.data_ptr<double>(),
+              current_stream());
     for (const auto& o : outs)           // written behind autograd's back
         if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     return norm;

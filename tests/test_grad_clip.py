@@ -210,3 +210,32 @@ def test_version_counter():
     v = t._version
     ops.clip_grads_([t], 0.1)
     assert t._version > v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('sizes', [
+    [4095, 4096, 4097, 12288] * 3,             # pieces that end on a border
+    [9000001, 5, 3000000, 1],                  # more pieces than blocks
+    [30000 + i % 5 for i in range(560)],       # several launches, many sums
+], ids=['borders', 'long', 'many'])
+def test_long_lists_of_every_type(sizes):
+    src = [torch.randn(n, device='cuda').to(DTYPES[i % 3])
+           for i, n in enumerate(sizes)]
+    norm = math.sqrt(sum(float(t.double().square().sum()) for t in src))
+    flat = torch.full((sum(sizes) + 2,), 7.0, device='cuda',
+                      dtype=torch.bfloat16)
+    outs = list(flat[1:-1].split(sizes))
+    assert float(ops.clip_grads_(src, 0.5 * norm, out=outs)) == pytest.approx(
+        norm, rel=2.0 ** -23)
+    # the factor, the product in fp32, the rounding
+    near = lambda o, t, h: ((o.double() - t.double() / 2).abs() <= (  # noqa: E731
+        h + 2.0 ** -22) * t.double().abs() / 2 + torch.finfo(
+            o.dtype).smallest_normal * 2 * h).all()
+    assert all(near(o, t, 2.0 ** -8) for o, t in zip(outs, src))
+    assert flat[0] == 7 and flat[-1] == 7
+    again = [t.clone() for t in src]
+    ops.clip_grads_(again, 0.5 * norm)
+    assert all(near(o, t, torch.finfo(t.dtype).eps / 2)
+               for o, t in zip(again, src))
+    assert torch.equal(ops.grad_norm(src),
+                       ops.clip_grads_(src, 2 * norm, out=outs))
