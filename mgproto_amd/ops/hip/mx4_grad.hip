@@ -226,18 +226,12 @@ Sums sums(long M, long N) {
 struct Small {
     const void* g;
     long M, N, K;
-    int g_dt;
     const uint8_t *wc, *ws, *xc, *xs;    // of the results that are wanted
     void *dx, *dw, *db;
     int dx_dt, dw_dt, db_dt;
     int dx_blocks, dw_blocks, kb;        // kb: blocks along K
 };
 
-static __device__ __forceinline__ float load_g(const Small& a, long i) {
-    if (a.g_dt == F32) return reinterpret_cast<const float*>(a.g)[i];
-    if (a.g_dt == BF16) return (float)reinterpret_cast<const __bf16*>(a.g)[i];
-    return (float)reinterpret_cast<const _Float16*>(a.g)[i];
-}
 static __device__ __forceinline__ void store_any(void* p, int dt, long i, float v) {
     if (dt == F32) reinterpret_cast<float*>(p)[i] = v;
     else if (dt == BF16) reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
@@ -248,16 +242,18 @@ static __device__ __forceinline__ void store_any(void* p, int dt, long i, float 
 // lanes take 8 columns each, the 32 groups of them every 32nd b, joined in
 // order. g(a, b) lies at a * ga + b * gb.
 constexpr int SA = 4;
+template <int DT>
 static __device__ void small_product(const Small& p, long A, long B, long ga,
                                      long gb, const uint8_t* codes,
                                      const uint8_t* scales, void* out, int dt,
                                      int block) {
+    const typename Elem<DT>::T* g = (const typename Elem<DT>::T*)p.g;
     __shared__ float red[32][SA][65];
     const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
     const long a0 = (long)(block / p.kb) * SA, k = (long)(block % p.kb) * 64 + x * 8;
     float v[SA][8] = {};
     if (k < p.K) {
-        #pragma unroll 4
+        #pragma unroll 8
         for (long b = y; b < B; b += 32) {
             const unsigned c = reinterpret_cast<const unsigned*>(codes)[
                 ((size_t)(k >> 7) * B + b) * 16 + (k >> 3 & 15)];
@@ -265,7 +261,7 @@ static __device__ void small_product(const Small& p, long A, long B, long ga,
             float gv[SA], f[8];
             #pragma unroll
             for (int i = 0; i < SA; ++i)
-                gv[i] = load_g(p, min(a0 + i, A - 1) * ga + b * gb);
+                gv[i] = (float)g[min(a0 + i, A - 1) * ga + b * gb];
             values8(c, byte, f);
             #pragma unroll
             for (int i = 0; i < SA; ++i)
@@ -288,33 +284,37 @@ static __device__ void small_product(const Small& p, long A, long B, long ga,
     store_any(out, dt, a * p.K + kk, s);
 }
 
+template <int DT>
 __global__ __launch_bounds__(256)
 void small_grads_kernel(const Small p) {
     int block = blockIdx.x;
     if (block < p.dx_blocks) {
-        small_product(p, p.M, p.N, p.N, 1, p.wc, p.ws, p.dx, p.dx_dt, block);
+        small_product<DT>(p, p.M, p.N, p.N, 1, p.wc, p.ws, p.dx, p.dx_dt, block);
         return;
     }
     block -= p.dx_blocks;
     if (block < p.dw_blocks) {
-        small_product(p, p.N, p.M, 1, p.N, p.xc, p.xs, p.dw, p.dw_dt, block);
+        small_product<DT>(p, p.N, p.M, 1, p.N, p.xc, p.xs, p.dw, p.dw_dt, block);
         return;
     }
     block -= p.dw_blocks;
-    // 64 columns, every fourth row a wave
-    __shared__ float red[4][64];
-    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
-    const long n = (long)block * 64 + lane;
+    // 8 columns, every 32nd row a group of lanes
+    __shared__ float red[32][9];
+    const typename Elem<DT>::T* g = (const typename Elem<DT>::T*)p.g;
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
+    const long n = (long)block * 8 + x;
     float v = 0.f;
     if (n < p.N) {
-        #pragma unroll 4
-        for (long m = q; m < p.M; m += 4) v += load_g(p, m * p.N + n);
+        #pragma unroll 8
+        for (long m = y; m < p.M; m += 32) v += (float)g[m * p.N + n];
     }
-    red[q][lane] = v;
+    red[y][x] = v;
     __syncthreads();
-    if (q == 0 && n < p.N)
-        store_any(p.db, p.db_dt, n, (red[0][lane] + red[1][lane])
-                                    + (red[2][lane] + red[3][lane]));
+    if (y || n >= p.N) return;
+    float s = 0.f;
+    #pragma unroll
+    for (int k = 0; k < 32; ++k) s += red[k][x];
+    store_any(p.db, p.db_dt, n, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -330,11 +330,15 @@ bool dw_in_place(const GradArgs& a) {
     return a.g_dt == BF16 && a.aligned && a.N % 8 == 0;
 }
 
-// One launch against five to nine of 4 us: the plain arithmetic keeps up to
-// 2^24 multiplications (83x200x65 fp32: 13 us of backward against 42; 2^25, as
-// 3136x128x64, 28 against 31).
+// One launch against five to nine of 4 us. All three gradients in us, MxKxN:
+// 83x200x65 fp32 6.5 against 34, 512x512x512 bf16 21 against 44, 1024x512x512 37
+// against 47 (700^3 45 against 60, but 49 without db). A lane's sum over every 32nd
+// row is a chain of loads, so long sums go to the tiles: 1500x64x64 bf16 17
+// against 25, 3136x64x64 34 against 24. Wider types are cut into parts first
+// there: 2048x256x256 fp32 21 against 59, 4000x128x256 54 against 55.
 bool small(const GradArgs& a) {
-    return (double)a.M * a.N * a.K <= 0x1p24 && std::max(a.M, a.N) <= 4096;
+    return (double)a.M * a.N * a.K <= 0x1p28 &&
+           std::max(a.M, a.N) <= (a.g_dt == BF16 ? 1536 : 2560);
 }
 
 template <bool STEPPED>
@@ -448,14 +452,18 @@ size_t grads_bytes(const GradArgs& a, int form) {
 
 void grads(const GradArgs& a, int form, void* work, hipStream_t stream) {
     if (form < 0 ? small(a) : form == 0) {
-        Small p{a.g, a.M, a.N, a.K, a.g_dt, a.wc, a.ws, a.xc, a.xs, a.dx, a.dw,
+        Small p{a.g, a.M, a.N, a.K, a.wc, a.ws, a.xc, a.xs, a.dx, a.dw,
                 a.db, a.dx_dt, a.dw_dt, a.db_dt, 0, 0, (int)((a.K + 63) / 64)};
         p.dx_blocks = a.dx ? (int)((a.M + SA - 1) / SA) * p.kb : 0;
         p.dw_blocks = a.dw ? (int)((a.N + SA - 1) / SA) * p.kb : 0;
-        const int db = a.db ? (int)((a.N + 63) / 64) : 0;
-        hipLaunchKernelGGL(small_grads_kernel,
-                           dim3((unsigned)(p.dx_blocks + p.dw_blocks + db)),
-                           dim3(256), 0, stream, p);
+        const int db = a.db ? (int)((a.N + 7) / 8) : 0;
+        const dim3 grid((unsigned)(p.dx_blocks + p.dw_blocks + db));
+        #define MX4_S(DT) \
+            hipLaunchKernelGGL((small_grads_kernel<DT>), grid, dim3(256), 0, stream, p)
+        if (a.g_dt == F32) MX4_S(F32);
+        else if (a.g_dt == BF16) MX4_S(BF16);
+        else MX4_S(F16);
+        #undef MX4_S
         return;
     }
     if (a.dx) run_dx(a, (char*)work, stream);
