@@ -182,16 +182,21 @@ union Piece {
     T v[W];
     Word u[W * sizeof(T) / B];
 };
-// whole where n >= W elements are left for it, wherever q points
-template <class T, int W>
+// Whole where n >= W elements are left for it, wherever q points. STREAM: past
+// the caches, for rows that are written in one go (where a row is written in
+// parts, the L2 has to gather them: 62720x1024->256 took 42 us for 38 with it).
+template <bool STREAM = false, class T, int W>
 static __device__ __forceinline__ void store_piece(T* q, const Piece<T, W>& o,
                                                    long n) {
     using P = Piece<T, W>;
-    struct __attribute__((packed, aligned(sizeof(T)))) Any { typename P::Word u; };
+    typedef typename P::Word Loose __attribute__((aligned(sizeof(T))));
     if (n >= W) {
+        Loose* to = reinterpret_cast<Loose*>(q);
         #pragma unroll
-        for (int i = 0; i < (int)(W * sizeof(T)) / P::B; ++i)
-            reinterpret_cast<Any*>(q)[i].u = o.u[i];
+        for (int i = 0; i < (int)(W * sizeof(T)) / P::B; ++i) {
+            if constexpr (STREAM) __builtin_nontemporal_store(o.u[i], to + i);
+            else to[i] = o.u[i];
+        }
     } else {
         #pragma unroll
         for (int e = 0; e < W; ++e)

@@ -4,7 +4,10 @@
 // reading back. Four lanes share a block, 8 elements each, and its maximum goes
 // over them by two lane exchanges. A wave takes 512 elements of a row (or 128
 // of four rows, where rows are that short), so that it reads in pieces of 1 KB
-// or more, and four such pieces at once to have enough loads under way.
+// or more, and four such pieces at once to have enough loads under way. Values
+// read back go out past the caches (250880x512 62 -> 47 us), unless pieces of two
+// rows share 16 bytes (62720x1023 26 -> 32).
+// 62720x1024 bf16: rounded in 24 us, read back in 24 (6.7 TB/s each).
 
 #include <hip/hip_runtime.h>
 
@@ -101,6 +104,7 @@ void dequantize_kernel(const uint8_t* __restrict__ codes,
     const int chunk = (int)(wave % chunks);
     const long row0 = wave / chunks * (RPW * ROWS) + lane / LPR;
     const int k = chunk * 512 + sub * 8;
+    const bool whole = K % 8 == 0;
     if (k >= K) return;
     unsigned c[ROWS], byte[ROWS];
     #pragma unroll
@@ -119,7 +123,8 @@ void dequantize_kernel(const uint8_t* __restrict__ codes,
         values8(c[i], byte[i], f);
         #pragma unroll
         for (int e = 0; e < 8; ++e) o.v[e] = from_f32<DT>(f[e]);
-        store_piece(out + row * K + k, o, K - k);
+        if (whole) store_piece<true>(out + row * K + k, o, K - k);
+        else store_piece(out + row * K + k, o, K - k);
     }
 }
 
