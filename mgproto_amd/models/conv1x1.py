@@ -13,6 +13,7 @@ reference behavior.
 """
 
 import os
+import weakref
 
 import torch
 import torch.nn as nn
@@ -70,12 +71,20 @@ class GemmConv2d(nn.Conv2d):
 
     # ------------------------------------------------------------ 4-bit form
     def _mx4_pack(self):
-        w = self.weight.detach()
-        q = ops.mx4_quantize(w.reshape(self.out_channels, -1))
-        # not in the state dict: made from the weight again where that changes
-        self.register_buffer('_mx4_codes', q.codes, persistent=False)
-        self.register_buffer('_mx4_scales', q.scales, persistent=False)
-        self._mx4_version = _version(self.weight)
+        # tensors of the ordinary kind whatever mode the caller is in
+        with torch.inference_mode(False), torch.no_grad():
+            q = ops.mx4_quantize(self.weight.reshape(self.out_channels, -1))
+            old = getattr(self, '_mx4_codes', None)
+            if (old is not None and old.shape == q.codes.shape
+                    and old.device == q.device):
+                # in place: a captured graph reads them where they are
+                old.copy_(q.codes)
+                self._mx4_scales.copy_(q.scales)
+            else:
+                # not in the state dict: made from the weight again
+                self.register_buffer('_mx4_codes', q.codes, persistent=False)
+                self.register_buffer('_mx4_scales', q.scales, persistent=False)
+        self._mx4_of = weakref.ref(self.weight), _state(self.weight)
 
     def _mx4_weight(self):
         if self.mx4 == 'train':
@@ -85,10 +94,18 @@ class GemmConv2d(nn.Conv2d):
             raise RuntimeError(
                 'this 1x1 convolution holds its weight in 4 bits and cannot '
                 'train it: use_mx4(model, train=True), or freeze the weight')
-        if self._mx4_version != _version(self.weight):
+        made_of, state = self._mx4_of
+        if made_of() is not self.weight or state != _state(self.weight):
             self._mx4_pack()
         return ops.MX4Tensor(self._mx4_codes, self._mx4_scales,
                              (self.out_channels, self.in_channels))
+
+    def __getstate__(self):
+        # copies and files: rounded again from the weight that they hold
+        state = self.__dict__.copy()
+        if '_mx4_of' in state:
+            state['_mx4_of'] = _nothing, None
+        return state
 
     def _mx4_forward(self, x):
         kind = x.device.type
@@ -101,8 +118,12 @@ class GemmConv2d(nn.Conv2d):
         return y.permute(0, 3, 1, 2)                   # channels_last NCHW
 
 
-def _version(w: torch.Tensor) -> int:
-    return -1 if w.is_inference() else w._version
+def _state(w: torch.Tensor):
+    return w.dtype, -1 if w.is_inference() else w._version
+
+
+def _nothing():
+    """In the place of a reference to a weight."""
 
 
 def use_mx4(module: nn.Module, train: bool = False) -> int:
@@ -111,8 +132,11 @@ def use_mx4(module: nn.Module, train: bool = False) -> int:
     channels, fp32 sums). Returns how many there are.
 
     ``train=False`` rounds the weights now and holds them in 4 bits, for
-    inference; a later in-place update of a weight (an optimizer's, or
-    ``load_state_dict``) rounds it again, one through ``.data`` is not seen.
+    inference. The forward that follows an update of a weight (an optimizer's,
+    ``load_state_dict``'s, another parameter in its place) rounds it again; an
+    update through ``.data`` is not seen, nor is any by the replay of a captured
+    graph, until ``use_mx4`` is called again, which writes the new codes in the
+    place of the old ones.
     ``train=True`` rounds them in every forward, with straight-through
     gradients to the float weights: fine-tuning for the former. The state dict
     stays what it was either way. ``use_mx4(model.features)`` leaves the
@@ -133,7 +157,7 @@ def no_mx4(module: nn.Module):
     for m in module.modules():
         if isinstance(m, GemmConv2d) and m.mx4 is not None:
             if m.mx4 == 'held':
-                del m._mx4_codes, m._mx4_scales
+                del m._mx4_codes, m._mx4_scales, m._mx4_of
             m.mx4 = None
 
 

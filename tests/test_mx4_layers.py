@@ -2,6 +2,7 @@
 layers, trainer, serving."""
 
 import copy
+import io
 import json
 import os
 import subprocess
@@ -101,6 +102,63 @@ def test_held_weights_follow_the_float_ones():
     xg = x.clone().requires_grad_()
     conv(xg).sum().backward()               # the input's gradient is there
     assert xg.grad.abs().sum() > 0 and conv.weight.grad is None
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_no_stale_codes(device):
+    """Other parameters of the same version, copies and files of a layer whose
+    weight changed after its codes were made."""
+    conv = GemmConv2d(32, 8, 1).to(device)
+    use_mx4(conv)
+    x = torch.randn(1, 32, 2, 2, device=device)
+
+    def check(c):
+        with torch.no_grad():
+            want, mass = _want(c, x)
+            assert_close(c(x), want, mass, 33)
+
+    other = GemmConv2d(32, 8, 1).to(device)
+    assert other.weight._version == conv.weight._version
+    conv.load_state_dict(other.state_dict(), assign=True)
+    check(conv)
+    conv.weight = torch.nn.Parameter(torch.randn_like(conv.weight))
+    check(conv)
+    with torch.no_grad():
+        conv.weight.mul_(-3)
+    again = copy.deepcopy(conv)
+    check(again)
+    f = io.BytesIO()
+    torch.save(conv, f)
+    f.seek(0)
+    check(torch.load(f, weights_only=False))
+    conv.to(torch.bfloat16)
+    x = x.bfloat16()
+    check(conv)
+    with torch.inference_mode():
+        conv.weight.mul_(2)
+        conv(x)
+    check(conv)
+    with torch.inference_mode():
+        late = GemmConv2d(32, 8, 1).to(device).bfloat16()
+        use_mx4(late)
+    assert not late._mx4_codes.is_inference()
+
+
+@pytest.mark.gpu
+def test_a_captured_layer_takes_new_codes():
+    conv = GemmConv2d(32, 8, 1).cuda()
+    use_mx4(conv)
+    x = torch.randn(2, 32, 3, 3, device='cuda')
+    with torch.no_grad():
+        conv(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = conv(x)
+        for k in range(3):
+            conv.weight.normal_()
+            use_mx4(conv)
+            graph.replay()
+            assert torch.equal(y, conv(x))
 
 
 @pytest.mark.parametrize('device', DEVICES)
