@@ -28,6 +28,8 @@ void refuse_unless(bool ok, A&&... what) {
 #define CHECK_VALUE(ok, ...) refuse_unless<py::value_error>(ok, __VA_ARGS__)
 
 int dtype_code(const Tensor& t, const char* what) {
+    CHECK_TYPE(!t.is_neg(), what, ": a view that stands for its negative; "
+               "resolve_neg() it first");
     switch (t.scalar_type()) {
         case at::kFloat: return mx4::F32;
         case at::kBFloat16: return mx4::BF16;
@@ -55,6 +57,8 @@ Tensor matrix(const Tensor& x, const char* what) {
     CHECK_VALUE(K < (1L << 22), what, ": rows of at most 2^22 elements");
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
+    // 64 rows a block, at the least, and 2^32 threads a launch
+    CHECK_VALUE(M < (1L << 29), what, ": fewer than 2^29 rows");
     Tensor x2 = x.dim() == 2 ? x : x.reshape({M, K});
     if ((K > 1 && x2.stride(1) != 1) || (M > 1 && x2.stride(0) < K))
         x2 = x2.contiguous();
@@ -145,15 +149,18 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
     return out;
 }
 
-// what blocks of 16 x 16 results can number
-void check_tiles(int64_t M, int64_t N) {
-    CHECK_VALUE((M + 15) / 16 * ((N + 15) / 16) < (1L << 31), "mx4_linear: ",
-                M, " x ", N, " results are too many");
-}
-
-int pick(int64_t form, int chosen) {
+// The form that is asked for, or the chosen one. A launch has 2^32 threads at
+// most; forms of small blocks have one for each 16 x 16 or 32 x 32 results.
+int pick(int64_t form, int chosen, int64_t M, int64_t N) {
     CHECK_VALUE(form >= -1 && form < mx4::FORMS, "mx4_linear: no form ", form);
-    return form < 0 ? chosen : (int)form;
+    const int f = form < 0 ? chosen : (int)form;
+    const bool small = f == mx4::ROWS16 || f == mx4::HELD16;
+    const bool tiles = f == mx4::TILES128 || f == mx4::TILES256;
+    const int64_t t = small ? 16 : f == mx4::ROUNDING ? 64 : 32;
+    CHECK_VALUE((tiles || (M + t - 1) / t * ((N + t - 1) / t) < (1L << 24)) &&
+                    (M + 127) / 128 * ((N + 127) / 128) < (1L << 30),
+                "mx4_linear: ", M, " x ", N, " results are too many");
+    return f;
 }
 
 struct Bias {            // contiguous, and its type
@@ -179,7 +186,6 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws, int64_t K,
                 ", weight on ", wc.device());
     check_packed(wc, ws, K, "mx4_linear: weight");
     check_bias(bias, N, x);
-    check_tiles(M, N);
     c10::DeviceGuard guard(x.device());
     auto y = at::empty(shape_of(x, N), x.options());
     if (!M || !N) return y;
@@ -187,7 +193,7 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws, int64_t K,
     const int64_t ldx = row_stride(x2);
     const bool aligned = (uintptr_t)x2.data_ptr() % 16 == 0 &&
                          ldx * x2.element_size() % 16 == 0;
-    const int f = pick(form, mx4::linear_form(M, K, N, aligned));
+    const int f = pick(form, mx4::linear_form(M, K, N, aligned), M, N);
     Tensor work;
     if (const size_t bytes = mx4::linear_bytes(f, M, K))
         work = workspace(bytes, x);
@@ -202,12 +208,11 @@ Tensor product_q(const Tensor& xc, const Tensor& xs, int64_t K,
                  std::vector<int64_t> shape, int dt, int64_t form) {
     const int64_t M = xc.size(1), N = wc.size(1);
     check_bias(bias, N, xc);
-    check_tiles(M, N);
     auto y = at::empty(shape, xc.options().dtype(scalar_type(dt)));
     if (!M || !N) return y;
     const Bias b(bias);
-    const int f = std::max(pick(form, mx4::linear_q_form(M, K, N)),
-                           (int)mx4::HELD16);
+    const int chosen = mx4::linear_q_form(M, K, N);
+    const int f = pick(form < 0 || form >= mx4::HELD16 ? form : chosen, chosen, M, N);
     mx4::linear_q(xc.data_ptr<uint8_t>(), xs.data_ptr<uint8_t>(), M, K,
                   wc.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), N, b.ptr(),
                   b.dt, y.data_ptr(), dt, f, current_stream());
@@ -265,15 +270,19 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
     a.g_dt = dtype_code(grad, "mx4_linear: output gradient");
     a.N = grad.size(-1), a.M = 1, a.K = K;
     for (int64_t i = 0; i + 1 < grad.dim(); ++i) a.M *= grad.size(i);
-    CHECK_VALUE(a.M < (1L << 31) && a.N < (1L << 22),
-                "mx4_linear: output gradient: too large");
+    CHECK_VALUE(a.M < (1L << 29) && a.N < (1L << 22) && K >= 0 &&
+                    K < (1L << 22), "mx4_linear: output gradient: too large");
     if (dx_dt >= 0) {
+        CHECK_VALUE(wc.has_value() && ws.has_value(),
+                    "mx4_linear: no weight for the input's gradient");
         check_packed(*wc, *ws, K, "mx4_linear: weight");
         CHECK_VALUE(wc->size(1) == a.N && grad.device() == wc->device(),
                     "mx4_linear: output gradient does not match the weight");
         a.wc = wc->data_ptr<uint8_t>(), a.ws = ws->data_ptr<uint8_t>();
     }
     if (dw_dt >= 0) {
+        CHECK_VALUE(xc.has_value() && xs.has_value(),
+                    "mx4_linear: no rows for the weight's gradient");
         check_packed(*xc, *xs, K, "mx4_linear: input");
         CHECK_VALUE(xc->size(1) == a.M && grad.device() == xc->device(),
                     "mx4_linear: output gradient does not match the input");

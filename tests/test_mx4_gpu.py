@@ -395,6 +395,22 @@ def test_refusals():
         ext.mx4_linear(x, qd.codes[:, :, ::2], qd.scales, 64, None)
     with pytest.raises(ValueError, match='no form'):
         ext.mx4_linear(x, qd.codes, qd.scales, 64, None, 7)
+    with pytest.raises(ValueError, match='2\\^29 rows'):
+        ops.mx4_quantize(x[:1, :1].expand(2 ** 29, 1))
+    with pytest.raises(ValueError, match='2\\^22 elements'):
+        ops.mx4_linear(x[:1, :1].expand(1, 2 ** 22), qd)
+    neg = torch.complex(x, x).conj().imag
+    assert neg.is_neg()
+    with pytest.raises(TypeError, match='resolve_neg'):
+        ops.mx4_linear(neg, qd)
+    assert torch.equal(ops.mx4_linear(neg.resolve_neg(), qd),
+                       ops.mx4_linear(-x, qd))
+    with pytest.raises(TypeError, match='resolve_neg'):
+        ops.grad_norm([neg])
+    with pytest.raises(ValueError, match='no weight'):
+        ext.mx4_linear_backward(x, None, None, None, None, 64, 0, -1, -1)
+    with pytest.raises(ValueError, match='no rows'):
+        ext.mx4_linear_backward(x, None, None, None, None, 64, -1, 0, -1)
     with pytest.raises(ValueError, match='does not match'):
         ext.mx4_linear_backward(torch.randn(4, 7, device='cuda'), qd.codes,
                                 qd.scales, None, None, 64, 0, -1, -1)
