@@ -191,9 +191,7 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws, int64_t K,
     if (!M || !N) return y;
     const Bias b(bias);
     const int64_t ldx = row_stride(x2);
-    const bool aligned = (uintptr_t)x2.data_ptr() % 16 == 0 &&
-                         ldx * x2.element_size() % 16 == 0;
-    const int f = pick(form, mx4::linear_form(M, K, N, aligned), M, N);
+    const int f = pick(form, mx4::linear_form(M, K, N), M, N);
     Tensor work;
     if (const size_t bytes = mx4::linear_bytes(f, M, K))
         work = workspace(bytes, x);

@@ -236,7 +236,7 @@ void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
 enum Form : int {
     ROWS16 = 0,       // 16 x 16 of y a block, x rounded by each block
     ROWS32 = 1,       // 32 x 32, the same
-    ROUNDING = 2,     // tiles of 128 rows, x rounded on its way into LDS
+    ROUNDING = 2,     // tiles of 64 rows, x rounded on its way into LDS
     HELD16 = 3,       // x rounded before; then the same from 4-bit rows,
     HELD32 = 4,
     TILES128 = 5,     // or tiles of them
@@ -245,7 +245,7 @@ enum Form : int {
 };
 
 // y[M,N] = Q(x) W^T + bias
-int linear_form(long M, long K, long N, bool aligned);
+int linear_form(long M, long K, long N);
 size_t linear_bytes(int form, long M, long K);        // of workspace
 void linear(const void* x, int dt, long M, long K, long ldx,
             const uint8_t* wc, const uint8_t* ws, long N, const void* bias,

@@ -42,10 +42,13 @@ static __device__ __forceinline__ i32x4 round_block(
     return c;
 }
 
-// FM x FN tiles of 16 x 16 a block. Its four waves take every fourth step of
-// 128 each and are joined in LDS, in their order.
-template <int AT, int OT, int FM, int FN>
-__global__ __launch_bounds__(256)
+// FM x FN tiles of 16 x 16 a block. Its WV waves take every WVth step of 128 each
+// and are joined in LDS, in their order. One row is bound by the weights' way from
+// memory: 1x4096->4096 (9 MB) takes 4.0 us where the caches hold them, 6.1 where
+// not (four waves: 4.9 and 8.7; 16: 4.3 and 5.6), 1x16384->4096 11 and 15 (20 and
+// 25).
+template <int AT, int OT, int FM, int FN, int WV>
+__global__ __launch_bounds__(64 * WV)
 void linear_rows_kernel(const void* __restrict__ xv,
                         const uint8_t* __restrict__ xs, long M, int K, int steps,
                         long ldx, const uint8_t* __restrict__ wc,
@@ -74,7 +77,7 @@ void linear_rows_kernel(const void* __restrict__ xv,
         #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
 
-    for (int s = wave; s < steps; s += 4) {
+    for (int s = wave; s < steps; s += WV) {
         i32x4 w[FN], x[FM];
         int wb[FN], xb[FM];
         #pragma unroll
@@ -104,7 +107,7 @@ void linear_rows_kernel(const void* __restrict__ xv,
                     wide(w[j]), wide(x[i]), acc[i][j], 4, 4, 0, wb[j], 0, xb[i]);
     }
 
-    __shared__ f32x4 part[3][FM * FN][64];
+    __shared__ f32x4 part[WV - 1][FM * FN][64];
     if (wave) {
         #pragma unroll
         for (int i = 0; i < FM; ++i)
@@ -115,7 +118,7 @@ void linear_rows_kernel(const void* __restrict__ xv,
     __syncthreads();
     if (wave) return;
     #pragma unroll
-    for (int p = 0; p < 3; ++p)
+    for (int p = 0; p < WV - 1; ++p)
         #pragma unroll
         for (int i = 0; i < FM; ++i)
             #pragma unroll
@@ -131,14 +134,15 @@ void launch_rows(const void* x, const uint8_t* xs, long M, long K, long ldx,
                  const uint8_t* wc, const uint8_t* ws, long N,
                  const void* bias, int bias_dt, void* y, int form,
                  hipStream_t stream) {
-    #define MX4_L(F) do { \
+    #define MX4_L(F, WV) do { \
         const long mt = (M + 16 * F - 1) / (16 * F), nt = (N + 16 * F - 1) / (16 * F); \
-        hipLaunchKernelGGL((linear_rows_kernel<AT, OT, F, F>), \
-            dim3((unsigned)(mt * nt)), dim3(256), 0, stream, x, xs, M, (int)K, \
+        hipLaunchKernelGGL((linear_rows_kernel<AT, OT, F, F, WV>), \
+            dim3((unsigned)(mt * nt)), dim3(64 * WV), 0, stream, x, xs, M, (int)K, \
             (int)steps_of(K), ldx, wc, ws, N, bias, bias_dt, (typename Elem<OT>::T*)y, \
             (int)nt); } while (0)
-    if (form == ROWS16 || form == HELD16) MX4_L(1);
-    else MX4_L(2);
+    if (form != ROWS16 && form != HELD16) MX4_L(2, 4);
+    else if (steps_of(K) >= 8) MX4_L(1, 8);
+    else MX4_L(1, 4);
     #undef MX4_L
 }
 
@@ -146,22 +150,41 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace
 
-// The choice, by the multiplications M K N (at least 16 rows count); times in
-// us, bf16, on an MI355X.
+// The choice; times in us, bf16, on an MI355X.
 //
-// Rounding in the blocks saves a launch (4 us) and a pass over x, but every
-// block rounds its rows again: 784x1024->256 5.4 against 9.0 with the rounding
-// before, 64x4096->4096 (2^30) 12.8 against 11.5, 128x4096->4096 22 against 16.
+// Blocks of 16 x 16 where there are too few of 32 x 32 for 256 units:
+// 64x4096->1024 (64 of those) 6.7 against 12.2, 196x2048->512 (112) 6.7 against 7.5,
+// 784x1024->256 (200) 6.9 against 5.3.
+static bool small_blocks(long M, long N) {
+    return M <= 16 || (M + 31) / 32 * ((N + 31) / 32) <= 128;
+}
+
+// Rounding in the blocks saves a launch (4 us) and a pass over x, but every block
+// rounds its rows again: with few multiplications M K N (16 rows count at least)
+// 784x1024->256 takes 5.4 against 8.4 with the rounding before, 128x2048->2048
+// (2^29) 7.6 against 8.0, 196x2048->2048 12.5 against 10.0, a longer sum
+// 64x4096->2048 (2^29) 12.4 against 10.0.
 //
-// Many rows and few columns: x's way from memory counts, and tiles of 128 rows
-// round it on the way: 62720x1024->256 39 against 42, 1003520x256->64 146
-// against 208. With more columns the rows would be rounded again and again
-// (62720x512->512 43 against 36), and a short K leaves nothing to overlap
-// (1003520x64->64 167 against 87).
-int linear_form(long M, long K, long N, bool aligned) {
+// Many rows and few columns: x's way from memory counts, and tiles of 64 rows
+// round it on the way: 62720x1024->256 35 against 42, 131072x256->64 15 against
+// 24, 8192x512->256 7.7 against 10.5. There have to be blocks enough to cover a
+// long sum's waits: 8192x1024->128 10.2 against 13.0 but 8192x2048->128 22 against
+// 18, 32768x4096->128 56 against 77. With more columns x is rounded again:
+// 16384x512->512 11.6 against 15.3, 131072x512->512 74 against 69. A short sum with
+// many results is bound by their way out, where tiles of more rows do better:
+// 131072x64->256 26 against 29, but 1003520x64->256 255 against 172.
+static bool few_columns(long M, long K, long N) {
+    if (M < (K <= 512 ? 4096 : K <= 1024 ? 8192 : 32768)) return false;
+    if (N <= 64) return true;
+    if (N <= 256) return K >= 256 || M <= 131072;
+    return N <= 512 && M <= 32768 && K <= 512;
+}
+
+int linear_form(long M, long K, long N) {
+    if (few_columns(M, K, N)) return ROUNDING;
     const double work = (double)(M > 16 ? M : 16) * K * N;
-    if (work < 0x1p30) return M <= 16 ? ROWS16 : ROWS32;
-    if (aligned && M >= 4096 && N <= 256 && K >= 256) return ROUNDING;
+    if (work <= (K <= 2048 ? 0x1p29 : 0x1p28))
+        return small_blocks(M, N) ? ROWS16 : ROWS32;
     return linear_q_form(M, K, N);
 }
 
@@ -173,7 +196,7 @@ int linear_form(long M, long K, long N, bool aligned) {
 // empty, 250880x512->128 31 against 24.
 int linear_q_form(long M, long K, long N) {
     if (M <= 16) return HELD16;
-    if ((double)M * K * N <= 0x1p31) return HELD32;
+    if ((double)M * K * N <= 0x1p31) return small_blocks(M, N) ? HELD16 : HELD32;
     const long tiles = (M + 255) / 256 * ((N + 255) / 256);
     return N > 128 && tiles >= 384 ? TILES256 : TILES128;
 }

@@ -1,12 +1,17 @@
 // Products whose rows are rounded on the way: y = Q(x) W^T + bias for many rows
 // and few columns, where the time is x's way from memory.
 //
-// A block of 128 rows takes all columns it can (up to 256), so that x is read
-// and rounded once for each 256 of them. Two buffers of 256 elements: while the
+// A block of 64 rows takes all columns it can (up to 256), so that x is read and
+// rounded once for each 256 of them. Two buffers of 128 elements: while the
 // matrix cores work on one, the weights' codes go into the other past the
 // registers, and the next rows of x come into registers, are rounded there
 // (four lanes share a block, two lane exchanges for its maximum) and written as
 // codes. One barrier a buffer.
+//
+// Bound by x's way from memory: 62720x1024->256 takes 35 us (4.6 TB/s),
+// 250880x256->64 27 (6.0). Three blocks and more share a unit, so that one reads
+// while another starts or writes: tiles of 128 rows and 256 elements, one on a
+// unit, took 39 and 38. x two steps ahead: 36 and 27, 62720x512->128 18 for 16.
 
 #include <hip/hip_runtime.h>
 
@@ -26,12 +31,12 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int W = DT == F32 ? 2 : 1;
-    constexpr int UNITS = BM * 32 / THREADS;     // of 8 elements, 32 a row
+    constexpr int UNITS = BM * 16 / THREADS;     // of 8 elements, 16 a row
     constexpr int CALLS = BN / 16;               // copies of a step's codes
-    // codes of two steps; x's scale bytes: 2*g + s of a row; W's as stored
-    __shared__ __attribute__((aligned(16))) uint8_t xl[2][2][BM * 64];
-    __shared__ __attribute__((aligned(16))) uint8_t wl[2][2][BN * 64];
-    __shared__ __attribute__((aligned(16))) uint8_t xsl[2][BM * 8];
+    // codes of a step; x's scale bytes, 4 a row; W's as stored, of four steps
+    __shared__ __attribute__((aligned(16))) uint8_t xl[2][BM * 64];
+    __shared__ __attribute__((aligned(16))) uint8_t wl[2][BN * 64];
+    __shared__ __attribute__((aligned(16))) uint8_t xsl[2][BM * 4];
     __shared__ __attribute__((aligned(16))) uint8_t wsl[2][BN * 16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -45,24 +50,20 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     const long m0 = (long)(t / nt) * BM, n0 = (long)(t % nt) * BN;
     const int lastw = (int)min((long)BN, N - n0) - 1;
     const int lastx = (int)min((long)BM, M - m0) - 1;
-    const int turns = (steps + 1) >> 1;
 
     auto send_w = [&](int k, int buf) {
         #pragma unroll
-        for (int q = 0; q < 2 * CALLS / WAVES; ++q) {
-            const int call = q * WAVES + wave;
-            const int s = call / CALLS, c = call % CALLS;
-            if (2 * k + s >= steps) break;
-            const int r = c * 16 + (lane >> 2);
-            copy16_to_lds(wc + ((size_t)(2 * k + s) * N + n0) * 64,
+        for (int q = 0; q < CALLS / WAVES; ++q) {
+            const int c = q * WAVES + wave, r = c * 16 + (lane >> 2);
+            copy16_to_lds(wc + ((size_t)k * N + n0) * 64,
                           min(r, lastw) * 64 + ((lane & 3) ^ w_key<FN>(r)) * 16,
-                          lds_address(wl[buf][s]) + c * 1024);
+                          lds_address(wl[buf]) + c * 1024);
         }
-        if ((k & 1) == 0 && wave < BN / 64) {    // four steps' scales
+        if ((k & 3) == 0 && wave < BN / 64) {    // four steps' scales
             const int r = wave * 64 + lane;
-            copy16_to_lds(ws + ((size_t)(k >> 1) * N + n0) * 16,
+            copy16_to_lds(ws + ((size_t)(k >> 2) * N + n0) * 16,
                           min(r, lastw) * 16,
-                          lds_address(wsl[k >> 1 & 1]) + wave * 1024);
+                          lds_address(wsl[k >> 2 & 1]) + wave * 1024);
         }
     };
     u32x4 raw[UNITS][W];
@@ -70,8 +71,8 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     auto load_x = [&](int k) {
         #pragma unroll
         for (int q = 0; q < UNITS; ++q) {
-            const int u = q * THREADS + tid, r = u >> 5;
-            const int at = k * 256 + (u & 31) * 8;
+            const int u = q * THREADS + tid, r = u >> 4;
+            const int at = k * 128 + (u & 15) * 8;
             const typename Elem<DT>::T* p = x0 + min(r, lastx) * ldx + at;
             if (at + 8 <= K) load8<DT>(p, raw[q]);
             else load8_tail<DT>(p, K - at, raw[q]);
@@ -80,13 +81,12 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     auto store_x = [&](int buf) {
         #pragma unroll
         for (int q = 0; q < UNITS; ++q) {
-            const int u = q * THREADS + tid, r = u >> 5, c8 = u & 31;
-            const int s = c8 >> 4, b = c8 >> 2 & 3;
+            const int u = q * THREADS + tid, r = u >> 4, c8 = u & 15, b = c8 >> 2;
             const unsigned byte = scale_byte<DT>(quad_max(absmax_bits<DT>(raw[q], W)));
             const unsigned c = codes8<DT>(raw[q], scale_f32(byte));
             *reinterpret_cast<unsigned*>(
-                xl[buf][s] + r * 64 + ((b ^ x_key(r)) << 4) + (c8 & 3) * 4) = c;
-            if ((c8 & 3) == 0) xsl[buf][r * 8 + 2 * b + s] = (uint8_t)byte;
+                xl[buf] + r * 64 + ((b ^ x_key(r)) << 4) + (c8 & 3) * 4) = c;
+            if ((c8 & 3) == 0) xsl[buf][r * 4 + b] = (uint8_t)byte;
         }
     };
 
@@ -99,59 +99,42 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     const int xr = wm + r16, wr = wn + (r16 >> 2) * (4 * FN) + (r16 & 3);
     const int xp = xr * 64 + ((g ^ x_key(xr)) << 4);
     const int wp = wr * 64 + ((g ^ w_key<FN>(wr)) << 4);
-    auto compute = [&](int k, int buf, auto both) {
+    auto compute = [&](int k, int buf) {
         int wb[FN], xb[FM];
+        i32x4 w[FN];
         #pragma unroll
         for (int j = 0; j < FN; ++j)
-            wb[j] = *reinterpret_cast<const unsigned short*>(
-                wsl[k >> 1 & 1] + (wr + j * 4) * 16 + g * 4 + (k & 1) * 2);
+            wb[j] = wsl[k >> 2 & 1][(wr + j * 4) * 16 + g * 4 + (k & 3)];
         #pragma unroll
-        for (int i = 0; i < FM; ++i)
-            xb[i] = *reinterpret_cast<const unsigned short*>(
-                xsl[buf] + (xr + i * 16) * 8 + 2 * g);
+        for (int i = 0; i < FM; ++i) xb[i] = xsl[buf][(xr + i * 16) * 4 + g];
         #pragma unroll
-        for (int s = 0; s < (decltype(both)::value ? 2 : 1); ++s) {
-            i32x4 w[FN];
+        for (int j = 0; j < FN; ++j)
+            w[j] = *reinterpret_cast<const i32x4*>(wl[buf] + wp + j * 256);
+        #pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const i32x4 a = *reinterpret_cast<const i32x4*>(xl[buf] + xp + i * 1024);
             #pragma unroll
             for (int j = 0; j < FN; ++j)
-                w[j] = *reinterpret_cast<const i32x4*>(wl[buf][s] + wp + j * 256);
-            #pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const i32x4 a = *reinterpret_cast<const i32x4*>(xl[buf][s] + xp + i * 1024);
-                #pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = s == 0
-                        ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                              wide(w[j]), wide(a), acc[i][j], 4, 4, 0, wb[j], 0, xb[i])
-                        : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                              wide(w[j]), wide(a), acc[i][j], 4, 4, 1, wb[j], 1, xb[i]);
-            }
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    wide(w[j]), wide(a), acc[i][j], 4, 4, 0, wb[j], 0, xb[i]);
         }
     };
-    // Waits until a buffer's bytes have arrived and no wave reads the other
-    // one any more, and sends for the next.
-    auto turn = [&](int k) {
-        wait_copies<0>();
-        __syncthreads();
-        if (k + 1 < turns) {
-            send_w(k + 1, (k + 1) & 1);
-            load_x(k + 1);
-        }
-    };
-    if (turns) {
+    if (steps) {
         send_w(0, 0);
         load_x(0);
         store_x(0);
     }
-    const int whole = steps >> 1;
-    for (int k = 0; k < whole; ++k) {
-        turn(k);
-        compute(k, k & 1, std::true_type());
-        if (k + 1 < turns) store_x((k + 1) & 1);
-    }
-    if (steps & 1) {
-        turn(whole);
-        compute(whole, whole & 1, std::false_type());
+    for (int k = 0; k < steps; ++k) {
+        // the buffer's bytes have arrived, and no wave reads the other one any
+        // more
+        wait_copies<0>();
+        __syncthreads();
+        if (k + 1 < steps) {
+            send_w(k + 1, (k + 1) & 1);
+            load_x(k + 1);
+        }
+        compute(k, k & 1);
+        if (k + 1 < steps) store_x((k + 1) & 1);
     }
 
     const long n = n0 + wn + g * (4 * FN);
@@ -179,15 +162,15 @@ void rounding(const void* x, int dt, long M, long K, long ldx,
               const uint8_t* wc, const uint8_t* ws, long N, const void* bias,
               int bias_dt, void* y, hipStream_t stream) {
     #define MX4_T(DT, BN, WM, WN) \
-        launch_rounding<DT, 128, BN, WM, WN>(x, M, K, ldx, wc, ws, N, bias, \
-                                             bias_dt, y, stream)
+        launch_rounding<DT, 64, BN, WM, WN>(x, M, K, ldx, wc, ws, N, bias, \
+                                            bias_dt, y, stream)
     #define MX4_D(BN, WM, WN) do { \
         if (dt == F32) MX4_T(F32, BN, WM, WN); \
         else if (dt == BF16) MX4_T(BF16, BN, WM, WN); \
         else MX4_T(F16, BN, WM, WN); } while (0)
-    if (N > 128) MX4_D(256, 2, 4);
-    else if (N > 64) MX4_D(128, 4, 2);
-    else MX4_D(64, 8, 1);
+    if (N > 128) MX4_D(256, 1, 4);
+    else if (N > 64) MX4_D(128, 2, 2);
+    else MX4_D(64, 4, 1);
     #undef MX4_D
     #undef MX4_T
 }
