@@ -155,22 +155,45 @@ static __device__ __forceinline__ void load8(const typename Elem<DT>::T* p,
     if constexpr (DT == F32) u[1] = a.v[1];
 }
 
-// n <= 8 elements at p, the rest zero, as codes8 takes them
+// n elements at p, eight at most, the rest zero: one load where there are eight,
+// pieces of 4, 2 and 1 where the row ends (777x333->1001 fp16 8.3 us; 9.3 with single
+// elements).
 template <int DT>
 static __device__ __forceinline__ void load8_tail(
         const typename Elem<DT>::T* p, int n, u32x4* u) {
+    constexpr int W = DT == F32 ? 2 : 1;
+    if (n >= 8) {
+        load8<DT>(p, u);
+        return;
+    }
+    #pragma unroll
+    for (int i = 0; i < W; ++i) u[i] = (u32x4){0, 0, 0, 0};
+    if (n <= 0) return;
     if constexpr (DT == F32) {
+        struct __attribute__((packed, aligned(4))) Four { u32x4 v; };
+        const unsigned* q = reinterpret_cast<const unsigned*>(p);
+        unsigned r[3] = {0, 0, 0};
+        if (n & 4) u[0] = reinterpret_cast<const Four*>(q)->v;
+        q += n & 4;
         #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            u[i >> 2][i & 3] = i < n ? __float_as_uint(p[i]) : 0u;
+        for (int i = 0; i < 3; ++i)
+            if (i < (n & 3)) r[i] = q[i];
+        const u32x4 v = {r[0], r[1], r[2], 0};
+        if (n & 4) u[1] = v;
+        else u[0] = v;
     } else {
+        struct __attribute__((packed, aligned(2))) Four { u32x2 v; };
+        struct __attribute__((packed, aligned(2))) Two { unsigned v; };
         const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned lo = 2 * i < n ? q[2 * i] : 0;
-            const unsigned hi = 2 * i + 1 < n ? q[2 * i + 1] : 0;
-            u[0][i] = lo | (hi << 16);
-        }
+        u32x2 four = {0, 0};
+        unsigned two = 0, one = 0;
+        if (n & 4) four = reinterpret_cast<const Four*>(q)->v;
+        q += n & 4;
+        if (n & 2) two = reinterpret_cast<const Two*>(q)->v;
+        q += n & 2;
+        if (n & 1) one = *q;
+        const unsigned lo = n & 2 ? two : one, hi = n & 2 ? one : 0u;
+        u[0] = n & 4 ? (u32x4){four.x, four.y, lo, hi} : (u32x4){lo, hi, 0, 0};
     }
 }
 

@@ -56,6 +56,34 @@ def test_quantize_every_value_at_every_scale():
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+def test_every_tail_of_a_row(dtype):
+    """Rows that end anywhere in a piece of 8, from any place; NaN around."""
+    for K in range(1, 41):
+        big = torch.full((6, K + 9), math.nan, dtype=dtype, device='cuda')
+        x = torch.randn(6, K).to(dtype)
+        w = ops.mx4_quantize(torch.randn(5, K))
+        wd = w.to('cuda')
+        xv, wv = values(x), values(w.dequantize(torch.float32))
+        for at in (0, 1, 5):
+            big.fill_(math.nan)
+            big[:, at:at + K] = x.cuda()
+            rows = big[:, at:at + K]
+            _same(ops.mx4_quantize(rows), ops.mx4_quantize(x))
+            for form in (0, 1, 2):
+                y = ops._native_or_die().mx4_linear(rows, wd.codes, wd.scales,
+                                                    K, None, form)
+                assert_close(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), K)
+        g = torch.randn(6, K).to(dtype)          # K columns of a gradient
+        v = ops.mx4_quantize(torch.randn(K, 32))
+        vd, vv = v.to('cuda'), values(v.dequantize(torch.float32))
+        dx, _, db = ops._native_or_die().mx4_linear_backward(
+            g.cuda(), vd.codes, vd.scales, None, None, 32, 0, -1, 0, 1)
+        g64 = g.double()
+        assert_close(dx, g64 @ vv, g64.abs() @ vv.abs(), K)
+        assert_close(db, g64.sum(0), g64.abs().sum(0), 6)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_quantize_strides_and_alignments(dtype):
     base = torch.randn(40, 300).to(dtype)
     for view in (lambda t: t[:, :256], lambda t: t[:, 1:257],
