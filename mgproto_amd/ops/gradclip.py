@@ -10,7 +10,7 @@ from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
 
-from . import reference
+from . import _native_or_die, reference
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -44,7 +44,6 @@ def _ext(ts):
     """The extension for GPU tensors, which makes the checks below itself."""
     if not (ts and isinstance(ts[0], torch.Tensor) and ts[0].is_cuda):
         return None
-    from . import _native_or_die
     return _native_or_die()
 
 

@@ -22,7 +22,7 @@ from typing import Optional, Union
 
 import torch
 
-from . import reference
+from . import _native_or_die, reference
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -36,10 +36,7 @@ def _check_float(t: torch.Tensor, what: str):
 
 def _ext(t: torch.Tensor):
     """The extension for GPU tensors, None for the PyTorch form."""
-    if not t.is_cuda:
-        return None
-    from . import _native_or_die
-    return _native_or_die()
+    return _native_or_die() if t.is_cuda else None
 
 
 class MX4Tensor:
@@ -134,12 +131,14 @@ def _matrix(x: torch.Tensor) -> torch.Tensor:
 
 def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
     """[..., K] float32, bfloat16 or float16 -> 4-bit rows. No gradient."""
+    if isinstance(x, torch.Tensor) and x.is_cuda:
+        ext = _ext(x)                  # refuses what the checks below refuse
+        if ext is not None:
+            return MX4Tensor._of(*ext.mx4_quantize(x), x.shape, x.dtype)
     _check_float(x, 'mx4_quantize')
     if x.dim() < 1:
         raise ValueError('mx4_quantize: a tensor of rows, not a number')
-    ext = _ext(x)
-    codes, scales = (ext.mx4_quantize(x) if ext is not None
-                     else reference.mx4_quantize(_matrix(x.detach())))
+    codes, scales = reference.mx4_quantize(_matrix(x.detach()))
     return MX4Tensor._of(codes, scales, x.shape, x.dtype)
 
 

@@ -423,6 +423,12 @@ def test_refusals():
         ext.mx4_linear(x, qd.codes[:, :, ::2], qd.scales, 64, None)
     with pytest.raises(ValueError, match='no form'):
         ext.mx4_linear(x, qd.codes, qd.scales, 64, None, 7)
+    with pytest.raises(TypeError, match='Double'):
+        ops.mx4_quantize(x.double())
+    with pytest.raises(ValueError, match='not a number'):
+        ops.mx4_quantize(x[0, 0])
+    with pytest.raises(TypeError, match='a tensor, not list'):
+        ops.mx4_quantize([x])
     with pytest.raises(ValueError, match='2\\^29 rows'):
         ops.mx4_quantize(x[:1, :1].expand(2 ** 29, 1))
     with pytest.raises(ValueError, match='2\\^22 elements'):
