@@ -12,11 +12,11 @@ static inline long up32(long v) { return (v + 31) / 32 * 32; }
 static inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // dx = A B^T on tiles: A is `parts` matrices of M rows, read 32 elements of the
-// sum at a time (64 bytes), from a + step * a_step + row * a_row; B is
-// [steps][K][32] bf16 and serves every part. C [M, K].
-void grad_input_tiles(const void* a, size_t a_step, size_t a_row, int parts,
-                      int steps, const void* b, long M, long K, void* c,
-                      int dt, void* partial, hipStream_t stream);
+// sum at a time (64 bytes), from a + part * a_part + step * a_step + row * a_row; B
+// is [steps][K][32] bf16 and serves every part. C [M, K].
+void grad_input_tiles(const void* a, size_t a_step, size_t a_row, size_t a_part,
+                      int parts, int steps, const void* b, long M, long K,
+                      void* c, int dt, void* partial, hipStream_t stream);
 size_t grad_input_partial(long M, long K, long steps);
 
 // dw = G^T X on tiles: G is `parts` matrices of M rows of N bf16, `row` elements

@@ -355,57 +355,70 @@ void launch_parts(const GradArgs& a, int Np, void* out, hipStream_t stream) {
     #undef MX4_G
 }
 
+// Both products read one set of parts, in rows: 15680x512x2048 fp32 325 us for 382
+// with a set for each.
+bool share_parts(const GradArgs& a) {
+    return a.dx && a.dw && !dx_in_place(a) && !dw_in_place(a);
+}
+size_t part_bytes(const GradArgs& a, long Np) {
+    return (size_t)parts_of(a.g_dt) * a.M * Np * 2;
+}
+
 size_t dx_bytes(const GradArgs& a) {
     const long Np = up32(a.N);
-    const int P = parts_of(a.g_dt);
     return up256((size_t)a.K * Np * 2)
-        + (dx_in_place(a) ? 0 : up256((size_t)P * a.M * Np * 2))
-        + grad_input_partial(a.M, a.K, Np / 32 * P);
+        + (dx_in_place(a) || share_parts(a) ? 0 : up256(part_bytes(a, Np)))
+        + grad_input_partial(a.M, a.K, Np / 32 * parts_of(a.g_dt));
 }
 
 size_t dw_bytes(const GradArgs& a) {
-    const int P = parts_of(a.g_dt);
-    return (dw_in_place(a) ? 0 : up256((size_t)P * a.M * ((a.N + 7) / 8 * 8) * 2))
-        + grad_weight_partial(a.M, a.N, a.K, P);
+    return (dw_in_place(a) || share_parts(a)
+                ? 0 : up256(part_bytes(a, (a.N + 7) / 8 * 8)))
+        + grad_weight_partial(a.M, a.N, a.K, parts_of(a.g_dt));
 }
 
 size_t db_bytes(const GradArgs& a) {
     return up256((size_t)sums(a.M, a.N).chunks * a.N * 4);
 }
 
-// W^T is written once as bf16 (W is small beside g, or the product large)
-void run_dx(const GradArgs& a, char* at, hipStream_t stream) {
+// W^T is written once as bf16 (W is small beside g, or the product large).
+// `rows`: parts in rows of up32(N), where there are some.
+void run_dx(const GradArgs& a, const char* rows, char* at, hipStream_t stream) {
     const long Np = up32(a.N);
-    const int P = parts_of(a.g_dt);
+    const int P = parts_of(a.g_dt), per = (int)(Np / 32);
     __bf16* wt = (__bf16*)at;
     at += up256((size_t)a.K * Np * 2);
     hipLaunchKernelGGL(values_t_kernel,
                        dim3((unsigned)(Np / 32), (unsigned)steps_of(a.K)),
                        dim3(256), 0, stream, a.wc, a.ws, a.N, a.K, wt);
-    if (dx_in_place(a)) {
-        grad_input_tiles(a.g, 64, a.N * 2, 1, (int)(Np / 32), wt, a.M, a.K, a.dx,
-                         a.dx_dt, at, stream);
+    const size_t row = Np * 2;               // = N * 2 where g is read in place
+    if (rows || dx_in_place(a)) {
+        grad_input_tiles(rows ? rows : a.g, 64, row, a.M * row, P, per, wt, a.M,
+                         a.K, a.dx, a.dx_dt, at, stream);
         return;
     }
     char* parts = at;
-    at += up256((size_t)P * a.M * Np * 2);
+    at += up256(part_bytes(a, Np));
     launch_parts<true>(a, (int)Np, parts, stream);
-    grad_input_tiles(parts, (size_t)a.M * 64, 64, P, (int)(Np / 32), wt, a.M, a.K,
-                     a.dx, a.dx_dt, at, stream);
+    grad_input_tiles(parts, (size_t)a.M * 64, 64, per * (size_t)a.M * 64, P, per,
+                     wt, a.M, a.K, a.dx, a.dx_dt, at, stream);
 }
 
-void run_dw(const GradArgs& a, char* at, hipStream_t stream) {
+void run_dw(const GradArgs& a, const char* rows, char* at, hipStream_t stream) {
     const int P = parts_of(a.g_dt);
-    if (dw_in_place(a)) {
-        grad_weight_tiles(a.g, a.N, 0, 1, a.M, a.N, a.K, a.xc, a.xs, a.dw,
-                          a.dw_dt, at, stream);
-        return;
+    long Np = a.N;
+    const void* g = a.g;
+    if (rows) {
+        Np = up32(a.N);
+        g = rows;
+    } else if (!dw_in_place(a)) {
+        Np = (a.N + 7) / 8 * 8;
+        launch_parts<false>(a, (int)Np, at, stream);
+        g = at;
+        at += up256(part_bytes(a, Np));
     }
-    const long Np = (a.N + 7) / 8 * 8;
-    const size_t part = (size_t)a.M * Np * 2;
-    launch_parts<false>(a, (int)Np, at, stream);
-    grad_weight_tiles(at, Np, part, P, a.M, a.N, a.K, a.xc, a.xs, a.dw, a.dw_dt,
-                      at + up256(P * part), stream);
+    grad_weight_tiles(g, Np, (size_t)a.M * Np * 2, P, a.M, a.N, a.K, a.xc, a.xs,
+                      a.dw, a.dw_dt, at, stream);
 }
 
 void run_db(const GradArgs& a, char* at, hipStream_t stream) {
@@ -446,7 +459,8 @@ void join(const float* part, int S, long n, void* out, int dt,
 size_t grads_bytes(const GradArgs& a, int form) {
     if (form < 0 ? small(a) : form == 0) return 0;
     // one after the other on the stream: the same bytes serve all
-    return std::max({a.dx ? dx_bytes(a) : 0, a.dw ? dw_bytes(a) : 0,
+    return (share_parts(a) ? up256(part_bytes(a, up32(a.N))) : 0)
+        + std::max({a.dx ? dx_bytes(a) : 0, a.dw ? dw_bytes(a) : 0,
                      a.db ? db_bytes(a) : 0});
 }
 
@@ -466,9 +480,15 @@ void grads(const GradArgs& a, int form, void* work, hipStream_t stream) {
         #undef MX4_S
         return;
     }
-    if (a.dx) run_dx(a, (char*)work, stream);
-    if (a.dw) run_dw(a, (char*)work, stream);
-    if (a.db) run_db(a, (char*)work, stream);
+    char *rows = nullptr, *at = (char*)work;
+    if (share_parts(a)) {
+        rows = at;
+        at += up256(part_bytes(a, up32(a.N)));
+        launch_parts<false>(a, (int)up32(a.N), rows, stream);
+    }
+    if (a.dx) run_dx(a, rows, at, stream);
+    if (a.dw) run_dw(a, rows, at, stream);
+    if (a.db) run_db(a, at, stream);
 }
 
 }  // namespace mx4

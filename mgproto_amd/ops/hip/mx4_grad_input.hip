@@ -25,7 +25,7 @@ constexpr int S = 4;
 template <int OT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2)
 void grad_input_kernel(const uint8_t* __restrict__ a, size_t a_step,
-                       size_t a_row, int steps, int per,
+                       size_t a_row, size_t a_part, int steps, int per,
                        const uint8_t* __restrict__ b, long M, long N,
                        typename Elem<OT>::T* __restrict__ c, int mt, int nt,
                        int splits, int group) {
@@ -64,9 +64,9 @@ void grad_input_kernel(const uint8_t* __restrict__ a, size_t a_step,
         place(lt, m0, n0, lk, lend);
         const int lasta = (int)min((long)BM, M - m0) - 1;
         const int lastb = (int)min((long)BN, N - n0) - 1;
-        la = a + m0 * a_row + lk * a_step;
-        lb0 = b + n0 * 64;
         lp = lk % per;                            // step of this part
+        la = a + lk / per * a_part + lp * a_step + m0 * a_row;
+        lb0 = b + n0 * 64;
         lb = lb0 + (size_t)lp * N * 64;
         #pragma unroll
         for (int q = 0; q < XQ; ++q) {
@@ -80,6 +80,7 @@ void grad_input_kernel(const uint8_t* __restrict__ a, size_t a_step,
             bo[q] = min(r, lastb) * 64 + ((lane & 3) ^ w_key<FN>(r)) * 16;
         }
     };
+    const size_t next_part = a_part - per * a_step;
     bool more = true;
     auto send = [&](int buf, int q) {
         if (q < XQ)
@@ -92,7 +93,7 @@ void grad_input_kernel(const uint8_t* __restrict__ a, size_t a_step,
     auto sent = [&]() {
         if (!more) return;
         la += a_step, lb += (size_t)N * 64;
-        if (++lp == per) lp = 0, lb = lb0;
+        if (++lp == per) lp = 0, lb = lb0, la += next_part;
         if (++lk == lend) {
             more = lt + stride < hi;
             if (more) lt += stride;
@@ -199,9 +200,9 @@ size_t grad_input_partial(long M, long K, long steps) {
     return s > 1 ? up256((size_t)s * M * K * 4) : 0;
 }
 
-void grad_input_tiles(const void* a, size_t a_step, size_t a_row, int parts,
-                      int per, const void* b, long M, long K, void* c, int dt,
-                      void* partial, hipStream_t stream) {
+void grad_input_tiles(const void* a, size_t a_step, size_t a_row, size_t a_part,
+                      int parts, int per, const void* b, long M, long K,
+                      void* c, int dt, void* partial, hipStream_t stream) {
     const int steps = per * parts;
     const Plan p = plan(M, K, steps);
     const int mt = (int)((M + p.bm - 1) / p.bm), nt = (int)((K + p.bn - 1) / p.bn);
@@ -212,7 +213,7 @@ void grad_input_tiles(const void* a, size_t a_step, size_t a_row, int parts,
         hipLaunchKernelGGL((grad_input_kernel<OT, BM, BN, WM, WN>), \
             dim3(std::min((total + 7) / 8 * 8, p.slots)), \
             dim3(64 * WM * WN), 0, stream, (const uint8_t*)a, a_step, a_row, \
-            steps, per, (const uint8_t*)b, M, K, (typename Elem<OT>::T*)out, mt, \
+            a_part, steps, per, (const uint8_t*)b, M, K, (typename Elem<OT>::T*)out, mt, \
             nt, p.splits, 4)
     #define MX4_T(OT) do { \
         if (p.bn == 256) MX4_G(OT, 256, 256, 2, 4); \

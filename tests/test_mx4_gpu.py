@@ -221,6 +221,39 @@ def test_gradients_at_the_ends_of_the_scales(form):
         assert torch.equal(dx.double().cpu(), want)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16])
+@pytest.mark.parametrize('M,K,N', [(300, 200, 136), (130, 257, 131),
+                                   (2000, 70, 1000), (3001, 128, 33)])
+def test_every_part_of_a_wide_output_gradient(M, K, N, dtype):
+    """Alone and together, where both products read the same parts: each has
+    its bits of the sum."""
+    ext = ops._native_or_die()
+    x, w, g = torch.randn(M, K), torch.randn(N, K), torch.randn(M, N).to(dtype)
+    xv, wv, g64 = values(x), values(w), g.double()
+    xq, wq = ops.mx4_quantize(x.cuda()), ops.mx4_quantize(w.cuda())
+    for want_x, want_w in ((0, -1), (-1, 0), (0, 0)):
+        dx, dw, _ = ext.mx4_linear_backward(
+            g.cuda(), wq.codes, wq.scales, xq.codes, xq.scales, K, want_x,
+            want_w, -1, 1)
+        # three parts for each term of a sum
+        if want_x == 0:
+            assert_close(dx, g64 @ wv, g64.abs() @ wv.abs(), 3 * N)
+        if want_w == 0:
+            assert_close(dw, g64.t() @ xv, g64.abs().t() @ xv.abs(), 3 * M)
+    # one term whose last bit only the last part holds
+    g = torch.zeros(M, N, dtype=dtype)
+    g[5, 7] = 1 + torch.finfo(dtype).eps
+    wq, xq = (ops.mx4_quantize(torch.ones(n, K).cuda()) for n in (N, M))
+    for want_x, want_w in ((0, -1), (-1, 0), (0, 0)):
+        dx, dw, _ = ext.mx4_linear_backward(
+            g.cuda(), wq.codes, wq.scales, xq.codes, xq.scales, K, want_x,
+            want_w, -1, 1)
+        if want_x == 0:
+            assert torch.equal(dx.cpu(), g.float().sum(1, True).expand(M, K))
+        if want_w == 0:
+            assert torch.equal(dw.cpu(), g.float().sum(0)[:, None].expand(N, K))
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('M,K,N', [(70, 130, 40), (3000, 200, 300)])
 def test_infinities_in_the_output_gradient(M, K, N, dtype):
