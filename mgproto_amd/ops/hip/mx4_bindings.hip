@@ -1,6 +1,7 @@
 // Tensor entry points of the MX4 product and of gradient clipping.
 
 #include <torch/extension.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -45,6 +46,12 @@ at::ScalarType scalar_type(int64_t dt) {
     TORCH_CHECK(dt >= 0 && dt <= 2, "unknown type code ", dt);
     return dt == mx4::F32 ? at::kFloat : dt == mx4::BF16 ? at::kBFloat16
                                                          : at::kHalf;
+}
+
+// at::empty, past the dispatcher: small calls are bound by the host (1x512->512 4.6 us
+// -> 4.2, rounding 5.0 -> 4.4)
+Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+    return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
 }
 
 hipStream_t current_stream() { return at::hip::getCurrentHIPStream(); }
@@ -106,17 +113,15 @@ void check_bias(const OptTensor& bias, int64_t N, const Tensor& like) {
 }
 
 Tensor workspace(size_t bytes, const Tensor& like) {
-    return at::empty({(int64_t)std::max<size_t>(bytes, 1)},
-                     like.options().dtype(at::kByte));
+    return fresh({(int64_t)std::max<size_t>(bytes, 1)}, at::kByte, like);
 }
 
 struct Packed {               // room for the blocks of a matrix
     Tensor codes, scales;
     explicit Packed(const Tensor& x2) {
         const int64_t R = x2.size(0), K = x2.size(1);
-        auto opt = x2.options().dtype(at::kByte);
-        codes = at::empty({mx4::steps_of(K), R, 64}, opt);
-        scales = at::empty({mx4::chunks_of(K), R, 16}, opt);
+        codes = fresh({mx4::steps_of(K), R, 64}, at::kByte, x2);
+        scales = fresh({mx4::chunks_of(K), R, 16}, at::kByte, x2);
     }
 };
 
@@ -141,8 +146,7 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
                   int64_t dt) {
     check_packed(codes, scales, K, "mx4_dequantize");
     c10::DeviceGuard guard(codes.device());
-    auto out = at::empty({codes.size(1), K},
-                         codes.options().dtype(scalar_type(dt)));
+    auto out = fresh({codes.size(1), K}, scalar_type(dt), codes);
     mx4::dequantize(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
                     codes.size(1), K, out.data_ptr(), (int)dt,
                     current_stream());
@@ -187,7 +191,7 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws, int64_t K,
     check_packed(wc, ws, K, "mx4_linear: weight");
     check_bias(bias, N, x);
     c10::DeviceGuard guard(x.device());
-    auto y = at::empty(shape_of(x, N), x.options());
+    auto y = fresh(shape_of(x, N), x.scalar_type(), x);
     if (!M || !N) return y;
     const Bias b(bias);
     const int64_t ldx = row_stride(x2);
@@ -206,7 +210,7 @@ Tensor product_q(const Tensor& xc, const Tensor& xs, int64_t K,
                  std::vector<int64_t> shape, int dt, int64_t form) {
     const int64_t M = xc.size(1), N = wc.size(1);
     check_bias(bias, N, xc);
-    auto y = at::empty(shape, xc.options().dtype(scalar_type(dt)));
+    auto y = fresh(shape, scalar_type(dt), xc);
     if (!M || !N) return y;
     const Bias b(bias);
     const int chosen = mx4::linear_q_form(M, K, N);
@@ -293,7 +297,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
     auto make = [&](std::vector<int64_t> shape, int64_t dt, int64_t over,
                     OptTensor& t, void*& ptr, int& code) {
         if (dt < 0) return;
-        t = at::empty(shape, g.options().dtype(scalar_type(dt)));
+        t = fresh(shape, scalar_type(dt), g);
         code = (int)dt;
         if (!t->numel()) return;
         if (over) ptr = t->data_ptr();
@@ -471,10 +475,9 @@ Tensor grad_norm(const std::vector<Tensor>& grads, double p) {
         const int dt = dtype_code(c, "grad_norm");
         items.push_back({c.data_ptr(), nullptr, c.numel(), dt, dt});
     }
-    auto norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+    auto norm = fresh({}, at::kFloat, grads[0]);
     const gradclip::List list(items);
-    auto work = at::empty({(int64_t)list.workspace_doubles()},
-                          norm.options().dtype(at::kDouble));
+    auto work = fresh({(int64_t)list.workspace_doubles()}, at::kDouble, norm);
     list.norm(kind, norm.data_ptr<float>(), work.data_ptr<double>(),
               current_stream());
     return norm;
@@ -514,10 +517,9 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
                          dtype_code(o, "clip_grads_: out")});
     }
     check_apart(items);
-    auto norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+    auto norm = fresh({}, at::kFloat, grads[0]);
     const gradclip::List list(items);
-    auto work = at::empty({(int64_t)list.workspace_doubles()},
-                          norm.options().dtype(at::kDouble));
+    auto work = fresh({(int64_t)list.workspace_doubles()}, at::kDouble, norm);
     list.clip(kind, max_norm, norm.data_ptr<float>(), work.data_ptr<double>(),
               current_stream());
     for (const auto& o : outs)           // written behind autograd's back
