@@ -223,7 +223,8 @@ def test_gradients_at_the_ends_of_the_scales(form):
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.float16])
 @pytest.mark.parametrize('M,K,N', [(300, 200, 136), (130, 257, 131),
-                                   (2000, 70, 1000), (3001, 128, 33)])
+                                   (2000, 70, 1000), (3001, 128, 33),
+                                   (2101, 333, 235)])
 def test_every_part_of_a_wide_output_gradient(M, K, N, dtype):
     """Alone and together, where both products read the same parts: each has
     its bits of the sum."""
