@@ -170,10 +170,13 @@ static bool small_blocks(long M, long N) {
 // 24, 8192x512->256 7.7 against 10.5. There have to be blocks enough to cover a
 // long sum's waits: 8192x1024->128 10.2 against 13.0 but 8192x2048->128 22 against
 // 18, 32768x4096->128 56 against 77. With more columns x is rounded again:
-// 16384x512->512 11.6 against 15.3, 131072x512->512 74 against 69. A short sum with
-// many results is bound by their way out, where tiles of more rows do better:
-// 131072x64->256 26 against 29, but 1003520x64->256 255 against 172.
-static bool few_columns(long M, long K, long N) {
+// 16384x512->512 11.6 against 15.3, 131072x512->512 74 against 69; where the sum is
+// short that does not matter, 2048x64->2048 5.6 against 8.4, 8551x12->1611 18 against
+// 20 (and 39 in small blocks), until the results' way out counts, where tiles of
+// more rows do better: 62720x256->1024 46 against 41, 131072x64->256 26 against 29 but
+// 1003520x64->256 255 against 172.
+static bool rounds_on_the_way(long M, long K, long N) {
+    if (K <= 256 && M <= 16384 && (M + 31) / 32 * ((N + 31) / 32) >= 1536) return true;
     if (M < (K <= 512 ? 4096 : K <= 1024 ? 8192 : 32768)) return false;
     if (N <= 64) return true;
     if (N <= 256) return K >= 256 || M <= 131072;
@@ -181,22 +184,28 @@ static bool few_columns(long M, long K, long N) {
 }
 
 int linear_form(long M, long K, long N) {
-    if (few_columns(M, K, N)) return ROUNDING;
+    if (rounds_on_the_way(M, K, N)) return ROUNDING;
     const double work = (double)(M > 16 ? M : 16) * K * N;
     if (work <= (K <= 2048 ? 0x1p29 : 0x1p28))
         return small_blocks(M, N) ? ROWS16 : ROWS32;
     return linear_q_form(M, K, N);
 }
 
-// Small blocks share a sum among their waves and read past LDS: 128x4096->4096
-// (2^31) 11.5 against 16.7 us with tiles of 128, 256x4096->4096 20.8 against
-// 16.7. Tiles of 256 take half the bytes a result, but there have to be some for
-// each of 256 units: 8192x4096->16384 (2048 tiles) 262 against 318,
+// Small blocks share a sum among their waves and read past LDS: 128x4096->4096 (2^31)
+// 11.5 us against 16.7 with tiles of 128. They lose where they read too much,
+// 256x4096->4096 20.8 against 16.7, or are so many that tiles fill the card (and are
+// full themselves): 2048x512->1024 (2048 blocks) 7.5 against 6.0, 65536x32->128 11.3
+// against 7.4; but 1024^3 (1024) 7.1 and 7.0, 64337x635->11 (2011, its tiles all but
+// empty) 6.8 against 8.0. Tiles of 256 take half the bytes a result, but there have
+// to be some for each of 256 units: 8192x4096->16384 (2048 tiles) 262 against 318,
 // 2048x4096->4096 (128 tiles) 34 against 25; with 128 columns half of a tile is
 // empty, 250880x512->128 31 against 24.
 int linear_q_form(long M, long K, long N) {
     if (M <= 16) return HELD16;
-    if ((double)M * K * N <= 0x1p31) return small_blocks(M, N) ? HELD16 : HELD32;
+    const long blocks = (M + 31) / 32 * ((N + 31) / 32);
+    const bool many = blocks >= 1536 && (M + 127) / 128 * ((N + 127) / 128) * 12 <= blocks;
+    if ((double)M * K * N <= 0x1p31 && !many)
+        return small_blocks(M, N) ? HELD16 : HELD32;
     const long tiles = (M + 255) / 256 * ((N + 255) / 256);
     return N > 128 && tiles >= 384 ? TILES256 : TILES128;
 }
