@@ -257,7 +257,7 @@ void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
 // Forms of the product; linear_form() and linear_q_form() choose. Each is right
 // for every size.
 enum Form : int {
-    ROWS16 = 0,       // 16 x 16 of y a block, x rounded by each block
+    ROWS16 = 0,       // 16 x 16 or 32 of y a block, x rounded by each block
     ROWS32 = 1,       // 32 x 32, the same
     ROUNDING = 2,     // tiles of 64 rows, x rounded on its way into LDS
     HELD16 = 3,       // x rounded before; then the same from 4-bit rows,

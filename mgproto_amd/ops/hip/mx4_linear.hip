@@ -134,15 +134,17 @@ void launch_rows(const void* x, const uint8_t* xs, long M, long K, long ldx,
                  const uint8_t* wc, const uint8_t* ws, long N,
                  const void* bias, int bias_dt, void* y, int form,
                  hipStream_t stream) {
-    #define MX4_L(F, WV) do { \
-        const long mt = (M + 16 * F - 1) / (16 * F), nt = (N + 16 * F - 1) / (16 * F); \
-        hipLaunchKernelGGL((linear_rows_kernel<AT, OT, F, F, WV>), \
+    #define MX4_L(FM, FN, WV) do { \
+        const long mt = (M + 16 * FM - 1) / (16 * FM); \
+        const long nt = (N + 16 * FN - 1) / (16 * FN); \
+        hipLaunchKernelGGL((linear_rows_kernel<AT, OT, FM, FN, WV>), \
             dim3((unsigned)(mt * nt)), dim3(64 * WV), 0, stream, x, xs, M, (int)K, \
             (int)steps_of(K), ldx, wc, ws, N, bias, bias_dt, (typename Elem<OT>::T*)y, \
             (int)nt); } while (0)
-    if (form != ROWS16 && form != HELD16) MX4_L(2, 4);
-    else if (steps_of(K) >= 8) MX4_L(1, 8);
-    else MX4_L(1, 4);
+    if (form != ROWS16 && form != HELD16) MX4_L(2, 2, 4);
+    else if (M > 16 && (M + 15) / 16 * ((N + 15) / 16) > 256) MX4_L(1, 2, 4);
+    else if (steps_of(K) >= 8) MX4_L(1, 1, 8);
+    else MX4_L(1, 1, 4);
     #undef MX4_L
 }
 
@@ -152,11 +154,12 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // The choice; times in us, bf16, on an MI355X.
 //
-// Blocks of 16 x 16 where there are too few of 32 x 32 for 256 units:
-// 64x4096->1024 (64 of those) 6.7 against 12.2, 196x2048->512 (112) 6.7 against 7.5,
-// 784x1024->256 (200) 6.9 against 5.3.
+// The smallest blocks of which every one of 256 units has one at most: 16 x 16,
+// 64x4096->1024 (256 of them) 6.7 us, 8.3 in 16 x 32 and 12.4 in 32 x 32; 16 x 32,
+// 196x2048->512 (208) 5.4 against 6.7 and 7.5; 32 x 32, 784x1024->256 (200) 5.2 against
+// 6.7 and 5.4.
 static bool small_blocks(long M, long N) {
-    return M <= 16 || (M + 31) / 32 * ((N + 31) / 32) <= 128;
+    return M <= 16 || (M + 15) / 16 * ((N + 31) / 32) <= 256;
 }
 
 // Rounding in the blocks saves a launch (4 us) and a pass over x, but every block
