@@ -155,14 +155,14 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
 
 // The form that is asked for, or the chosen one. A launch has 2^32 threads at
 // most: forms of small blocks have 256 (512) for each 16 x 16 or 32 x 32 results, the
-// one that rounds on the way for 64 rows of up to 256 columns; tiles take turns.
+// one that rounds on the way for 64 rows of 64 to 256 columns; tiles take turns.
 int pick(int64_t form, int chosen, int64_t M, int64_t N) {
     CHECK_VALUE(form >= -1 && form < mx4::FORMS, "mx4_linear: no form ", form);
     const int f = form < 0 ? chosen : (int)form;
     int64_t rows = 128, cols = 128, most = 1L << 30;
     if (f == mx4::ROWS16 || f == mx4::HELD16) rows = cols = 16, most = 1L << 23;
     else if (f == mx4::ROWS32 || f == mx4::HELD32) rows = cols = 32, most = 1L << 24;
-    else if (f == mx4::ROUNDING) rows = 64, cols = N > 128 ? 256 : 64, most = 1L << 24;
+    else if (f == mx4::ROUNDING) rows = 64, cols = N > 128 ? 256 : 64, most = 1L << 23;
     CHECK_VALUE((M + rows - 1) / rows * ((N + cols - 1) / cols) < most,
                 "mx4_linear: ", M, " x ", N, " results are too many");
     return f;

@@ -8,10 +8,12 @@
 // (four lanes share a block, two lane exchanges for its maximum) and written as
 // codes. One barrier a buffer.
 //
-// Bound by x's way from memory: 62720x1024->256 takes 35 us (4.6 TB/s),
-// 250880x256->64 27 (6.0). Three blocks and more share a unit, so that one reads
-// while another starts or writes: tiles of 128 rows and 256 elements, one on a
-// unit, took 39 and 38. x two steps ahead: 36 and 27, 62720x512->128 18 for 16.
+// Bound by x's way from memory: 62720x1024->256 takes 35 us where the caches hold x
+// (4.6 TB/s), 40 where not, 250880x256->64 27 (6.0). Two blocks and more share a
+// unit, so that one reads while another starts or writes: tiles of 128 rows and 256
+// elements, one on a unit, took 39 and 38; four waves for 256 columns instead of
+// eight 37 and 42 (62720x333->200 24 and 28 for 20 and 24). x two steps ahead: 36,
+// 62720x512->128 18 for 16.
 
 #include <hip/hip_runtime.h>
 
@@ -168,7 +170,7 @@ void rounding(const void* x, int dt, long M, long K, long ldx,
         if (dt == F32) MX4_T(F32, BN, WM, WN); \
         else if (dt == BF16) MX4_T(BF16, BN, WM, WN); \
         else MX4_T(F16, BN, WM, WN); } while (0)
-    if (N > 128) MX4_D(256, 1, 4);
+    if (N > 128) MX4_D(256, 2, 4);
     else if (N > 64) MX4_D(128, 2, 2);
     else MX4_D(64, 4, 1);
     #undef MX4_D
