@@ -101,12 +101,19 @@ void rounding_kernel(const typename Elem<DT>::T* __restrict__ x, long M, int K,
     const int xr = wm + r16, wr = wn + (r16 >> 2) * (4 * FN) + (r16 & 3);
     const int xp = xr * 64 + ((g ^ x_key(xr)) << 4);
     const int wp = wr * 64 + ((g ^ w_key<FN>(wr)) << 4);
+    int wb[FN];                          // scales of this step and up to 3 more
     auto compute = [&](int k, int buf) {
-        int wb[FN], xb[FM];
+        int xb[FM];
         i32x4 w[FN];
-        #pragma unroll
-        for (int j = 0; j < FN; ++j)
-            wb[j] = wsl[k >> 2 & 1][(wr + j * 4) * 16 + g * 4 + (k & 3)];
+        if ((k & 3) == 0) {
+            #pragma unroll
+            for (int j = 0; j < FN; ++j)
+                wb[j] = *reinterpret_cast<const int*>(
+                    wsl[k >> 2 & 1] + (wr + j * 4) * 16 + g * 4);
+        } else {
+            #pragma unroll
+            for (int j = 0; j < FN; ++j) wb[j] = (unsigned)wb[j] >> 8;
+        }
         #pragma unroll
         for (int i = 0; i < FM; ++i) xb[i] = xsl[buf][(xr + i * 16) * 4 + g];
         #pragma unroll
