@@ -8,8 +8,8 @@
 // (four lanes share a block, two lane exchanges for its maximum) and written as
 // codes. One barrier a buffer.
 //
-// Bound by x's way from memory: 62720x1024->256 takes 35 us where the caches hold x
-// (4.6 TB/s), 40 where not, 250880x256->64 27 (6.0). Two blocks and more share a
+// Bound by x's way from memory: 62720x1024->256 takes 34 us where the caches hold x
+// (4.8 TB/s), 39 where not, 250880x256->64 27 (6.0). Two blocks and more share a
 // unit, so that one reads while another starts or writes: tiles of 128 rows and 256
 // elements, one on a unit, took 39 and 38; four waves for 256 columns instead of
 // eight 37 and 42 (62720x333->200 24 and 28 for 20 and 24). x two steps ahead: 36,
