@@ -24,6 +24,9 @@ Capture constraints and how they are met:
 * the EM update runs INLINE in the graph (no side stream: cross-stream
   event sync inside capture is legal but buys nothing when every step
   runs EM);
+* the library's memset nodes (weight gradients of convolutions, reductions)
+  become fill kernels before the graph is instantiated: such nodes write
+  wrongly in later replays on this hardware (utils/graphs.py);
 * per-step scalars (loss terms, batch accuracy) are written into static
   device buffers inside the graph and read by the trainer afterwards —
   no host sync is added.
@@ -38,6 +41,8 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+
+from ..utils.graphs import capture_graph
 
 
 def graphs_enabled(device, world: int = 1) -> bool:
@@ -178,10 +183,9 @@ class GraphedStep:
                 self._warm_count += 1
                 return self.stats
             try:
-                g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g):
-                    self._compute(optimizer, reducer, em_active, use_mine)
-                self.graph = g
+                self.graph, _ = capture_graph(
+                    lambda: self._compute(optimizer, reducer, em_active,
+                                          use_mine))
                 # the capture itself did not execute: replay once so THIS
                 # batch trains too
                 self.graph.replay()

@@ -1027,9 +1027,11 @@ std::vector<torch::Tensor> gemm1x1_fwd(torch::Tensor x, torch::Tensor w,
                                        int64_t mode);
 
 void register_mx4(pybind11::module& m);      // mx4_bindings.hip
+void register_graph(pybind11::module& m);    // graph_fill.hip
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     register_mx4(m);
+    register_graph(m);
     m.def("gmm_fwd", &gmm_fwd, "fused GMM score GEMM forward (MFMA f32)");
     m.def("gmm_bwd", &gmm_bwd, "GMM score GEMM backward wrt features");
     m.def("gmm_fwd_uni", &gmm_fwd_uni,

@@ -22,6 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from .models import use_mx4
+from .utils.graphs import capture_graph
 from .utils.receptive_field import compute_rf_prototype
 
 
@@ -73,9 +74,8 @@ class InferenceEngine:
             for _ in range(3):
                 self._forward(self._static_in)
         torch.cuda.current_stream().wait_stream(s)
-        self._graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self._graph):
-            self._static_out = self._forward(self._static_in)
+        self._graph, self._static_out = capture_graph(
+            lambda: self._forward(self._static_in))
         return self
 
     def _run(self, x: torch.Tensor):

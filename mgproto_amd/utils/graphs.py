@@ -1,0 +1,26 @@
+"""Capture into a HIP graph that replays as it ran."""
+
+from typing import Any, Callable, Tuple
+
+import torch
+
+
+def capture_graph(fn: Callable[[], Any]) -> Tuple[torch.cuda.CUDAGraph, Any]:
+    """Captures ``fn()``; (the graph, ready to replay, and fn's result).
+
+    Libraries record hipMemsetAsync where they clear workspaces and results.
+    Replays after the first get such nodes wrong on this hardware, so they are
+    replaced by fill kernels (ops/hip/graph_fill.hip) before the graph is
+    instantiated."""
+    from .. import ops
+    ext = ops._load_extension()
+    if ext is None:
+        raise RuntimeError('capture_graph: the mgproto_hip extension is '
+                           'required: it replaces memset nodes, which replay '
+                           'wrongly')
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        out = fn()
+    ext.graph_fill_nodes(graph.raw_cuda_graph())
+    graph.instantiate()
+    return graph, out
