@@ -95,7 +95,8 @@ class GemmConv2d(nn.Conv2d):
                 'this 1x1 convolution holds its weight in 4 bits and cannot '
                 'train it: use_mx4(model, train=True), or freeze the weight')
         made_of, state = self._mx4_of
-        if made_of() is not self.weight or state != _state(self.weight):
+        if (state is None or made_of() is not self.weight
+                or state != _state(self.weight)):
             self._mx4_pack()
         return ops.MX4Tensor(self._mx4_codes, self._mx4_scales,
                              (self.out_channels, self.in_channels))
@@ -119,7 +120,9 @@ class GemmConv2d(nn.Conv2d):
 
 
 def _state(w: torch.Tensor):
-    return w.dtype, -1 if w.is_inference() else w._version
+    """What changes with an update; None where updates leave no trace: codes
+    of a parameter made in inference mode are made in every forward."""
+    return None if w.is_inference() else (w.dtype, w._version)
 
 
 def _nothing():
