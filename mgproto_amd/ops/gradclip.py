@@ -9,6 +9,7 @@ same gradients.
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native_or_die, reference
 
@@ -27,6 +28,9 @@ def _tensors(ts: List[torch.Tensor], what: str):
         if t.device != ts[0].device:
             raise ValueError(f'{what}: tensors on {ts[0].device} and '
                              f'{t.device}')
+        if (forward_ad._current_level >= 0
+                and forward_ad.unpack_dual(t).tangent is not None):
+            raise NotImplementedError(f'{what}: no forward-mode derivative')
 
 
 def _check_p(norm_type: float, what: str) -> float:

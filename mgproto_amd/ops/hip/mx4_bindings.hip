@@ -28,6 +28,14 @@ void refuse_unless(bool ok, A&&... what) {
 #define CHECK_TYPE(ok, ...) refuse_unless<py::type_error>(ok, __VA_ARGS__)
 #define CHECK_VALUE(ok, ...) refuse_unless<py::value_error>(ok, __VA_ARGS__)
 
+// A forward-mode derivative would be dropped without a word.
+void check_no_tangent(const Tensor& t, const char* what) {
+    if (!t._fw_grad(0).defined()) return;
+    PyErr_SetString(PyExc_NotImplementedError, c10::str(
+        what, ": no forward-mode derivative").c_str());
+    throw py::error_already_set();
+}
+
 int dtype_code(const Tensor& t, const char* what) {
     CHECK_TYPE(!t.is_neg(), what, ": a view that stands for its negative; "
                "resolve_neg() it first");
@@ -379,6 +387,9 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
 };
 
 bool needs_grad(const Tensor& x, const OptTensor& w, const OptTensor& bias) {
+    check_no_tangent(x, "mx4_linear: input");
+    if (w.has_value()) check_no_tangent(*w, "mx4_linear: weight");
+    if (bias.has_value()) check_no_tangent(*bias, "mx4_linear: bias");
     return at::GradMode::is_enabled() &&
            (x.requires_grad() || (w.has_value() && w->requires_grad()) ||
             (bias.has_value() && bias->requires_grad()));
@@ -420,6 +431,7 @@ void check_list(const std::vector<Tensor>& ts, const char* what) {
         CHECK_VALUE(t.device() == ts[0].device(), what, ": tensors on ",
                     ts[0].device(), " and ", t.device());
         CHECK_VALUE(t.is_cuda(), what, ": on ", t.device(), ", not on a GPU");
+        check_no_tangent(t, what);
         dtype_code(t, what);
     }
 }

@@ -40,3 +40,41 @@ def test_held_codes_follow_weights_made_in_inference_mode(device):
     with torch.inference_mode():
         conv.weight.mul_(-3)
     _check_layer(conv, x)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('which', ['x', 'w', 'b'])
+@pytest.mark.parametrize('held', [False, True])
+@pytest.mark.parametrize('leaf', [False, True])
+def test_forward_mode_derivatives_are_refused(which, held, leaf, device):
+    if held and which == 'w':
+        return                           # held weights have no derivative
+    from torch.autograd import forward_ad
+    every = {'x': torch.randn(4, 64, device=device),
+             'w': torch.randn(8, 64, device=device),
+             'b': torch.randn(8, device=device)}
+    weight = ops.mx4_quantize(every['w']) if held else None
+    with forward_ad.dual_level():
+        t = every[which].requires_grad_(leaf)
+        every[which] = forward_ad.make_dual(t, torch.ones_like(t))
+        with pytest.raises(NotImplementedError):
+            ops.mx4_linear(every['x'], weight or every['w'], every['b'])
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            ops.mx4_linear(every['x'], weight or every['w'], every['b'])
+        # an ordinary call within the level is none of its business
+        ops.mx4_linear(torch.randn(2, 64, device=device),
+                       ops.mx4_quantize(torch.randn(3, 64, device=device)))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_clipping_refuses_forward_mode_derivatives(device):
+    from torch.autograd import forward_ad
+    t, out = torch.randn(9, device=device), torch.zeros(9, device=device)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.grad_norm([t, d]),
+                     lambda: ops.clip_grads_([d], 0.1),
+                     lambda: ops.clip_grads_([d], 0.1, out=[out])):
+            with pytest.raises(NotImplementedError, match='forward-mode'):
+                call()
+    assert not out.any()
