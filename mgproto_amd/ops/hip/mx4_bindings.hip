@@ -72,7 +72,7 @@ Tensor matrix(const Tensor& x, const char* what) {
     CHECK_VALUE(K < (1L << 22), what, ": rows of at most 2^22 elements");
     int64_t M = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) M *= x.size(i);
-    // 64 rows a block, at the least, and 2^32 threads a launch
+    // the products' launches: 64 rows a block in the longest ones, 2^32 threads
     CHECK_VALUE(M < (1L << 29), what, ": fewer than 2^29 rows");
     Tensor x2 = x.dim() == 2 ? x : x.reshape({M, K});
     if ((K > 1 && x2.stride(1) != 1) || (M > 1 && x2.stride(0) < K))

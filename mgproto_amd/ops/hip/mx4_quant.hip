@@ -71,21 +71,28 @@ static __device__ __forceinline__ void quantize_rows(const Rows& a, int K,
     }
 }
 
+// The number of this block; a grid too long for one axis has several rows of
+// blocks, the last ones of which find no rows left.
+static __device__ __forceinline__ long block_number() {
+    return (long)blockIdx.y * gridDim.x + blockIdx.x;
+}
+
 template <int DT, int LPR>
 __global__ __launch_bounds__(256)
 void quantize_kernel(const Rows a, int K, int steps, int chunks) {
-    quantize_rows<DT, LPR>(a, K, steps, chunks, blockIdx.x);
+    quantize_rows<DT, LPR>(a, K, steps, chunks, block_number());
 }
 
 // Two matrices of the same row length, the first in the first blocks: one
 // launch less for a training step, which rounds the weight and the rows.
 template <int LPR>
 __global__ __launch_bounds__(256)
-void quantize_two_kernel(const Rows a, const Rows b, unsigned first, int K,
+void quantize_two_kernel(const Rows a, const Rows b, long first, int K,
                          int steps, int chunks) {
-    const bool is_a = blockIdx.x < first;
+    const long number = block_number();
+    const bool is_a = number < first;
     const Rows& r = is_a ? a : b;
-    const long block = is_a ? blockIdx.x : blockIdx.x - first;
+    const long block = is_a ? number : number - first;
     if (r.dt == F32) quantize_rows<F32, LPR>(r, K, steps, chunks, block);
     else if (r.dt == BF16)
         quantize_rows<BF16, LPR>(r, K, steps, chunks, block);
@@ -100,7 +107,7 @@ void dequantize_kernel(const uint8_t* __restrict__ codes,
     using T = typename Elem<DT>::T;
     constexpr int RPW = 64 / LPR;
     const int lane = threadIdx.x & 63, sub = lane % LPR;
-    const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long wave = block_number() * 4 + (threadIdx.x >> 6);
     const int chunk = (int)(wave % chunks);
     const long row0 = wave / chunks * (RPW * ROWS) + lane / LPR;
     const int k = chunk * 512 + sub * 8;
@@ -129,10 +136,18 @@ void dequantize_kernel(const uint8_t* __restrict__ codes,
 }
 
 // blocks of four waves; short rows lie four side by side
-unsigned blocks_for(long R, long K, bool shortrow) {
+long blocks_for(long R, long K, bool shortrow) {
     const long waves = shortrow ? (R + 4 * ROWS - 1) / (4 * ROWS)
                                 : (R + ROWS - 1) / ROWS * chunks_of(K);
-    return (unsigned)((waves + 3) / 4);
+    return (waves + 3) / 4;
+}
+
+// An axis of a launch has fewer than 2^32 threads, and a block takes 16 rows of 512
+// elements: 2^28 rows of 129 fill more than one.
+dim3 grid_of(long blocks) {
+    constexpr long MOST = 1L << 23;
+    if (blocks <= MOST) return dim3((unsigned)blocks);
+    return dim3((unsigned)MOST, (unsigned)((blocks + MOST - 1) / MOST));
 }
 
 }  // namespace
@@ -142,7 +157,7 @@ void quantize(const void* x, int dt, long rows, long K, long ldx,
     if (rows == 0 || K == 0) return;
     const bool shortrow = K <= 128;
     const Rows a{x, rows, ldx, codes, scales, dt};
-    const dim3 grid(blocks_for(rows, K, shortrow));
+    const dim3 grid = grid_of(blocks_for(rows, K, shortrow));
     #define MX4_Q(DT, L) \
         hipLaunchKernelGGL((quantize_kernel<DT, L>), grid, dim3(256), 0, stream, \
                            a, (int)K, (int)steps_of(K), (int)chunks_of(K))
@@ -167,8 +182,8 @@ void quantize_two(const void* x, int dt, long rows, long ldx, uint8_t* codes,
     const bool shortrow = K <= 128;
     const Rows a{x, rows, ldx, codes, scales, dt};
     const Rows b{x2, rows2, ldx2, codes2, scales2, dt2};
-    const unsigned first = blocks_for(rows, K, shortrow);
-    const dim3 grid(first + blocks_for(rows2, K, shortrow));
+    const long first = blocks_for(rows, K, shortrow);
+    const dim3 grid = grid_of(first + blocks_for(rows2, K, shortrow));
     #define MX4_Q(L) \
         hipLaunchKernelGGL((quantize_two_kernel<L>), grid, dim3(256), 0, stream, \
                            a, b, first, (int)K, (int)steps_of(K), \
@@ -182,7 +197,7 @@ void dequantize(const uint8_t* codes, const uint8_t* scales, long rows,
                 long K, void* out, int dt, hipStream_t stream) {
     if (rows == 0 || K == 0) return;
     const bool shortrow = K <= 128;
-    const dim3 grid(blocks_for(rows, K, shortrow));
+    const dim3 grid = grid_of(blocks_for(rows, K, shortrow));
     #define MX4_D(DT, L) \
         hipLaunchKernelGGL((dequantize_kernel<DT, L>), grid, dim3(256), 0, \
                            stream, codes, scales, rows, (int)K, \

@@ -78,3 +78,33 @@ def test_clipping_refuses_forward_mode_derivatives(device):
             with pytest.raises(NotImplementedError, match='forward-mode'):
                 call()
     assert not out.any()
+
+
+@pytest.mark.gpu
+def test_more_blocks_than_one_axis_of_a_launch():
+    """2^28 rows of 129: 2^24 blocks of 256 threads, rounded alone and beside
+    a weight, and read back."""
+    R, K = 2 ** 28 + 5, 129
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 200 * 2 ** 30:
+        pytest.skip('needs 200 GiB')
+    x = torch.empty(R, K, device='cuda', dtype=torch.bfloat16).normal_()
+    # ends, and around the rows of block 2^23, where a second axis begins
+    parts = [slice(0, 40), slice(2 ** 27 - 40, 2 ** 27 + 40),
+             slice(R - 40, R)]
+    small = [ops.mx4_quantize(x[p].clone()) for p in parts]
+    q = ops.mx4_quantize(x)
+    for p, s in zip(parts, small):
+        assert torch.equal(q.codes[:, p], s.codes)
+        assert torch.equal(q.scales[:, p], s.scales)
+    v = q.dequantize()
+    for p, s in zip(parts, small):
+        assert torch.equal(v[p], s.dequantize())
+    del v, q
+    w = torch.randn(1, K, device='cuda', requires_grad=True)
+    y = ops.mx4_linear(x, w)
+    for p in parts:
+        a, b = values(x[p]), values(w)
+        assert_close(y[p], a @ b.t(), a.abs() @ b.abs().t(), K)
+    del x, y, small
+    torch.cuda.empty_cache()
