@@ -4,6 +4,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -61,6 +62,9 @@ at::ScalarType scalar_type(int64_t dt) {
 Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
     return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
 }
+
+// A launch that was refused raises here, instead of leaving what the memory held.
+void check_launches() { C10_HIP_CHECK(hipGetLastError()); }
 
 hipStream_t current_stream() { return at::hip::getCurrentHIPStream(); }
 
@@ -139,6 +143,7 @@ Packed pack(const Tensor& x2, int dt) {
     mx4::quantize(x2.data_ptr(), dt, R, K, row_stride(x2),
                   p.codes.data_ptr<uint8_t>(), p.scales.data_ptr<uint8_t>(),
                   current_stream());
+    check_launches();
     return p;
 }
 
@@ -158,6 +163,7 @@ Tensor dequantize(const Tensor& codes, const Tensor& scales, int64_t K,
     mx4::dequantize(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(),
                     codes.size(1), K, out.data_ptr(), (int)dt,
                     current_stream());
+    check_launches();
     return out;
 }
 
@@ -211,6 +217,7 @@ Tensor linear(const Tensor& x, const Tensor& wc, const Tensor& ws, int64_t K,
     mx4::linear(x2.data_ptr(), dt, M, K, ldx, wc.data_ptr<uint8_t>(),
                 ws.data_ptr<uint8_t>(), N, b.ptr(), b.dt, y.data_ptr(), f,
                 work.defined() ? work.data_ptr() : nullptr, current_stream());
+    check_launches();
     return y;
 }
 
@@ -227,6 +234,7 @@ Tensor product_q(const Tensor& xc, const Tensor& xs, int64_t K,
     mx4::linear_q(xc.data_ptr<uint8_t>(), xs.data_ptr<uint8_t>(), M, K,
                   wc.data_ptr<uint8_t>(), ws.data_ptr<uint8_t>(), N, b.ptr(),
                   b.dt, y.data_ptr(), dt, f, current_stream());
+    check_launches();
     return y;
 }
 
@@ -263,6 +271,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_train(
         x2.data_ptr(), dt, x2.size(0), row_stride(x2),
         px.codes.data_ptr<uint8_t>(), px.scales.data_ptr<uint8_t>(), K,
         current_stream());
+    check_launches();
     Tensor y = product_q(px.codes, px.scales, K, pw.codes, pw.scales, bias,
                          shape_of(x, w.size(0)), dt, -1);
     return {y, px.codes, px.scales, pw.codes, pw.scales};
@@ -324,6 +333,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
         work = workspace(bytes, g);
     mx4::grads(a, (int)form, work.defined() ? work.data_ptr() : nullptr,
                current_stream());
+    check_launches();
     return {dx, dw, db};
 }
 
@@ -493,6 +503,7 @@ Tensor grad_norm(const std::vector<Tensor>& grads, double p) {
     auto work = fresh({(int64_t)list.workspace_doubles()}, at::kDouble, norm);
     list.norm(kind, norm.data_ptr<float>(), work.data_ptr<double>(),
               current_stream());
+    check_launches();
     return norm;
 }
 
@@ -535,6 +546,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
     auto work = fresh({(int64_t)list.workspace_doubles()}, at::kDouble, norm);
     list.clip(kind, max_norm, norm.data_ptr<float>(), work.data_ptr<double>(),
               current_stream());
+    check_launches();
     for (const auto& o : outs)           // written behind autograd's back
         if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     return norm;

@@ -108,3 +108,37 @@ def test_more_blocks_than_one_axis_of_a_launch():
         assert_close(y[p], a @ b.t(), a.abs() @ b.abs().t(), K)
     del x, y, small
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('call', ['quantize', 'dequantize', 'held', 'few',
+                                  'train', 'backward', 'norm', 'clip'])
+def test_errors_of_launches_are_reported(call):
+    """Every entry point asks for the runtime's last error after its launches;
+    here it is one that a host call left."""
+    import ctypes
+    hip = ctypes.CDLL('libamdhip64.so')
+    ext = ops._native_or_die()
+    x, w = (torch.randn(40, 64, device='cuda') for _ in range(2))
+    q = ops.mx4_quantize(w)
+    y = torch.empty(40, 40, device='cuda')
+    ws = w.clone().requires_grad_()
+    calls = {
+        'quantize': lambda: ops.mx4_quantize(x),
+        'dequantize': lambda: q.dequantize(),
+        'held': lambda: ops.mx4_linear(x, q),
+        'few': lambda: ext.mx4_linear_q(q.codes, q.scales, 64, q.codes,
+                                        q.scales, None, 0),
+        'train': lambda: ops.mx4_linear(x, ws),
+        'backward': lambda: ext.mx4_linear_backward(
+            y, q.codes, q.scales, q.codes, q.scales, 64, 0, 0, 0),
+        'norm': lambda: ops.grad_norm([x, w]),
+        'clip': lambda: ops.clip_grads_([x, w], 1.0)}
+    for c in calls.values():
+        c()
+    torch.cuda.synchronize()
+    assert hip.hipGetDeviceCount(None) != 0       # no place for the result
+    with pytest.raises(RuntimeError, match='invalid argument'):
+        calls[call]()
+    calls[call]()                                 # it is reported once
+    torch.cuda.synchronize()
