@@ -18,9 +18,10 @@ Capture constraints and how they are met:
   calls run eagerly on a side stream (they are REAL training steps);
 * Adam must be constructed with ``capturable=True`` (train.py does when
   graphs are enabled);
-* phase flips (warm<->joint optimizer swap, mining on, EM on) change the
-  captured program — the step signature is checked per call and the graph
-  is re-captured when it changes (a handful of times per run);
+* phase flips (warm<->joint optimizer swap, mining on, EM on), another
+  ``clip_grad_norm`` and ``use_mx4``/``no_mx4`` change the captured
+  program — the step signature is checked per call and the graph is
+  re-captured when it changes (a handful of times per run);
 * the EM update runs INLINE in the graph (no side stream: cross-stream
   event sync inside capture is legal but buys nothing when every step
   runs EM);
@@ -42,6 +43,7 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from ..models.conv1x1 import GemmConv2d
 from ..utils.graphs import capture_graph
 
 
@@ -101,7 +103,10 @@ class GraphedStep:
     # ------------------------------------------------------------------
     def _signature(self, optimizer, use_mine, em_active):
         return (id(optimizer), bool(use_mine), bool(em_active),
-                tuple(p.requires_grad for p in self.model.parameters()))
+                self.clip_grad_norm,
+                tuple(p.requires_grad for p in self.model.parameters()),
+                tuple(m.mx4 for m in self.model.modules()
+                      if isinstance(m, GemmConv2d)))
 
     def matches(self, image, optimizer, use_mine, em_active) -> bool:
         """Can this batch go through the graphed path (possibly after a

@@ -142,3 +142,39 @@ def test_errors_of_launches_are_reported(call):
         calls[call]()
     calls[call]()                                 # it is reported once
     torch.cuda.synchronize()
+
+
+def _captured(net):
+    from mgproto_amd.engine.graphstep import GraphedStep
+    gs = GraphedStep(net, None, {}, torch.device('cpu'), 2, 8,
+                     channels_last=False)
+    opt = torch.optim.SGD(net.parameters(), lr=0.1)
+    x = torch.zeros(2, 3, 8, 8)
+
+    def kept():
+        before = gs.graph = object()              # as if it were captured
+        assert gs.matches(x, opt, True, False)
+        return gs.graph is before
+
+    kept()
+    assert kept()
+    return gs, kept
+
+
+def test_a_captured_step_knows_its_clipping_and_its_layers():
+    from mgproto_amd.models import no_mx4
+    net = torch.nn.Sequential(GemmConv2d(3, 4, 1), torch.nn.ReLU(),
+                              GemmConv2d(4, 4, 1))
+    gs, kept = _captured(net)
+    gs.clip_grad_norm = 1.0
+    assert not kept() and kept()
+    gs.clip_grad_norm = 0.5
+    assert not kept() and kept()
+    use_mx4(net, train=True)
+    assert not kept() and kept()
+    use_mx4(net[2], train=True)                   # as it was
+    assert kept()
+    no_mx4(net[0])
+    assert not kept() and kept()
+    use_mx4(net[2])
+    assert not kept() and kept()
