@@ -84,6 +84,10 @@ def _training(model, dataloader, optimizer=None, aux_criterion=None,
               clip_grad_norm=None):
     device = device or next(_unwrap(model).parameters()).device
     m = _unwrap(model)
+    if graph_step is not None and graph_step.clip_grad_norm != clip_grad_norm:
+        # full batches would be clipped by the one, others by the other
+        raise ValueError(f'clip_grad_norm {clip_grad_norm}, but '
+                         f'{graph_step.clip_grad_norm} in the captured step')
     start = time.time()
 
     n_examples = torch.zeros((), device=device)

@@ -178,3 +178,14 @@ def test_a_captured_step_knows_its_clipping_and_its_layers():
     assert not kept() and kept()
     use_mx4(net[2])
     assert not kept() and kept()
+
+
+@pytest.mark.parametrize('here,there', [(1.0, None), (None, 1.0), (1.0, 2.0)])
+def test_a_captured_step_clips_as_the_trainer(here, there):
+    from mgproto_amd.engine import trainer
+    net = torch.nn.Sequential(GemmConv2d(3, 4, 1))
+    gs, _ = _captured(net)
+    gs.clip_grad_norm = there
+    with pytest.raises(ValueError, match='clip_grad_norm'):
+        trainer._training(net, [], device=torch.device('cpu'), graph_step=gs,
+                          clip_grad_norm=here)
