@@ -18,9 +18,9 @@ Capture constraints and how they are met:
   calls run eagerly on a side stream (they are REAL training steps);
 * Adam must be constructed with ``capturable=True`` (train.py does when
   graphs are enabled);
-* phase flips (warm<->joint optimizer swap, mining on, EM on), another
-  ``clip_grad_norm`` and ``use_mx4``/``no_mx4`` change the captured
-  program — the step signature is checked per call and the graph is
+* phase flips (warm<->joint optimizer swap, mining on, EM on), other loss
+  weights, another learning rate or ``clip_grad_norm``, and
+  ``use_mx4``/``no_mx4`` change the captured program — the step signature is checked per call and the graph is
   re-captured when it changes (a handful of times per run);
 * the EM update runs INLINE in the graph (no side stream: cross-stream
   event sync inside capture is legal but buys nothing when every step
@@ -104,6 +104,11 @@ class GraphedStep:
     def _signature(self, optimizer, use_mine, em_active):
         return (id(optimizer), bool(use_mine), bool(em_active),
                 self.clip_grad_norm,
+                # numbers are part of the program, tensors are read by it
+                tuple(sorted((k, v) for k, v in self.coefs.items())),
+                tuple((k, v) for g in optimizer.param_groups
+                      for k, v in g.items()
+                      if isinstance(v, (bool, int, float, tuple))),
                 tuple(p.requires_grad for p in self.model.parameters()),
                 tuple(m.mx4 for m in self.model.modules()
                       if isinstance(m, GemmConv2d)))

@@ -189,3 +189,33 @@ def test_a_captured_step_clips_as_the_trainer(here, there):
     with pytest.raises(ValueError, match='clip_grad_norm'):
         trainer._training(net, [], device=torch.device('cpu'), graph_step=gs,
                           clip_grad_norm=here)
+
+
+def test_a_captured_step_follows_the_learning_rate():
+    from mgproto_amd.engine.graphstep import GraphedStep
+    net = torch.nn.Linear(4, 4)
+    gs = GraphedStep(net, None, {'aux': 0.5, 'crs_ent': 1.0},
+                     torch.device('cpu'), 2, 8, channels_last=False)
+    opt = torch.optim.Adam([{'params': [net.weight], 'lr': 0.1},
+                            {'params': [net.bias]}])
+    decay = torch.optim.lr_scheduler.StepLR(opt, 1, 0.4)
+    x = torch.zeros(2, 3, 8, 8)
+
+    def kept():
+        before = gs.graph = object()
+        assert gs.matches(x, opt, True, False)
+        return gs.graph is before
+
+    kept()
+    assert kept()
+    opt.step()
+    decay.step()
+    assert not kept() and kept()
+    opt.param_groups[1]['weight_decay'] = 1e-4
+    assert not kept() and kept()
+    gs.coefs['aux'] = 0.25
+    assert not kept() and kept()
+    opt.param_groups[0]['lr'] = torch.tensor(0.1)     # read by the step
+    kept()
+    opt.param_groups[0]['lr'].mul_(0.5)
+    assert kept()
