@@ -209,13 +209,24 @@ void finish_kernel(const double* __restrict__ part, int n,
     norm[0] = (float)root<KIND>(v);
 }
 
-// one rounding, from 64 bits where either type has 32
+// 64 bits where either type has 32, rounded once: on the way to 16 bits the 32 in
+// between are rounded to odd (by truncation, the last bit set where something was
+// lost), which keeps an element next to the middle of two values on its side.
 template <int SD, int DD>
 static __device__ __forceinline__ typename Type<DD>::T scaled(
         typename Type<SD>::T v, double f, float f32) {
-    if constexpr (SD == F32 || DD == F32)
-        return (typename Type<DD>::T)(float)((double)(float)v * f);
-    else return (typename Type<DD>::T)((float)v * f32);
+    if constexpr (SD == F32 || DD == F32) {
+        const double d = (double)(float)v * f;
+        float r = (float)d;
+        if constexpr (DD != F32) {
+            if ((double)r != d) {
+                unsigned b = __float_as_uint(r);
+                b -= __builtin_fabs((double)r) > __builtin_fabs(d);
+                r = __uint_as_float(b | 1u);
+            }
+        }
+        return (typename Type<DD>::T)r;
+    } else return (typename Type<DD>::T)((float)v * f32);
 }
 
 template <int SD, int DD>

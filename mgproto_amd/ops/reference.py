@@ -467,10 +467,22 @@ def _check_written(grads, outs):
             out_end = max(out_end, end)
 
 
+def _round_once(v: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """float64 to the nearest value of a type. torch goes to 16 bits by way of
+    32; rounded to odd there, an element next to the middle of two values stays
+    on its side."""
+    f = v.float()
+    if dtype == torch.float32:
+        return f
+    bits = f.view(torch.int32)
+    odd = torch.where(f.double().abs() > v.abs(), bits - 1, bits) | 1
+    return torch.where(f.double() == v, bits, odd).view(torch.float32).to(dtype)
+
+
 def clip_grads(grads, outs, max_norm: float, p: float) -> torch.Tensor:
     norm = grad_norm(grads, p)
     factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
     _check_written(grads, outs)
     for g, o in zip(grads, outs):
-        o.copy_((g.double() * factor).to(o.dtype))
+        o.copy_(_round_once(g.double() * factor, o.dtype))
     return norm.float()

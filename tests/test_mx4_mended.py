@@ -219,3 +219,43 @@ def test_a_captured_step_follows_the_learning_rate():
     kept()
     opt.param_groups[0]['lr'].mul_(0.5)
     assert kept()
+
+
+def _nearest(v, dtype):
+    """float64 -> the nearest value of a 16-bit type, ties to even, with no
+    type in between; normal numbers."""
+    bits = 8 if dtype == torch.bfloat16 else 11
+    m, e = torch.frexp(v)
+    return torch.ldexp(torch.round(m * 2.0 ** bits), e - bits)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_wide_gradients_are_rounded_once(dtype, device):
+    half = torch.finfo(dtype).eps / 2
+    # alone, the element becomes max_norm (1 - 1e-6 / v): a billionth below the
+    # middle of two values, which 32 bits cannot tell from it
+    for sign in (1, -1):
+        for middle, want in ((1 + 3 * half, 1 + 2 * half), (1 + half, 1.0)):
+            g = torch.zeros(5000, device=device)
+            g[4321] = sign * 2.0 ** 20
+            out = torch.empty(5000, device=device, dtype=dtype)
+            ops.clip_grads_([g], middle, out=[out])
+            assert float(out[4321]) == sign * want
+            assert int((out != 0).sum()) == 1
+    g = torch.randn(300, 41, device=device)
+    out = torch.empty_like(g, dtype=dtype)
+    norm = float(g.double().norm())
+    ops.clip_grads_([g], 100 * norm / 3e2, out=[out])
+    v = g.double().cpu() * (100 * norm / 3e2 / (
+        float(g.cpu().double().square().sum()) ** 0.5 + 1e-6))
+    # where the factor's last bits decide, either neighbour
+    lo, hi = (_nearest(v * (1 + s * 2.0 ** -50), dtype) for s in (-1, 1))
+    got = out.double().cpu()
+    tiny = v.abs() < torch.finfo(dtype).tiny
+    assert ((got == lo) | (got == hi) | tiny).all()
+    # infinities and numbers past the type
+    g = torch.tensor([3e38, -3e38, 1.0], device=device)
+    out = torch.empty(3, device=device, dtype=dtype)
+    ops.clip_grads_([g], math.inf, out=[out])
+    assert torch.equal(out.cpu(), torch.tensor([3e38, -3e38, 1.0]).to(dtype))
