@@ -211,10 +211,14 @@ void finish_kernel(const double* __restrict__ part, int n,
 
 // 64 bits where either type has 32, rounded once: on the way to 16 bits the 32 in
 // between are rounded to odd (by truncation, the last bit set where something was
-// lost), which keeps an element next to the middle of two values on its side.
+// lost), which keeps an element next to the middle of two values on its side. From 16
+// bits to 16, the factor f = m 2^e is rounded to 32 (m, between 1/2 and 1) and so is
+// the product: two times 2^-24 beside the result's 2^-9 or 2^-12. Its exponent comes
+// last: the norm of bf16 gradients may pass 2^128, and the factor then lies below
+// what 32 bits hold, where the products need not.
 template <int SD, int DD>
 static __device__ __forceinline__ typename Type<DD>::T scaled(
-        typename Type<SD>::T v, double f, float f32) {
+        typename Type<SD>::T v, double f, float m, int e) {
     if constexpr (SD == F32 || DD == F32) {
         const double d = (double)(float)v * f;
         float r = (float)d;
@@ -226,7 +230,7 @@ static __device__ __forceinline__ typename Type<DD>::T scaled(
             }
         }
         return (typename Type<DD>::T)r;
-    } else return (typename Type<DD>::T)((float)v * f32);
+    } else return (typename Type<DD>::T)__builtin_ldexpf((float)v * m, e);
 }
 
 template <int SD, int DD>
@@ -237,7 +241,8 @@ static __device__ __forceinline__ void scale_chunk(const void* src, void* dst,
     constexpr int E = 16 / sizeof(S);
     const S* p = reinterpret_cast<const S*>(src) + at;
     D* q = reinterpret_cast<D*>(dst) + at;
-    const float f32 = (float)f;
+    int e = 0;
+    const float m = (float)frexp(f, &e);
     if (n == elements(SD)) {
         Unit<SD, E> u[LOADS];
         #pragma unroll
@@ -246,7 +251,7 @@ static __device__ __forceinline__ void scale_chunk(const void* src, void* dst,
         for (int i = 0; i < LOADS; ++i) {
             Unit<DD, E> o;
             #pragma unroll
-            for (int e = 0; e < E; ++e) o.v[e] = scaled<SD, DD>(u[i].v[e], f, f32);
+            for (int j = 0; j < E; ++j) o.v[j] = scaled<SD, DD>(u[i].v[j], f, m, e);
             o.store(q + (i * 256 + threadIdx.x) * E);
         }
         return;
@@ -257,11 +262,11 @@ static __device__ __forceinline__ void scale_chunk(const void* src, void* dst,
         Unit<DD, E> o;
         u.load(p + i * E);
         #pragma unroll
-        for (int e = 0; e < E; ++e) o.v[e] = scaled<SD, DD>(u.v[e], f, f32);
+        for (int j = 0; j < E; ++j) o.v[j] = scaled<SD, DD>(u.v[j], f, m, e);
         o.store(q + i * E);
     }
     const int i = whole * E + threadIdx.x;
-    if (i < n) q[i] = scaled<SD, DD>(p[i], f, f32);
+    if (i < n) q[i] = scaled<SD, DD>(p[i], f, m, e);
 }
 
 template <int KIND, int T>

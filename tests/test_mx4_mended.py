@@ -259,3 +259,27 @@ def test_wide_gradients_are_rounded_once(dtype, device):
     out = torch.empty(3, device=device, dtype=dtype)
     ops.clip_grads_([g], math.inf, out=[out])
     assert torch.equal(out.cpu(), torch.tensor([3e38, -3e38, 1.0]).to(dtype))
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('to', [torch.bfloat16, torch.float16, torch.float32])
+def test_norms_past_the_range_of_32_bits(to, device):
+    """The factor is below the smallest fp32 number, what it gives is not."""
+    n, m = 4096, 4096 * 5 + 3
+    g = [torch.full((n,), 2.0 ** 127, device=device, dtype=torch.bfloat16),
+         torch.randn(m, device=device).mul(1e37).bfloat16()]
+    norm = math.sqrt(sum(float((t.double().cpu() * 2.0 ** -127).square().sum())
+                         for t in g)) * 2.0 ** 127
+    assert norm > 2.0 ** 132
+    for max_norm in (1.0, 2.0 ** -20):
+        outs = [torch.empty_like(t, dtype=to) for t in g]
+        assert float(ops.clip_grads_(g, max_norm, out=outs)) == math.inf
+        f = max_norm / (norm + 1e-6)
+        h = torch.finfo(to).eps / 2
+        for o, t in zip(outs, g):
+            want = t.double().cpu() * f
+            # the factor and its product, both in 32 bits; the rounding, or
+            # half of the smallest step
+            tol = want.abs() * (h + 2.0 ** -23) * (1 + h) + \
+                torch.finfo(to).tiny * h
+            assert ((o.double().cpu() - want).abs() <= tol).all()
