@@ -446,21 +446,27 @@ void check_list(const std::vector<Tensor>& ts, const char* what) {
     }
 }
 
+// the end of a tensor's memory; gaps count
+uintptr_t end_of(const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return (uintptr_t)t.data_ptr() + (last + 1) * t.element_size();
+}
+
 // A written tensor may share memory with no other one, but for its own source
-// in the same place and of the same type.
-void check_apart(const std::vector<gradclip::Item>& items) {
+// within its own place, in the same type.
+void check_apart(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs) {
     struct Span { uintptr_t lo, hi; size_t i; bool out; };
     std::vector<Span> s;
-    s.reserve(items.size() * 2);
-    auto width = [](int dt) { return dt == mx4::F32 ? 4 : 2; };
-    for (size_t i = 0; i < items.size(); ++i) {
-        const auto& it = items[i];
-        if (!it.n) continue;
-        s.push_back({(uintptr_t)it.dst,
-                     (uintptr_t)it.dst + it.n * width(it.dst_dt), i, true});
-        if (it.src != it.dst || it.src_dt != it.dst_dt)
-            s.push_back({(uintptr_t)it.src,
-                         (uintptr_t)it.src + it.n * width(it.src_dt), i, false});
+    s.reserve(grads.size() * 2);
+    for (size_t i = 0; i < grads.size(); ++i) {
+        const Tensor &g = grads[i], &o = outs[i];
+        if (!o.numel()) continue;
+        const uintptr_t lo = (uintptr_t)o.data_ptr(), hi = end_of(o);
+        s.push_back({lo, hi, i, true});
+        if ((uintptr_t)g.data_ptr() != lo || g.scalar_type() != o.scalar_type() ||
+            end_of(g) > hi)
+            s.push_back({(uintptr_t)g.data_ptr(), end_of(g), i, false});
     }
     std::sort(s.begin(), s.end(),
               [](const Span& a, const Span& b) { return a.lo < b.lo; });
@@ -540,7 +546,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads,
                          dtype_code(g, "clip_grads_"),
                          dtype_code(o, "clip_grads_: out")});
     }
-    check_apart(items);
+    check_apart(grads, outs);
     auto norm = fresh({}, at::kFloat, grads[0]);
     const gradclip::List list(items);
     auto work = fresh({(int64_t)list.workspace_doubles()}, at::kDouble, norm);

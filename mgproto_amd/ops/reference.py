@@ -443,25 +443,30 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _end(t: torch.Tensor) -> int:
+    """The end of a tensor's memory; gaps count."""
+    return t.data_ptr() + t.element_size() * (1 + sum(
+        (n - 1) * st for n, st in zip(t.shape, t.stride())))
+
+
 def _check_written(grads, outs):
     """A written tensor may share memory with no other one, but for its own
-    source in the same place and of the same type."""
+    source within its own place, in the same type."""
     spans = []
     for i, (g, o) in enumerate(zip(grads, outs)):
         if not _dense(o):
             raise RuntimeError(f'clip_grads_: tensor {i} is written and has '
                                'gaps or shares elements with itself')
         if o.numel():
-            spans.append((o.data_ptr(), i, True, o))
-            if g.data_ptr() != o.data_ptr() or g.dtype != o.dtype:
-                spans.append((g.data_ptr(), i, False, g))
+            spans.append((o.data_ptr(), i, True, _end(o)))
+            if (g.data_ptr() != o.data_ptr() or g.dtype != o.dtype
+                    or _end(g) > _end(o)):
+                spans.append((g.data_ptr(), i, False, _end(g)))
     any_end = out_end = 0
-    for lo, i, written, t in sorted(spans, key=lambda e: e[0]):
+    for lo, i, written, end in sorted(spans, key=lambda e: e[0]):
         if lo < out_end or written and lo < any_end:
             raise RuntimeError('clip_grads_: a tensor that is written shares '
                                f'memory with another one (number {i})')
-        end = lo + t.element_size() * (1 + sum(
-            (n - 1) * st for n, st in zip(t.shape, t.stride())))
         any_end = max(any_end, end)
         if written:
             out_end = max(out_end, end)

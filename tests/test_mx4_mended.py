@@ -283,3 +283,33 @@ def test_norms_past_the_range_of_32_bits(to, device):
             tol = want.abs() * (h + 2.0 ** -23) * (1 + h) + \
                 torch.finfo(to).tiny * h
             assert ((o.double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_gradients_of_other_strides_are_checked_for_overlap(device):
+    """Before they are copied: both forms refuse what both promise to."""
+    keep = torch.randn(60, device=device)
+    rows = lambda t, lo: t[lo:lo + 20].view(4, 5)  # noqa: E731
+    calls = [
+        # a transposed gradient that another output is written over
+        lambda t: ([rows(t, 0).t(), rows(t, 20).t()],
+                   [rows(t, 40).view(5, 4), rows(t, 10).view(5, 4)]),
+        # one with gaps, from its own output's place into another's
+        lambda t: ([t[40:50], t[:20:2]], [t[10:20], t[:10]]),
+        lambda t: ([t[:20:2], t[40:50]], [t[:10], t[10:20]]),
+        # its own output, but not from the same place on
+        lambda t: ([rows(t, 2).t()], [rows(t, 0).view(5, 4)])]
+    for call in calls:
+        t = keep.clone()
+        grads, outs = call(t)
+        with pytest.raises(RuntimeError, match='shares'):
+            ops.clip_grads_(grads, 0.1, out=outs)
+        assert torch.equal(t, keep)
+    # a turned view of itself is its own source
+    t = keep.clone()
+    grads, outs = [t[:25].view(5, 5).t()], [t[:25].view(5, 5)]
+    want = keep[:25].view(5, 5).t()
+    norm = float(want.double().norm())
+    ops.clip_grads_(grads, 2 * norm, out=outs)
+    assert torch.equal(t[:25].view(5, 5), want)
+    assert torch.equal(t[25:], keep[25:])
