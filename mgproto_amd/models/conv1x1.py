@@ -84,7 +84,11 @@ class GemmConv2d(nn.Conv2d):
                 # not in the state dict: made from the weight again
                 self.register_buffer('_mx4_codes', q.codes, persistent=False)
                 self.register_buffer('_mx4_scales', q.scales, persistent=False)
-        self._mx4_of = weakref.ref(self.weight), _state(self.weight)
+        if self.weight.is_cuda and torch.cuda.is_current_stream_capturing():
+            # recorded, not done: the next forward makes them in earnest
+            self._mx4_of = _nothing, None
+        else:
+            self._mx4_of = weakref.ref(self.weight), _state(self.weight)
 
     def _mx4_weight(self):
         if self.mx4 == 'train':

@@ -313,3 +313,24 @@ def test_gradients_of_other_strides_are_checked_for_overlap(device):
     ops.clip_grads_(grads, 2 * norm, out=outs)
     assert torch.equal(t[:25].view(5, 5), want)
     assert torch.equal(t[25:], keep[25:])
+
+
+@pytest.mark.gpu
+def test_codes_made_in_a_capture_are_made_again_outside():
+    """A capture records the rounding of a changed weight and does not do it."""
+    conv = GemmConv2d(32, 8, 1).cuda()
+    use_mx4(conv)
+    x = torch.randn(2, 32, 3, 3, device='cuda')
+    with torch.no_grad():
+        conv(x)
+        conv.weight.normal_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = conv(x)
+        _check_layer(conv, x)                     # eager, before any replay
+        for _ in range(3):
+            conv.weight.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, conv(x))
+            _check_layer(conv, x)
