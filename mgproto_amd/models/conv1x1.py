@@ -113,14 +113,17 @@ class GemmConv2d(nn.Conv2d):
         return state
 
     def _mx4_forward(self, x):
+        if x.dim() not in (3, 4):
+            raise ValueError(f'an image [C, H, W] or a batch [N, C, H, W], '
+                             f'not {tuple(x.shape)}')
         kind = x.device.type
         if torch.is_autocast_enabled(kind):
             x = x.to(torch.get_autocast_dtype(kind))
         sh, sw = self.stride
         # NHWC rows: a view of a channels-last tensor, strided ones copied
-        rows = x[:, :, ::sh, ::sw].permute(0, 2, 3, 1)
+        rows = x[..., ::sh, ::sw].movedim(-3, -1)
         y = ops.mx4_linear(rows, self._mx4_weight(), self.bias)
-        return y.permute(0, 3, 1, 2)                   # channels_last NCHW
+        return y.movedim(-1, -3)                       # channels_last NCHW
 
 
 def _state(w: torch.Tensor):

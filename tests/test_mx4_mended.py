@@ -334,3 +334,20 @@ def test_codes_made_in_a_capture_are_made_again_outside():
             torch.cuda.synchronize()
             assert torch.equal(y, conv(x))
             _check_layer(conv, x)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('stride', [1, 2])
+def test_single_images(stride, device):
+    """Convolutions take an image without a batch axis, 4-bit ones too."""
+    conv = GemmConv2d(40, 24, 1, stride=stride).to(device)
+    x = torch.randn(1, 40, 7, 5, device=device)
+    shape = conv(x[0]).shape
+    for train in (False, True):
+        use_mx4(conv, train=train)
+        with torch.no_grad():
+            assert conv(x[0]).shape == shape
+            assert torch.equal(conv(x[0]), conv(x)[0])
+        for bad in (x[0, 0], x[None]):
+            with pytest.raises(ValueError, match='an image'):
+                conv(bad)
