@@ -166,7 +166,7 @@ def no_mx4(module: nn.Module):
     """The reverse of ``use_mx4``."""
     for m in module.modules():
         if isinstance(m, GemmConv2d) and m.mx4 is not None:
-            if m.mx4 == 'held':
+            if hasattr(m, '_mx4_codes'):    # held now, or before training
                 del m._mx4_codes, m._mx4_scales, m._mx4_of
             m.mx4 = None
 

@@ -351,3 +351,16 @@ def test_single_images(stride, device):
         for bad in (x[0, 0], x[None]):
             with pytest.raises(ValueError, match='an image'):
                 conv(bad)
+
+
+def test_no_mx4_leaves_nothing_behind():
+    from mgproto_amd.models import no_mx4
+    conv = GemmConv2d(32, 8, 1)
+    before = set(vars(conv)), list(conv.buffers())
+    for modes in ((False,), (True,), (False, True), (True, False),
+                  (False, True, False)):
+        for train in modes:
+            use_mx4(conv, train=train)
+        no_mx4(conv)
+        assert not list(conv.buffers())
+        assert set(vars(conv)) - before[0] <= {'mx4'} and conv.mx4 is None
