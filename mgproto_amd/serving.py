@@ -32,9 +32,12 @@ class InferenceEngine:
         if weights not in ('float', 'mx4'):
             raise ValueError(f"weights 'float' or 'mx4', not {weights!r}")
         self.model = model.eval()
-        self.weights = weights
-        if weights == 'mx4':
-            use_mx4(self.model.features)
+        if weights == 'mx4' and not use_mx4(self.model.features):
+            raise ValueError("weights 'mx4': this backbone has no 1x1 "
+                             'convolutions')
+        # what is served: a model may come with 4-bit layers
+        self.weights = 'mx4' if any(getattr(m, 'mx4', None) for m in
+                                    self.model.modules()) else 'float'
         self.device = device or next(model.parameters()).device
         self.amp = amp and self.device.type == 'cuda'
         self._graph = None

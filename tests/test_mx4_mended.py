@@ -364,3 +364,24 @@ def test_no_mx4_leaves_nothing_behind():
         no_mx4(conv)
         assert not list(conv.buffers())
         assert set(vars(conv)) - before[0] <= {'mx4'} and conv.mx4 is None
+
+
+def test_serving_says_what_it_serves():
+    from mgproto_amd.model import construct_MGProto
+    from mgproto_amd.serving import InferenceEngine
+
+    def engine(arch, weights, mx4=False):
+        m = construct_MGProto(arch, pretrained=False, img_size=64,
+                              prototype_shape=(20, 16, 1, 1), num_classes=5,
+                              add_on_layers_type='regular', sz_embedding=8,
+                              mem_capacity=8, mine_K=3)
+        if mx4:
+            use_mx4(m.features, train=True)
+        return InferenceEngine(m, torch.device('cpu'), weights=weights)
+
+    assert engine('resnet50', 'float').weights == 'float'
+    assert engine('resnet50', 'mx4').weights == 'mx4'
+    assert engine('resnet50', 'float', mx4=True).weights == 'mx4'
+    assert engine('vgg11', 'float').weights == 'float'
+    with pytest.raises(ValueError, match='no 1x1'):
+        engine('vgg11', 'mx4')
