@@ -39,7 +39,7 @@ static __device__ __forceinline__ void copy16_to_lds(const void* base,
                                                      unsigned off, unsigned l) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\t"
                  "global_load_lds_dwordx4 %0, %1"
-                 :: "v"(off), "s"(base), "s"(l) : "memory");
+                 :: "v"(off), "s"(base), "s"(l) : "memory", "m0");
 }
 // until at most N of this wave's memory instructions are under way (they end
 // in their order), and its reads of LDS are over
