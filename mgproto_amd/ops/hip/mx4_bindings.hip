@@ -571,8 +571,6 @@ void register_mx4(pybind11::module& m) {
           py::arg("codes"), py::arg("scales"), py::arg("bias"),
           py::arg("dtype"), py::arg("form") = -1);
     m.def("mx4_linear_float", &linear_float, "Q(x) Q(w)^T + bias");
-    m.def("mx4_linear_train", &linear_train,
-          "Q(x) Q(w)^T + bias, and the rounded x and w");
     m.def("mx4_linear_backward", &linear_backward,
           "gradients to the input, the weight and the bias", py::arg("grad"),
           py::arg("codes"), py::arg("scales"), py::arg("xcodes"),

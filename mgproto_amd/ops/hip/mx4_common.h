@@ -53,10 +53,6 @@ static __device__ __forceinline__ float scale_f32(unsigned byte) {
     return __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
 
-// The 32 elements of one block as they are loaded: 16 words of two 16-bit
-// elements, or 32 words.
-template <int DT> struct Raw32 { u32x4 u[DT == F32 ? 8 : 4]; };
-
 // max|x| of packed 16-bit floats by their bits (the order of the absolute
 // bits is the order of the values, infinities and NaN on top)
 static __device__ __forceinline__ u16x2 absmax16(u16x2 m, unsigned w) {
