@@ -2,7 +2,8 @@
 product, on the matrix cores that take them directly.
 
 * ``mx4_quantize(x)`` rounds the last axis to blocks -> ``MX4Tensor``;
-* ``MX4Tensor.dequantize()`` reads it back (exact in bf16 and fp32);
+* ``MX4Tensor.dequantize()`` reads it back (bf16 and fp32 hold every value
+  below 2^128, and so all that ``mx4_quantize`` makes);
 * ``mx4_linear(x, weight, bias)`` is ``Q(x) Q(weight)^T + bias`` with fp32
   sums. A held ``MX4Tensor`` weight serves; a float weight is rounded in the
   call and trains: the gradients are straight-through,
@@ -81,7 +82,9 @@ class MX4Tensor:
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor,
                    dtype: torch.dtype = torch.bfloat16) -> 'MX4Tensor':
         """From codes [..., K/2] and scales [..., K/32] in plain order, K a
-        multiple of 32, as other programs store them."""
+        multiple of 32, as other programs store them. Values of 2^128 and more
+        (scales 2^126 and 2^127 can make them, ``mx4_quantize`` does not) are
+        refused: neither bf16 nor fp32 holds them. Waits for the GPU."""
         K = codes.shape[-1] * 2
         if K % 32 or scales.shape != (*codes.shape[:-1], K // 32):
             raise ValueError(
@@ -89,9 +92,16 @@ class MX4Tensor:
                 f'{tuple(scales.shape)} are not blocks of 32')
         shape = (*codes.shape[:-1], K)
         R = math.prod(shape[:-1])
-        return cls(*reference.mx4_arrange(codes.reshape(R, K // 2),
-                                          scales.reshape(R, K // 32)),
-                   shape, dtype)
+        q = cls(*reference.mx4_arrange(codes.reshape(R, K // 2),
+                                       scales.reshape(R, K // 32)),
+                shape, dtype)
+        # the largest code of a block: 6 stands for 4, 4 for 2
+        top = torch.maximum(codes & 7, codes >> 4 & 7).reshape(R, K // 32, 16)
+        if R * K:
+            top, of = top.amax(2), scales.reshape(R, K // 32)
+            if ((of == 253) & (top >= 6) | (of == 254) & (top >= 4)).any():
+                raise ValueError('MX4Tensor: a value of 2^128 or more')
+        return q
 
     def parts(self):
         """(codes [..., K/2], scales [..., K/32]) in plain order, K rounded up
@@ -144,8 +154,9 @@ def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
 
 def mx4_dequantize(q: MX4Tensor,
                    dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """The values that 4-bit rows stand for. bf16 and fp32 hold them all;
-    fp16 rounds, and overflows, where a scale leaves its range."""
+    """The values that 4-bit rows stand for. bf16 and fp32 hold all that
+    ``mx4_quantize`` and ``from_parts`` give; fp16 rounds, and overflows, where a
+    scale leaves its range."""
     dtype = dtype or q.dtype
     if dtype not in _CODE:
         raise TypeError(f'mx4_dequantize: no values of type {dtype}')

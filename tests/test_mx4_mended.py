@@ -385,3 +385,29 @@ def test_serving_says_what_it_serves():
     assert engine('vgg11', 'float').weights == 'float'
     with pytest.raises(ValueError, match='no 1x1'):
         engine('vgg11', 'mx4')
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_values_past_the_range_are_refused(device):
+    """2^128 and more: no product or gradient of them could be right."""
+    grid = torch.tensor([0., .5, 1., 1.5, 2., 3., 4., 6.])
+    for scale in (252, 253, 254, 255):
+        for code in range(8):
+            codes = torch.zeros(3, 64 // 2, dtype=torch.uint8)
+            codes[1, 20] = code << 4 | 8              # and a negative zero
+            scales = torch.full((3, 2), 127, dtype=torch.uint8)
+            scales[1, 1] = scale
+            parts = codes.to(device), scales.to(device)
+            value = float(grid[code]) * 2.0 ** (scale - 127)
+            if scale < 255 and value >= 2.0 ** 128:
+                with pytest.raises(ValueError, match='2\\^128'):
+                    ops.MX4Tensor.from_parts(*parts)
+                continue
+            q = ops.MX4Tensor.from_parts(*parts)
+            for dtype in (torch.float32, torch.bfloat16):
+                got = float(q.dequantize(dtype)[1, 41])
+                assert got == value or scale == 255 and math.isnan(got)
+    empty = torch.zeros(0, 16, dtype=torch.uint8)
+    assert ops.MX4Tensor.from_parts(empty, empty[:, :1]).shape == (0, 32)
+    with pytest.raises(TypeError):
+        ops.MX4Tensor.from_parts(torch.zeros(2, 16), torch.zeros(2, 1))
