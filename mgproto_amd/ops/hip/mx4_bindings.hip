@@ -285,7 +285,8 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_backward(
         int64_t dw_dt, int64_t db_dt, int64_t form) {
     CHECK_VALUE(grad.is_cuda() && grad.dim() >= 1,
                 "mx4_linear: output gradient: rows on the GPU");
-    CHECK_VALUE(form >= -1 && form <= 1, "mx4_linear: no form ", form);
+    CHECK_VALUE(form >= -1 && form < mx4::GRAD_FORMS, "mx4_linear: no form ",
+                form);
     mx4::GradArgs a{};
     a.g_dt = dtype_code(grad, "mx4_linear: output gradient");
     a.N = grad.size(-1), a.M = 1, a.K = K;

@@ -278,8 +278,8 @@ void linear_q(const uint8_t* xc, const uint8_t* xs, long M, long K,
 
 // The gradients that are wanted of the product: dx[M,K] = g[M,N] W[N,K],
 // dw[N,K] = g^T X[M,K], db[N] = sum_m g; none of M, N, K is 0. `aligned`: g starts
-// on 16 bytes. Form 0 is the one of small products, 1 that of large ones, -1
-// chooses.
+// on 16 bytes. Form 0 is the one of small products, 1 that of large ones, 2 to 5 are
+// the same with a certain tile for dx, -1 chooses.
 struct GradArgs {
     const void* g;
     int g_dt;
@@ -289,6 +289,7 @@ struct GradArgs {
     void *dx, *dw, *db;                  // null where not wanted
     int dx_dt, dw_dt, db_dt;
 };
+constexpr int GRAD_FORMS = 6;
 size_t grads_bytes(const GradArgs& a, int form);      // of workspace
 void grads(const GradArgs& a, int form, void* work, hipStream_t stream);
 

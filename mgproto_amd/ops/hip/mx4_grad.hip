@@ -371,11 +371,14 @@ size_t part_bytes(const GradArgs& a, long Np) {
     return (size_t)parts_of(a.g_dt) * a.M * Np * 2;
 }
 
-size_t dx_bytes(const GradArgs& a) {
+// forms from 2 on ask for a tile of the input's gradient
+int tile_of(int form) { return form < 2 ? -1 : form - 2; }
+
+size_t dx_bytes(const GradArgs& a, int tile) {
     const long Np = up32(a.N);
     return up256((size_t)a.K * Np * 2)
         + (dx_in_place(a) || share_parts(a) ? 0 : up256(part_bytes(a, Np)))
-        + grad_input_partial(a.M, a.K, Np / 32 * parts_of(a.g_dt));
+        + grad_input_partial(a.M, a.K, Np / 32 * parts_of(a.g_dt), tile);
 }
 
 size_t dw_bytes(const GradArgs& a) {
@@ -390,7 +393,8 @@ size_t db_bytes(const GradArgs& a) {
 
 // W^T is written once as bf16 (W is small beside g, or the product large).
 // `rows`: parts in rows of up32(N), where there are some.
-void run_dx(const GradArgs& a, const char* rows, char* at, hipStream_t stream) {
+void run_dx(const GradArgs& a, int tile, const char* rows, char* at,
+            hipStream_t stream) {
     const long Np = up32(a.N);
     const int P = parts_of(a.g_dt), per = (int)(Np / 32);
     __bf16* wt = (__bf16*)at;
@@ -401,14 +405,14 @@ void run_dx(const GradArgs& a, const char* rows, char* at, hipStream_t stream) {
     const size_t row = Np * 2;               // = N * 2 where g is read in place
     if (rows || dx_in_place(a)) {
         grad_input_tiles(rows ? rows : a.g, 64, row, a.M * row, P, per, wt, a.M,
-                         a.K, a.dx, a.dx_dt, at, stream);
+                         a.K, a.dx, a.dx_dt, tile, at, stream);
         return;
     }
     char* parts = at;
     at += up256(part_bytes(a, Np));
     launch_parts<true>(a, (int)Np, parts, stream);
     grad_input_tiles(parts, (size_t)a.M * 64, 64, per * (size_t)a.M * 64, P, per,
-                     wt, a.M, a.K, a.dx, a.dx_dt, at, stream);
+                     wt, a.M, a.K, a.dx, a.dx_dt, tile, at, stream);
 }
 
 void run_dw(const GradArgs& a, const char* rows, char* at, hipStream_t stream) {
@@ -466,7 +470,7 @@ size_t grads_bytes(const GradArgs& a, int form) {
     if (form < 0 ? small(a) : form == 0) return 0;
     // one after the other on the stream: the same bytes serve all
     return (share_parts(a) ? up256(part_bytes(a, up32(a.N))) : 0)
-        + std::max({a.dx ? dx_bytes(a) : 0, a.dw ? dw_bytes(a) : 0,
+        + std::max({a.dx ? dx_bytes(a, tile_of(form)) : 0, a.dw ? dw_bytes(a) : 0,
                      a.db ? db_bytes(a) : 0});
 }
 
@@ -492,7 +496,7 @@ void grads(const GradArgs& a, int form, void* work, hipStream_t stream) {
         at += up256(part_bytes(a, up32(a.N)));
         launch_parts<false>(a, (int)up32(a.N), rows, stream);
     }
-    if (a.dx) run_dx(a, rows, at, stream);
+    if (a.dx) run_dx(a, tile_of(form), rows, at, stream);
     if (a.dw) run_dw(a, rows, at, stream);
     if (a.db) run_db(a, at, stream);
 }

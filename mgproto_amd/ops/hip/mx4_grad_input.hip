@@ -174,13 +174,15 @@ void grad_input_kernel(const uint8_t* __restrict__ a, size_t a_step,
 // a step (of all blocks on a unit). 15680x512 (sum 2048): 256 x 256 50 us, 256 x
 // 128 40, 128 x 128 43. Few columns: 256 x 64.
 struct Plan { int bm, bn, slots, splits; };
-Plan plan(long M, long K, long steps) {
-    static const struct { int bm, bn, slots, cycles; } T[] = {
+Plan plan(long M, long K, long steps, int tile) {
+    static const struct { int bm, bn, slots, cycles; } T[TILES] = {
         {256, 256, 256, 1260}, {256, 128, 256, 780}, {128, 128, 512, 1380},
         {256, 64, 512, 1000}};
     Plan p{};
     double best = 0;
-    for (const auto& t : T) {
+    for (int i = 0; i < TILES; ++i) {
+        if (tile >= 0 && i != tile) continue;
+        const auto& t = T[i];
         const long have = ((M + t.bm - 1) / t.bm) * ((K + t.bn - 1) / t.bn);
         const double cost = (double)((have + t.slots - 1) / t.slots) * t.cycles;
         if (p.bm && cost >= best) continue;
@@ -195,16 +197,17 @@ Plan plan(long M, long K, long steps) {
 
 }  // namespace
 
-size_t grad_input_partial(long M, long K, long steps) {
-    const int s = plan(M, K, steps).splits;
+size_t grad_input_partial(long M, long K, long steps, int tile) {
+    const int s = plan(M, K, steps, tile).splits;
     return s > 1 ? up256((size_t)s * M * K * 4) : 0;
 }
 
 void grad_input_tiles(const void* a, size_t a_step, size_t a_row, size_t a_part,
                       int parts, int per, const void* b, long M, long K,
-                      void* c, int dt, void* partial, hipStream_t stream) {
+                      void* c, int dt, int tile, void* partial,
+                      hipStream_t stream) {
     const int steps = per * parts;
-    const Plan p = plan(M, K, steps);
+    const Plan p = plan(M, K, steps, tile);
     const int mt = (int)((M + p.bm - 1) / p.bm), nt = (int)((K + p.bn - 1) / p.bn);
     void* out = p.splits > 1 ? partial : c;
     const int odt = p.splits > 1 ? F32 : dt;
