@@ -77,7 +77,8 @@ def clip_grads_(grads: Union[torch.Tensor, Iterable[torch.Tensor]],
     types (a flat fp32 buffer's views, say); ``grads`` then stay as they were.
     What is written has to be dense and apart from everything else in the
     call. A norm that is NaN makes every element NaN; an infinite one makes
-    the finite elements 0 and the infinite ones NaN."""
+    the finite elements 0 and the infinite ones NaN (all of them NaN where
+    ``max_norm`` is infinite too)."""
     ts = _list(grads)
     outs = ts if out is None else _list(out)
     ext = _ext(ts)
