@@ -185,6 +185,12 @@ def _training(model, dataloader, optimizer=None, aux_criterion=None,
                         (em_runner.run() if em_runner is not None
                          else m.update_GMM())
 
+            # the autograd graph ends with its batch: a capture of a backward
+            # pass fails while an eager graph of the same parameters lives
+            output = x_auxiliary = None
+            loss, cross_entropy = loss.detach(), cross_entropy.detach()
+            mine_loss, aux_loss = mine_loss.detach(), aux_loss.detach()
+
         if print_every and i % print_every == 0 \
                 and (comm is None or comm.rank == 0):
             if timer.enabled:

@@ -411,3 +411,54 @@ def test_values_past_the_range_are_refused(device):
     assert ops.MX4Tensor.from_parts(empty, empty[:, :1]).shape == (0, 32)
     with pytest.raises(TypeError):
         ops.MX4Tensor.from_parts(torch.zeros(2, 16), torch.zeros(2, 1))
+
+
+def test_no_eager_graph_lives_when_a_step_is_captured():
+    """A small batch runs eagerly, the next one may be captured: nothing of
+    the first one's autograd graph is left then."""
+    import gc
+    import types
+    import weakref
+    from mgproto_amd.engine import trainer
+    alive = []
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.lin = torch.nn.Linear(3, 4)
+            self.iteration_counter = torch.zeros(1)
+            self.queue = types.SimpleNamespace(mem_len=torch.zeros(4))
+            self.capacity_pc = torch.ones(4)
+            self.update_interval = 1
+
+        def forward(self, x, gt):
+            y = self.lin(x)
+            mark = y.grad_fn.metadata['mark'] = type('Mark', (), {})()
+            alive.append(weakref.ref(mark))       # as long as the node
+            return y[:, :, None].expand(-1, -1, 3) * 1.0, y * 2.0
+
+    class Step:
+        clip_grad_norm = None
+        seen = 0
+
+        def matches(self, image, *_):
+            return len(image) == 4
+
+        def step(self, *_, **__):
+            gc.collect()
+            assert alive and all(r() is None for r in alive)
+            self.seen += 1
+            z = torch.zeros(())
+            return dict.fromkeys(('loss', 'ce', 'mine', 'aux', 'n_correct',
+                                  'grad_norm'), z)
+
+    net, step = Net(), Step()
+    opt = torch.optim.SGD(net.parameters(), lr=0.1)
+    batches = [(torch.randn(n, 3), torch.randint(0, 4, (n,)))
+               for n in (2, 4, 3, 4)]
+    trainer._training(net, batches, optimizer=opt, use_mine=True,
+                      aux_criterion=lambda x, t: x.square().mean(),
+                      coefs={'crs_ent': 1.0, 'mine': 0.2, 'aux': 0.5},
+                      device=torch.device('cpu'), amp_dtype=None,
+                      graph_step=step, log=lambda *_: None, print_every=1)
+    assert step.seen == 2 and len(alive) == 2
