@@ -11,6 +11,8 @@ reference's driver and bench were one program, reference main.py:234-287).
 
 Capture constraints and how they are met:
 
+* no eager autograd graph of the same parameters is alive — steps stay
+  eager while one is;
 * static shapes — replay only when the incoming batch is full-size;
   remainder batches fall back to the eager path (the caller checks
   ``matches()``);
@@ -44,7 +46,7 @@ import torch
 import torch.nn.functional as F
 
 from ..models.conv1x1 import GemmConv2d
-from ..utils.graphs import capture_graph
+from ..utils.graphs import capture_graph, eager_graph_of
 
 
 def graphs_enabled(device, world: int = 1) -> bool:
@@ -88,6 +90,7 @@ class GraphedStep:
         self.broken = False          # capture failed -> permanent eager
         self._sig = None
         self._warm_count = 0
+        self._said = False
 
         self.static_img = torch.zeros(batch_size, 3, img_size, img_size,
                                       device=device)
@@ -182,7 +185,15 @@ class GraphedStep:
         self.static_tgt.copy_(target, non_blocking=True)
 
         if self.graph is None:
-            if self._warm_count < self.warmup_steps:
+            wait = self._warm_count >= self.warmup_steps and eager_graph_of(
+                [*self.model.parameters(), *(p for g in optimizer.param_groups
+                                             for p in g['params'])])
+            if wait and not self._said:
+                self._said = True
+                print('# hipGraph capture waits: an eager autograd graph of '
+                      'these parameters is alive (a loss or output that '
+                      'someone keeps)', flush=True)
+            if wait or self._warm_count < self.warmup_steps:
                 # real training steps, staged on a side stream so the
                 # allocations warm the capture pool
                 side = torch.cuda.Stream()

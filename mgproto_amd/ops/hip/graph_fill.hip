@@ -14,6 +14,7 @@
 #include <c10/core/Device.h>
 #include <c10/hip/HIPException.h>
 #include <hip/hip_runtime.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <vector>
@@ -103,9 +104,19 @@ int64_t graph_fill_nodes(uint64_t raw) {
     return count;
 }
 
+// Whether an autograd graph that ends in one of the tensors is alive.
+bool grad_graph_alive(const std::vector<at::Tensor>& leaves) {
+    return std::any_of(leaves.begin(), leaves.end(), [](const at::Tensor& t) {
+        return t.is_leaf() && t.requires_grad() &&
+               torch::autograd::impl::try_get_grad_accumulator(t) != nullptr;
+    });
+}
+
 }  // namespace
 
 void register_graph(pybind11::module& m) {
     m.def("graph_fill_nodes", &graph_fill_nodes,
           "memset nodes of a captured graph to fill kernels; how many");
+    m.def("grad_graph_alive", &grad_graph_alive,
+          "whether an autograd graph that ends in one of the tensors is alive");
 }

@@ -207,3 +207,43 @@ def test_captured_training_step_of_all_convolutions(mx4):
         assert float(ops.grad_norm(moved)) == pytest.approx(
             lr * min(norm, clip), rel=1e-4, abs=2 * slack)
         _other_work()
+
+
+def test_no_capture_while_an_eager_graph_lives(capsys):
+    """Steps stay eager, and train, until the last output of an eager forward
+    is dropped."""
+    from mgproto_amd.engine.graphstep import GraphedStep
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.conv = torch.nn.Conv2d(3, 5, 8)
+
+        def forward(self, x, gt):
+            y = self.conv(x).flatten(1)
+            return y[:, :, None], y
+
+    net = Net().cuda()
+    opt = torch.optim.SGD(net.parameters(), lr=1e-3)
+    gs = GraphedStep(net, None, {'crs_ent': 1.0, 'mine': 0.0, 'aux': 0.0},
+                     torch.device('cuda', 0), 4, 8, amp_dtype=None,
+                     warmup_steps=1)
+    x = torch.randn(4, 3, 8, 8, device='cuda')
+    t = torch.randint(0, 5, (4,), device='cuda')
+    kept = [net(x, t)[0]]
+    kept.append(kept)                         # a cycle
+    losses = []
+
+    def step():
+        assert gs.matches(x, opt, False, False)
+        losses.append(float(gs.step(x, t, opt)['ce']))
+
+    for _ in range(3):
+        step()
+        assert gs.graph is None and not gs.broken
+    assert capsys.readouterr().out.count('capture waits') == 1
+    del kept
+    for _ in range(3):
+        step()
+        assert gs.graph is not None
+    assert losses == sorted(losses, reverse=True) and len(set(losses)) == 6

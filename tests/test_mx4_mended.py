@@ -462,3 +462,22 @@ def test_no_eager_graph_lives_when_a_step_is_captured():
                       device=torch.device('cpu'), amp_dtype=None,
                       graph_step=step, log=lambda *_: None, print_every=1)
     assert step.seen == 2 and len(alive) == 2
+
+
+def test_living_graphs_are_seen():
+    from mgproto_amd.utils.graphs import eager_graph_of
+    if not ops.native_available():
+        pytest.skip('needs the extension')
+    a, b = (torch.randn(3, requires_grad=True) for _ in range(2))
+    c = torch.randn(3)
+    assert not eager_graph_of([a, b, c])
+    y = (a * 2).sum()
+    assert eager_graph_of([b, a]) and not eager_graph_of([b, c])
+    y.backward()
+    assert eager_graph_of([a])                # freed tensors, living nodes
+    y = y.detach()
+    assert not eager_graph_of([a])
+    kept = [(b + 1)]
+    kept.append(kept)
+    del kept
+    assert not eager_graph_of([b])            # a cycle is collected
