@@ -143,10 +143,11 @@ def use_mx4(module: nn.Module, train: bool = False) -> int:
 
     ``train=False`` rounds the weights now and holds them in 4 bits, for
     inference. The forward that follows an update of a weight (an optimizer's,
-    ``load_state_dict``'s, another parameter in its place) rounds it again; an
-    update through ``.data`` is not seen, nor is any by the replay of a captured
-    graph, until ``use_mx4`` is called again, which writes the new codes in the
-    place of the old ones.
+    ``load_state_dict``'s, another parameter in its place) rounds it again.
+    Updates that leave no trace, through ``.data`` or by a replayed training
+    step, are not seen, and the replay of a captured forward sees none, until
+    ``use_mx4`` is called again, which writes the new codes in the place of the
+    old ones.
     ``train=True`` rounds them in every forward, with straight-through
     gradients to the float weights: fine-tuning for the former. The state dict
     stays what it was either way. ``use_mx4(model.features)`` leaves the
