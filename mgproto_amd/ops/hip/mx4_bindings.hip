@@ -379,7 +379,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
         {
             at::AutoGradMode off(false);
             const auto [dx, dw, db] = linear_backward(
-                grads[0], t[0], t[1], t[2], t[3],
+                grads[0].resolve_neg(), t[0], t[1], t[2], t[3],
                 ctx->saved_data["K"].toInt(), types[0], types[1], types[2], -1);
             out[0] = dx.value_or(Tensor());
             out[1] = dw.value_or(Tensor());

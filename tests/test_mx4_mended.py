@@ -481,3 +481,15 @@ def test_living_graphs_are_seen():
     kept.append(kept)
     del kept
     assert not eager_graph_of([b])            # a cycle is collected
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_an_output_gradient_that_stands_for_its_negative(device):
+    x = torch.randn(5, 40, device=device, requires_grad=True)
+    w = torch.randn(7, 40, device=device, requires_grad=True)
+    g = torch.randn(5, 7, device=device)
+    neg = torch.complex(g, g).conj().imag
+    assert neg.is_neg()
+    got = torch.autograd.grad(ops.mx4_linear(x, w), (x, w), neg)
+    want = torch.autograd.grad(ops.mx4_linear(x, w), (x, w), -g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
